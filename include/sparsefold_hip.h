@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define SF_HIP_ABI_VERSION 11
+#define SF_HIP_ABI_VERSION 12
 
 /* ABI version of the loaded library (== SF_HIP_ABI_VERSION it was built with). */
 int sf_hip_abi_version(void);
@@ -469,6 +469,71 @@ typedef struct sf_diffusion_conditioning_args {
 size_t sf_hip_diffusion_conditioning_workspace_bytes(const sf_diffusion_conditioning_args* a);
 int sf_hip_diffusion_conditioning_fwd(const sf_diffusion_conditioning_args* a, void* workspace,
                                       size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Packed sequences of different lengths (no counterpart in the reference).
+ * Element types of these entry points.
+ * ------------------------------------------------------------------------------------- */
+#define SF_DTYPE_BF16 0
+#define SF_DTYPE_F16 1
+#define SF_DTYPE_F32 2
+
+/* Attention over packed sequences, grouped heads, optionally causal:
+ *   out[i,h,:] = sum_j softmax_j(scale * q[i,h,:].k[j,h/G,:]) v[j,h/G,:],  G = H / Hkv
+ * Sequence b's queries are rows cu_q[b] .. cu_q[b+1] - 1 of q and out, its keys rows cu_k[b] ..
+ * cu_k[b+1] - 1 of k and v; with len_q / len_k (or NULL) only the first len[b] of them are in use (a
+ * padded batch, a cache with free rows).  A query sees every key of its sequence; with causal != 0
+ * query i of n sees keys j <= i + m - n of m (the last query sees all).  A query without a key gives
+ * zeros; rows of out outside every sequence are left as they were.  What a key holds that a query
+ * does not see, and what rows behind a sequence's end hold, NaN and infinities included, has no
+ * influence on its result.  Offsets are clamped to the tensors: wrong ones give wrong results, no
+ * access outside them.
+ * bf16 or f16, last dimension contiguous, 16-byte aligned rows (strides multiples of 8); D % 8 == 0,
+ * D <= 128; k_s[0], v_s[0] in [D, 2^24).  fp32 softmax and accumulation; the weights are rounded to
+ * the element type for the product with v.  out may not overlap q, k or v. */
+typedef struct sf_packed_attention_args {
+  int32_t B, H, Hkv, D;
+  int64_t Tq, Tk;                               /* rows of q / out and of k / v */
+  float scale;
+  int32_t causal, dtype;                        /* SF_DTYPE_BF16 or SF_DTYPE_F16 */
+  const void* q; int64_t q_s[2];                /* strides [row, head], elements */
+  const void* k; int64_t k_s[2];
+  const void* v; int64_t v_s[2];
+  void* out;     int64_t o_s[2];
+  const int32_t* cu_q; const int32_t* cu_k;     /* [B + 1] */
+  const int32_t* len_q; const int32_t* len_k;   /* [B] or NULL */
+} sf_packed_attention_args;
+
+/* 0 where the call needs no workspace (or the arguments are refused). */
+size_t sf_hip_packed_attention_workspace_bytes(const sf_packed_attention_args* a);
+int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions of query and key heads, with an optional norm of each head before them:
+ *   x' = x | x rsqrt(mean x^2 + eps) weight | (x - mean x) rsqrt(var x + eps) weight + bias   (norm)
+ *   pairs (i, i + R/2), or (2i, 2i + 1) when interleaved, i < R/2, turned by positions[t] * freqs[i]
+ *   radians and multiplied by `magnitude`; dims R .. D - 1 keep x'.
+ * The angle is formed and reduced in 64 bits, the rest is fp32, rounded once.  q [T, H, D] and
+ * k [T, Hk, D] (Hk = 0: none) share token positions; the last dimension is contiguous.  q_out may be q
+ * and k_out may be k (same strides); otherwise outputs overlap no input.  D <= 256, R even, 2 <= R <= D.
+ * Weights and biases f32 [D] or NULL (1 and 0), read only where norm asks for them. */
+#define SF_NORM_NONE 0
+#define SF_NORM_RMS 1
+#define SF_NORM_LAYER 2
+typedef struct sf_rotary_args {
+  int64_t T; int32_t H, Hk, D, R;
+  int32_t interleaved, dtype, norm;             /* SF_DTYPE_*, SF_NORM_* */
+  float eps, magnitude;
+  const void* q; int64_t q_s[2];                /* strides [token, head], elements */
+  const void* k; int64_t k_s[2];
+  void* q_out;   int64_t qo_s[2];
+  void* k_out;   int64_t ko_s[2];
+  const void* positions; int32_t positions_64;  /* int32, or int64 when positions_64, [T] */
+  const double* freqs;                          /* [R / 2] radians per position */
+  const float* q_weight; const float* q_bias;
+  const float* k_weight; const float* k_bias;
+} sf_rotary_args;
+
+int sf_hip_rotary_fwd(const sf_rotary_args* a, void* stream);
 
 #ifdef __cplusplus
 }

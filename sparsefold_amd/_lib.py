@@ -10,8 +10,10 @@ import ctypes as C
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libsparsefold_hip.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 TRI_STAGE_PROJECT, TRI_STAGE_ATTEND, TRI_STAGE_OUTPUT, TRI_STAGE_ALL, TRI_STAGE_FUSE = 1, 2, 4, 7, 8
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2   # SF_DTYPE_*
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2    # SF_NORM_*
 NOALLOC_SCRATCH_BYTES = 64 << 20           # SF_HIP_NOALLOC_SCRATCH_BYTES
 
 _i32, _i64, _f32, _vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
@@ -155,6 +157,27 @@ class TriangleMultArgs(C.Structure):
   ]
 
 
+class PackedAttentionArgs(C.Structure):
+  _fields_ = [
+      ("B", _i32), ("H", _i32), ("Hkv", _i32), ("D", _i32), ("Tq", _i64), ("Tk", _i64),
+      ("scale", _f32), ("causal", _i32), ("dtype", _i32),
+      ("q", _vp), ("q_s", _i64 * 2), ("k", _vp), ("k_s", _i64 * 2), ("v", _vp), ("v_s", _i64 * 2),
+      ("out", _vp), ("o_s", _i64 * 2),
+      ("cu_q", _vp), ("cu_k", _vp), ("len_q", _vp), ("len_k", _vp),
+  ]
+
+
+class RotaryArgs(C.Structure):
+  _fields_ = [
+      ("T", _i64), ("H", _i32), ("Hk", _i32), ("D", _i32), ("R", _i32),
+      ("interleaved", _i32), ("dtype", _i32), ("norm", _i32), ("eps", _f32), ("magnitude", _f32),
+      ("q", _vp), ("q_s", _i64 * 2), ("k", _vp), ("k_s", _i64 * 2),
+      ("q_out", _vp), ("qo_s", _i64 * 2), ("k_out", _vp), ("ko_s", _i64 * 2),
+      ("positions", _vp), ("positions_64", _i32), ("freqs", _vp),
+      ("q_weight", _vp), ("q_bias", _vp), ("k_weight", _vp), ("k_bias", _vp),
+  ]
+
+
 STRUCTS = {
     "sf_attention_args": AttentionArgs,
     "sf_layer_norm_args": LayerNormArgs,
@@ -168,6 +191,8 @@ STRUCTS = {
     "sf_diffusion_conditioning_args": DiffusionConditioningArgs,
     "sf_triangle_mult_args": TriangleMultArgs,
     "sf_transition_args": TransitionArgs,
+    "sf_packed_attention_args": PackedAttentionArgs,
+    "sf_rotary_args": RotaryArgs,
 }
 
 # (name, restype, argtypes) of every exported entry point.
@@ -196,6 +221,9 @@ SIGNATURES = [
     ("sf_hip_transition_fwd", C.c_int, [C.POINTER(TransitionArgs), _vp, C.c_size_t, _vp]),
     ("sf_hip_triangle_mult_workspace_bytes", C.c_size_t, [_i32, _i32]),
     ("sf_hip_triangle_mult_fwd", C.c_int, [C.POINTER(TriangleMultArgs), _vp, C.c_size_t, _vp]),
+    ("sf_hip_packed_attention_workspace_bytes", C.c_size_t, [C.POINTER(PackedAttentionArgs)]),
+    ("sf_hip_packed_attention_fwd", C.c_int, [C.POINTER(PackedAttentionArgs), _vp, C.c_size_t, _vp]),
+    ("sf_hip_rotary_fwd", C.c_int, [C.POINTER(RotaryArgs), _vp]),
 ]
 
 _lib: C.CDLL | None = None

@@ -582,3 +582,294 @@ def triangle_multiplication(z: torch.Tensor, mask, w: dict, *, incoming: bool, a
   ws = torch.empty(ws_bytes, dtype=torch.uint8, device=z.device)
   _lib.check(lib.sf_hip_triangle_mult_fwd(C.byref(a), _vp(ws), ws.numel(), _stream(z)), "sf_hip_triangle_mult_fwd")
   return out.to(z.dtype) if z.dtype != torch.bfloat16 else out
+
+
+# ---------------------------------------------------------------------------------------
+# packed sequences: attention, rotary positions, norm of queries and keys with the rotation
+# (sf_hip_packed_attention_fwd, sf_hip_rotary_fwd)
+# ---------------------------------------------------------------------------------------
+
+_ELEMENT_TYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+
+
+def _no_grad(what: str, *ts) -> None:
+  """These calls have no backward pass: a tensor that expects a gradient through them is refused."""
+  if torch.is_grad_enabled():
+    for t in ts:
+      if t is not None and t.requires_grad:
+        raise ValueError(f"{what}: has no backward pass; detach the inputs or call it under torch.no_grad()")
+
+
+def _on_device(t: torch.Tensor):
+  """Context that makes t's device current for a launch (None where it is already)."""
+  return None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
+
+
+def _launch(fn, t: torch.Tensor, what: str, *args) -> None:
+  ctx = _on_device(t)
+  if ctx is None:
+    _lib.check(fn(*args, _stream(t)), what)
+  else:
+    with ctx:
+      _lib.check(fn(*args, _stream(t)), what)
+
+
+def _strides2(t: torch.Tensor) -> tuple[int, int]:
+  """Row and head strides of ``[T, H, D]``; those of a single row or head, which torch leaves
+  arbitrary, as if packed."""
+  T, H, D = t.shape
+  sh = t.stride(1) if H > 1 else D
+  return (t.stride(0) if T > 1 else max(H * sh, H * D)), sh
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int, int]:
+  """First byte, row stride and bytes of one row of ``[T, H, D]``."""
+  st, sh = _strides2(t)
+  return t.data_ptr(), st * t.element_size(), ((t.shape[1] - 1) * sh + t.shape[2]) * t.element_size()
+
+
+def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
+  """Whether two ``[T, H, D]`` views share no element: separate ranges, or separate columns of rows
+  of one width."""
+  if a.numel() == 0 or b.numel() == 0:
+    return True
+  (pa, sa, ea), (pb, sb, eb) = _extent(a), _extent(b)
+  if pa + (a.shape[0] - 1) * sa + ea <= pb or pb + (b.shape[0] - 1) * sb + eb <= pa:
+    return True
+  return sa == sb and ea <= sa and eb <= sa and eb <= (pa - pb) % sa <= sa - ea
+
+
+def _offsets32(t: torch.Tensor, name: str, n: int | None, what: str) -> torch.Tensor:
+  if t.dtype != torch.int32 or t.ndim != 1 or (n is not None and t.numel() != n):
+    raise ValueError(f"{what}: {name} must be int32 [{'sequences + 1' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
+  return t if t.is_contiguous() else t.contiguous()
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, *, len_q: torch.Tensor | None = None,
+                     len_k: torch.Tensor | None = None, causal: bool = False, scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+  """Attention over packed sequences of different lengths; returns ``out`` like ``q``.
+
+  ``q`` ``[Tq, H, D]``, ``k`` and ``v`` ``[Tk, Hkv, D]``, bf16 or fp16 (one type), ``H`` a multiple of
+  ``Hkv``: query head h reads key head ``h // (H // Hkv)``.  ``D`` a multiple of 8 up to 128.  Any row
+  and head strides (columns of a fused projection, a cache); what is not in 16-byte aligned rows is
+  copied first.
+
+  ``cu_q`` int32 ``[B + 1]`` on the device: sequence b has the query rows ``cu_q[b] .. cu_q[b+1] - 1``;
+  ``cu_k`` the same for its keys (None: the queries' offsets, and their ``len_q``).  ``len_q`` /
+  ``len_k`` int32 ``[B]``: only that many rows of each are in use (a padded batch, a cache with free
+  rows).  With ``causal``, query i of n sees keys ``j <= i + m - n`` of m: the last query sees all, so a
+  new token or the rest of a prompt attends to a cache.  A query without a key gives zeros.  Rows
+  of ``out`` outside every sequence are left as they were: undefined unless ``out`` is given.
+
+  The offsets are read on the device only: the call neither synchronises nor copies them, and can
+  be captured.  They must not decrease; wrong ones give wrong results but no access outside the
+  tensors.  ``out`` may not overlap an input."""
+  what = "packed_attention"
+  _no_grad(what, q, k, v)
+  dev = _require_cuda(q, k, v, cu_q, cu_k, len_q, len_k, out)
+  _require(q.ndim == 3 and k.ndim == 3 and v.ndim == 3, "packed_attention: q, k and v must be [tokens, heads, dim]")
+  Tq, H, D = q.shape
+  Tk, Hkv = k.shape[0], k.shape[1]
+  if k.shape[2] != D or v.shape != k.shape:
+    raise ValueError(f"packed_attention: shapes q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+  if H == 0 or Hkv == 0 or H % Hkv != 0:
+    raise ValueError(f"packed_attention: {H} query heads do not share {Hkv} key heads evenly")
+  if D % 8 != 0 or not 0 < D <= 128:
+    raise ValueError(f"packed_attention: head dim {D} is not a multiple of 8 up to 128")
+  dtype = q.dtype
+  if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
+    raise ValueError(f"packed_attention: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
+  cu_q = _offsets32(cu_q, "cu_q", None, what)
+  B = cu_q.numel() - 1
+  _require(B >= 1, "packed_attention: cu_q needs at least two offsets")
+  if cu_k is None:
+    cu_k, len_k = cu_q, (len_q if len_k is None else len_k)
+  else:
+    cu_k = _offsets32(cu_k, "cu_k", B + 1, what)
+  if len_q is not None:
+    len_q = _offsets32(len_q, "len_q", B, what)
+  if len_k is not None:
+    len_k = _offsets32(len_k, "len_k", B, what)
+  scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+  _require(abs(scale) <= 1e30, f"packed_attention: scale {scale} is not finite or above 1e30")
+
+  def rows(t, keys):
+    st, sh = _strides2(t)
+    if t.stride(2) != 1 or st % 8 or sh % 8 or t.data_ptr() % 16 or (keys and not D <= st < 1 << 24):
+      t = torch.empty(t.shape, dtype=dtype, device=dev).copy_(t)
+      st, sh = t.shape[1] * D, D
+    return t, (st, sh)
+
+  if out is None:
+    out = torch.empty((Tq, H, D), dtype=dtype, device=dev)
+    so = (H * D, D)
+  else:
+    so = _strides2(out) if out.ndim == 3 else (0, 0)
+    if tuple(out.shape) != (Tq, H, D) or out.dtype != dtype or out.stride(2) != 1 or so[0] % 8 or so[1] % 8 or out.data_ptr() % 16:
+      raise ValueError(f"packed_attention: out must be {dtype} {(Tq, H, D)} in 16-byte aligned rows")
+    if not (_disjoint(out, q) and _disjoint(out, k) and _disjoint(out, v)):
+      raise ValueError("packed_attention: out overlaps an input")
+  a = _lib.PackedAttentionArgs()
+  a.B, a.H, a.Hkv, a.D, a.Tq, a.Tk = B, H, Hkv, D, Tq, Tk
+  a.scale, a.causal, a.dtype = scale, int(bool(causal)), _ELEMENT_TYPES[dtype]
+  q, (a.q_s[0], a.q_s[1]) = rows(q, False)
+  k, (a.k_s[0], a.k_s[1]) = rows(k, True)
+  v, (a.v_s[0], a.v_s[1]) = rows(v, True)
+  a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+  a.o_s[0], a.o_s[1] = so
+  a.cu_q, a.cu_k, a.len_q, a.len_k = cu_q.data_ptr(), cu_k.data_ptr(), _vp(len_q), _vp(len_k)
+  lib = _lib.load()
+  ref = C.byref(a)
+  need = lib.sf_hip_packed_attention_workspace_bytes(ref)
+  ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+  _launch(lib.sf_hip_packed_attention_fwd, q, "sf_hip_packed_attention_fwd", ref, _vp(ws), need)
+  return out
+
+
+def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int | None = None, low_turns: float = 1.0, high_turns: float = 32.0,
+                       device=None) -> torch.Tensor:
+  """Radians per position of the ``rotary_dim / 2`` pairs, float64: ``base ** (-2 i / rotary_dim)``,
+  stretched for contexts ``factor`` times longer than the trained ones where ``scaling`` says how:
+
+  * ``"linear"``  every frequency divided by ``factor`` (positions interpolated);
+  * ``"base"``    ``base`` raised so that the slowest pair is divided by ``factor`` and the fastest stays;
+  * ``"turns"``   by the turns that a pair makes over ``original_length`` positions: from
+    ``high_turns`` on it stays, up to ``low_turns`` it is divided by ``factor``, between them linearly blended.
+
+  A set-up step on the host; a program keeps the tensor."""
+  _require(rotary_dim >= 2 and rotary_dim % 2 == 0, f"rotary_frequencies: rotary_dim {rotary_dim} is not even and positive")
+  _require(base > 0 and factor > 0, "rotary_frequencies: base and factor must be positive")
+  exponents = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+  if scaling == "base":
+    _require(rotary_dim > 2, "rotary_frequencies: scaling 'base' needs at least two pairs")
+    base = base * factor ** (rotary_dim / (rotary_dim - 2))
+  freqs = float(base) ** -exponents
+  if scaling == "linear":
+    freqs = freqs / factor
+  elif scaling == "turns":
+    _require(original_length is not None and original_length > 0 and high_turns > low_turns,
+             "rotary_frequencies: scaling 'turns' needs original_length > 0 and high_turns > low_turns")
+    keep = ((original_length * freqs / (2.0 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+    freqs = freqs * (keep + (1.0 - keep) / factor)
+  else:
+    _require(scaling in (None, "base"), f"rotary_frequencies: scaling {scaling!r} is not None, 'linear', 'base' or 'turns'")
+  return freqs.to(device) if device is not None else freqs
+
+
+def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, norm=0, eps=0.0, weights=(None,) * 4):
+  _no_grad(what, q, k, freqs, *weights)
+  dev = _require_cuda(q, k, positions, freqs, out_q, out_k, *weights)
+  if q.ndim < 3 or (k is not None and (k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+    raise ValueError(f"{what}: q must be [..., H, D] and k [..., Hk, D], got {tuple(q.shape)}"
+                     f"{'' if k is None else ' and ' + str(tuple(k.shape))}")
+  lead, H, D = q.shape[:-2], q.shape[-2], q.shape[-1]
+  dtype = q.dtype
+  if dtype not in _ELEMENT_TYPES or (k is not None and k.dtype != dtype):
+    raise ValueError(f"{what}: q and k must be bfloat16, float16 or float32 alike, got {dtype}{'' if k is None else f' and {k.dtype}'}")
+  if H == 0 or (k is not None and k.shape[-2] == 0) or not 0 < D <= 256:
+    raise ValueError(f"{what}: heads must be there and head dims lie in 1 .. 256, got {tuple(q.shape)}")
+  if freqs.dtype != torch.float64 or freqs.ndim != 1 or not 1 <= freqs.numel() <= D // 2:
+    raise ValueError(f"{what}: freqs must be float64 [R / 2], 1 to {D // 2} of them, got {freqs.dtype} {tuple(freqs.shape)}")
+  if positions.dtype not in (torch.int32, torch.int64):
+    raise ValueError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
+  if positions.shape != lead:
+    try:
+      positions = positions.expand(lead)
+    except RuntimeError:
+      raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit tokens {tuple(lead)}") from None
+  if not math.isfinite(magnitude):
+    raise ValueError(f"{what}: magnitude {magnitude} is not finite")
+
+  def three(t):
+    t3 = t if t.ndim == 3 else t.reshape(-1, t.shape[-2], D)
+    return t3 if t3.stride(2) == 1 or D == 1 else t3.contiguous()
+
+  def result(given, like, name):
+    if given is None:
+      o = torch.empty(like.shape, dtype=dtype, device=dev)
+      return o, three(o)
+    if given.shape != like.shape or given.dtype != dtype or (given.stride(-1) != 1 and D > 1):
+      raise ValueError(f"{what}: {name} must be {dtype} {tuple(like.shape)} with a unit last stride")
+    try:
+      return given, given if given.ndim == 3 else given.view(-1, given.shape[-2], D)
+    except RuntimeError:
+      raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
+
+  q3 = three(q)
+  k3 = None if k is None else three(k)
+  oq, oq3 = result(out_q, q, "out_q")
+  ok = ok3 = None
+  if k is not None:
+    ok, ok3 = result(out_k, k, "out_k")
+  elif out_k is not None:
+    raise ValueError(f"{what}: out_k without k")
+  if out_q is not None or out_k is not None:
+    same = lambda a, b: a.data_ptr() == b.data_ptr() and _strides2(a) == _strides2(b) and a.shape == b.shape
+    pairs = [(oq3, q3, True)]
+    if k is not None:
+      pairs += [(ok3, k3, True), (oq3, k3, False), (ok3, q3, False), (oq3, ok3, False)]
+    for a, b, own in pairs:
+      if not (_disjoint(a, b) or (own and same(a, b))):
+        raise ValueError(f"{what}: outputs may be their own input in place, and overlap nothing else")
+  a = _lib.RotaryArgs()
+  a.T, a.H, a.Hk, a.D, a.R = q3.shape[0], H, 0 if k is None else k.shape[-2], D, 2 * freqs.numel()
+  a.interleaved, a.dtype, a.norm = int(bool(interleaved)), _ELEMENT_TYPES[dtype], norm
+  a.eps, a.magnitude = eps, magnitude
+  positions = positions if positions.ndim == 1 and positions.is_contiguous() else positions.reshape(-1).contiguous()
+  freqs = freqs.contiguous()
+  a.q, a.q_out = q3.data_ptr(), oq3.data_ptr()
+  a.q_s[0], a.q_s[1] = _strides2(q3)
+  a.qo_s[0], a.qo_s[1] = _strides2(oq3)
+  if k is not None:
+    a.k, a.k_out = k3.data_ptr(), ok3.data_ptr()
+    a.k_s[0], a.k_s[1] = _strides2(k3)
+    a.ko_s[0], a.ko_s[1] = _strides2(ok3)
+  a.positions, a.positions_64, a.freqs = positions.data_ptr(), int(positions.dtype == torch.int64), freqs.data_ptr()
+  a.q_weight, a.k_weight, a.q_bias, a.k_bias = (_vp(w) for w in weights)
+  _launch(_lib.load().sf_hip_rotary_fwd, q3, "sf_hip_rotary_fwd", C.byref(a))
+  return oq, ok
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor, *,
+           interleaved: bool = False, magnitude: float = 1.0, out_q: torch.Tensor | None = None,
+           out_k: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+  """Rotary positions of ``q`` ``[..., H, D]`` and ``k`` ``[..., Hk, D]`` (or None); returns both turned.
+
+  The first ``R = 2 * len(freqs)`` dims of each head are turned in pairs, ``(i, i + R/2)`` or with
+  ``interleaved`` ``(2i, 2i + 1)``, by ``positions * freqs[i]`` radians and multiplied by ``magnitude``; the
+  others are copied.  ``positions`` int32 or int64 of the tokens' leading dims (broadcast where they are
+  fewer), ``freqs`` float64 on the device (``rotary_frequencies``).  bf16, fp16 or float32, head dims up
+  to 256, any strides with a unit last one.  The angle is formed in 64 bits, the rest in 32, rounded
+  once.  ``out_q`` may be ``q`` and ``out_k`` may be ``k`` (in place); they overlap nothing else."""
+  return _rotary("rotary", q, k, positions, freqs, interleaved, magnitude, out_q, out_k)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                   positions: torch.Tensor, freqs: torch.Tensor, *, norm: str = "rms", eps: float = 1e-6,
+                   q_bias: torch.Tensor | None = None, k_bias: torch.Tensor | None = None, interleaved: bool = False,
+                   magnitude: float = 1.0, out_q: torch.Tensor | None = None,
+                   out_k: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+  """Norm of each query and key head, then their rotary positions, in one pass; arguments and results
+  as ``rotary``.  ``norm`` ``"rms"``: ``x rsqrt(mean x^2 + eps) weight``; ``"layer"``:
+  ``(x - mean) rsqrt(var + eps) weight + bias``, over the D dims of a head.  Weights and biases ``[D]``
+  (None: 1 and 0; biases with ``"layer"`` only)."""
+  what = "qk_norm_rotary"
+  if norm not in _NORMS:
+    raise ValueError(f"{what}: norm {norm!r} is not 'rms' or 'layer'")
+  if norm == "rms" and (q_bias is not None or k_bias is not None):
+    raise ValueError(f"{what}: biases need norm='layer'")
+  if k is None and (k_weight is not None or k_bias is not None):
+    raise ValueError(f"{what}: a key weight or bias without k")
+  if not 0.0 <= eps < math.inf:
+    raise ValueError(f"{what}: eps {eps} is not finite and >= 0")
+  weights = (q_weight, k_weight, q_bias, k_bias)
+  for w in weights:
+    if w is not None and tuple(w.shape) != (q.shape[-1],):
+      raise ValueError(f"{what}: weights and biases must be [{q.shape[-1]}], got {tuple(w.shape)}")
+  _no_grad(what, *weights)
+  return _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, _NORMS[norm], float(eps),
+                 tuple(_f32(w) for w in weights))

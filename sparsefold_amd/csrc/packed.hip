@@ -1,0 +1,734 @@
+// Attention over packed sequences of different lengths, grouped heads, optionally causal.
+//
+//   o[i, h] = sum_j p_ij v[j, h / G] / sum_j p_ij,   p_ij = exp(scale q[i, h] . k[j, h / G] - m_i)
+//
+// over the keys j that query i of its sequence sees: all of them, or with `causal` those up to
+// i + (keys - queries), so that the last query sees every key whatever the cache holds before the
+// first one.  A query that sees no key gives zeros.
+//
+// A sequence's queries and the G heads that share a key head are one list of rows, token-major:
+// row r is token r / G, head r % G of the group.  So the rows of a tile share their keys whatever G
+// is, and a single new token still fills G rows of a matrix instruction.
+//
+// Two kernels over those rows, joined by a third where the keys are split:
+//   packed_tile_kernel    workgroups of many rows: K and V tiles of 64 keys shared through LDS
+//   packed_stream_kernel  32 rows: each wave streams its own slice of the keys
+//   packed_combine_kernel joins the slices of different workgroups
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
+#include "sf_common.h"
+
+namespace {
+
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef short v4i16p __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16p lds_v4i16p;
+
+// 16-bit element types: the matrix product, rounding of two weights to one word, their sum.
+struct Bf16 {
+  // a tile whose weights sum to more moves the reference point (2^60: weights far below bf16's largest)
+  static constexpr float kMassLimit = 1.152921504606846976e18f;
+  static constexpr float kHuge = 0x1p28f;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return __builtin_bit_cast(uint32_t, cvt_bf2(lo, hi)); }
+  static __device__ __forceinline__ float sum2(uint32_t w, float acc) { return add_bf2(__builtin_bit_cast(bf16x2, w), acc); }
+  static __device__ __forceinline__ float to_float(uint16_t v) { return bf2f(v); }
+  static __device__ __forceinline__ uint16_t from_float(float v) { return f2bf(v); }
+};
+struct Fp16 {
+  // 2^12: every weight stays finite in fp16
+  static constexpr float kMassLimit = 4096.f;
+  static constexpr float kHuge = 0x1p24f;
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, f16x2));
+  }
+  static __device__ __forceinline__ float sum2(uint32_t w, float acc) {
+    const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), one, acc, false);
+  }
+  static __device__ __forceinline__ float to_float(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+  static __device__ __forceinline__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+};
+
+// A reference point m of a row's products s = q.k: weights are 2^(c s - mc) with c = scale log2 e, one
+// fma and one exp2.  The rounding of mc scales all weights of the row alike; products so large
+// that it could overflow them (E::kHuge and up, in log2 units) take the power of two below |c|
+// instead, with which c m is exact: neighbouring fp32 products of that size weigh everything or
+// nothing against each other in either scale.
+template <class E>
+struct Ref {
+  float c, mc;
+  __device__ __forceinline__ Ref(float m, float c0) : c(fabsf(m * c0) < E::kHuge ? c0 : __uint_as_float(__float_as_uint(c0) & 0xff800000u)), mc(fminf(fmaxf(m * c, -FLT_MAX), FLT_MAX)) {}            // (finite: a logit of -inf weighs nothing)
+};
+// What sums against m are worth against mnew (the larger logit of the two).
+template <class E>
+__device__ __forceinline__ float rescale(float m, float mnew, float c0) {
+  const Ref<E> a(m, c0), b(mnew, c0);
+  return a.c == b.c ? fast_exp2(a.mc - b.mc) : 0.f;
+}
+
+struct PackedPlan {
+  int tiles;         // bound on the row tiles of one key head
+  int slices;        // key slices (workgroups per row tile)
+  float c0;          // scale log2 e
+  float* part;       // slices > 1: per (tile, head, slice) unnormalised O [R][DP], then (m, l) [R][2]
+};
+
+// Tile sizes.  KC: 16-dim steps of q.k that hold data; DP: head dim padded to whole 32-dim blocks.
+template <int KC>
+struct Dims {
+  static constexpr int DB = (KC + 1) / 2;                   // 32-dim blocks
+  static constexpr int DP = 32 * DB;
+  static constexpr int kRow = DP * 2;                       // bytes of a K or V row in LDS
+  static constexpr int kPieces = DP / 8;                    // 16-byte pieces of it
+  // K: pieces of a row are XORed by key so that the reads of 16 consecutive keys (one piece each) fall
+  // on 16 different 16-byte slots of the 256 bytes that the banks span.
+  static __device__ __forceinline__ int kpiece(int key, int piece) {
+    return DP == 128 ? piece ^ (key & 15) : DP == 64 ? piece ^ ((key >> 1) & 7) : piece ^ ((key >> 2) & 3);
+  }
+  // V: a transposing read takes 64 bytes of each of 4 consecutive keys: those 64-byte units fall on
+  // different quarters of the banks (rows of 64 and 192 bytes do so by themselves).
+  static __device__ __forceinline__ int vpiece(int key, int piece) {
+    return DP == 128 ? piece ^ ((key & 3) << 2) : DP == 64 ? piece ^ (((key >> 1) & 1) << 2) : piece;
+  }
+};
+
+// One sequence's part of the operands, clamped to what the tensors hold whatever the offsets say.
+struct Seq {
+  int q0, lq, k0, lk;
+};
+__device__ __forceinline__ void seq_range(const int32_t* cu, const int32_t* len, int b, int64_t total, int& start, int& n) {
+  const int64_t s = min(max((int64_t)cu[b], (int64_t)0), total);
+  int64_t e = min(max((int64_t)cu[b + 1], s), total);
+  if (len != nullptr) e = min(e, s + max(len[b], 0));
+  start = (int)s;
+  n = (int)(e - s);
+}
+
+// Tile `idx` of the sequences' row tiles of R rows each, laid end to end: its sequence and its index
+// there, or false past the last.  All lanes of the wave take part; the results are uniform.
+template <int R>
+__device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, int idx, Seq& s, int& tile, int& ntiles) {
+  const int lane = threadIdx.x & 63, G = a.H / a.Hkv;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    int start = 0, n = 0;
+    if (b < a.B) seq_range(a.cu_q, a.len_q, b, a.Tq, start, n);
+    const int nt = (int)(((int64_t)n * G + R - 1) / R);
+    int incl = nt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(incl, o);
+      incl += lane >= o ? up : 0;
+    }
+    const uint64_t past = __ballot(base + incl > idx);
+    if (past != 0) {
+      const int src = __builtin_ctzll(past);
+      s.q0 = __builtin_amdgcn_readlane(start, src);
+      s.lq = __builtin_amdgcn_readlane(n, src);
+      ntiles = __builtin_amdgcn_readlane(nt, src);
+      tile = idx - base - (__builtin_amdgcn_readlane(incl, src) - ntiles);
+      int k0, lk;
+      seq_range(a.cu_k, a.len_k, b0 + src, a.Tk, k0, lk);
+      s.k0 = __builtin_amdgcn_readfirstlane(k0);
+      s.lk = __builtin_amdgcn_readfirstlane(lk);
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
+
+// Last key that row r of the sequence sees (-1: none).
+__device__ __forceinline__ int last_key(const Seq& s, int causal, int r, int G) {
+  return causal ? max(min(r / G + s.lk - s.lq, s.lk - 1), -1) : s.lk - 1;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t bytes) {
+  // raw buffer, 32-bit data: loads past `bytes` return zeros
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+// One row exactly, by a wave, straight from its definition: keys 0 .. last in chunks of 64, a lane
+// each for the products, lanes over the dims for the sums.  For rows whose fast result is not
+// finite: there a NaN or infinite value of a key that the row does not see meets a weight of zero.
+template <class E>
+__device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, const Seq& s, int r, int hk, int last, float c0) {
+  const int lane = threadIdx.x & 63, G = a.H / a.Hkv, D = a.D;
+  const int64_t token = s.q0 + r / G;
+  const int h = hk * G + r % G;
+  const uint16_t* q = (const uint16_t*)a.q + token * a.q_s[0] + (int64_t)h * a.q_s[1];
+  const uint16_t* k = (const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1];
+  const uint16_t* v = (const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1];
+  float m = -FLT_MAX, l = 0.f, o[2] = {0.f, 0.f};
+  for (int j0 = 0; j0 <= last; j0 += 64) {
+    const int j = min(j0 + lane, last);
+    float t = 0.f;
+    for (int d = 0; d < D; ++d) t += E::to_float(q[d]) * E::to_float(k[(int64_t)j * a.k_s[0] + d]);
+    t = c0 < 0.f ? -t : t;
+    if (j0 + lane > last) t = -INFINITY;
+    float mx = fmaxf(t, m);
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    const float w = rescale<E>(m, mx, fabsf(c0));
+    const Ref<E> ref(mx, fabsf(c0));
+    m = mx;
+    const float p = fast_exp2(__builtin_fmaf(t, ref.c, -ref.mc));
+    l = l * w + wave_sum(p);
+    o[0] *= w;
+    o[1] *= w;
+    const int n = min(64, last + 1 - j0);
+    for (int x = 0; x < n; ++x) {
+      const float px = __shfl(p, x);
+      const uint16_t* vr = v + (int64_t)(j0 + x) * a.v_s[0];
+      if (lane < D) o[0] += px * E::to_float(vr[lane]);
+      if (lane + 64 < D) o[1] += px * E::to_float(vr[lane + 64]);
+    }
+  }
+  uint16_t* out = (uint16_t*)a.out + token * a.o_s[0] + (int64_t)h * a.o_s[1];
+  if (lane < D) out[lane] = last < 0 ? 0 : E::from_float(o[0] / l);
+  if (lane + 64 < D) out[lane + 64] = last < 0 ? 0 : E::from_float(o[1] / l);
+}
+
+// What a wave holds of its 32 rows: lane (li, half) has row li; o[db][r] is dim 32 db + 8 (r / 4) +
+// 4 half + r % 4; l is the lane's own part of the sum (its keys).
+template <class E, int KC>
+struct RowState {
+  using T = Dims<KC>;
+  u32x4 q[KC];                                               // Q operand: dims 16 kk + 8 half .. +7
+  f32x16 o[T::DB];
+  float m, l, c0;
+
+  __device__ __forceinline__ void init(const sf_packed_attention_args& a, const Seq& s, int r, int hk, float scale_c0) {
+    const int G = a.H / a.Hkv, half = (threadIdx.x >> 5) & 1;
+    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.q0 + r / G) * a.q_s[0] + (int64_t)(hk * G + r % G) * a.q_s[1];
+#pragma unroll
+    for (int kk = 0; kk < KC; ++kk) {
+      const int d0 = 16 * kk + 8 * half;
+      q[kk] = d0 < a.D ? ld16(qp + d0) : u32x4{0, 0, 0, 0};
+    }
+    // a negative scale turns the queries over, so that the largest product has the largest logit
+    if (scale_c0 < 0.f)
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[kk][e] ^= 0x80008000u;
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[db][x] = 0.f;
+    m = -FLT_MAX;
+    l = 0.f;
+    c0 = fabsf(scale_c0);
+  }
+
+  // One tile of 32 NB keys in LDS.  `last`: the last key of the tile that the lane's row sees (tiles
+  // where a row sees less than all: partial).  first: no tile before this one.
+  template <int NB>
+  __device__ __forceinline__ void tile(const uint8_t* kt, const uint8_t* vt, bool partial, int last, bool first) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
+    f32x16 s[NB];
+    // S^T = K Q^T: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk) {
+        const int key = 32 * kb + li;
+        s[kb] = E::mfma(ld16(kt + key * T::kRow + (T::kpiece(key, 2 * kk + half) << 4)), q[kk], s[kb]);
+      }
+    }
+    if (partial) {
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          s[kb][x] = 32 * kb + 8 * (x >> 2) + 4 * half + (x & 3) > last ? -INFINITY : s[kb][x];
+    }
+    // Weights against a reference point that stays where an earlier tile put it, until a tile's
+    // weights sum to more than the limit: no running maximum, exp or rescale of O in the others.
+    uint32_t p[8 * NB];
+    float sum = 0.f;
+    for (bool raise = first;; raise = true) {
+      if (raise) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[kb][x]);
+        mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+        const float w = rescale<E>(m, mx, c0);
+        m = mx;
+        l *= w;
+#pragma unroll
+        for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[db][x] *= w;
+      }
+      const Ref<E> ref(m, c0);
+      float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float w0 = fast_exp2(__builtin_fmaf(s[kb][2 * e], ref.c, -ref.mc));
+          const float w1 = fast_exp2(__builtin_fmaf(s[kb][2 * e + 1], ref.c, -ref.mc));
+          // rounded to 16 bits for the matrix product; the sum takes the rounded weights, so that
+          // they still average to one
+          p[8 * kb + e] = E::pack(w0, w1);
+          if (e & 1) t1 = E::sum2(p[8 * kb + e], t1); else t0 = E::sum2(p[8 * kb + e], t0);
+        }
+      sum = t0 + t1;
+      if (raise || !__any(!(sum <= E::kMassLimit))) break;
+    }
+    l += sum;
+    // O^T += V^T P^T; a 16-lane group of the transposing read takes 4 keys x 16 dims
+    const int grp = lane >> 4, ekey = (lane & 15) >> 2, q4 = lane & 3;
+#pragma unroll
+    for (int c2 = 0; c2 < 2 * NB; ++c2) {
+      const u32x4 pb = {p[4 * c2], p[4 * c2 + 1], p[4 * c2 + 2], p[4 * c2 + 3]};
+#pragma unroll
+      for (int db = 0; db < T::DB; ++db) {
+        const int d = 32 * db + 16 * (grp & 1) + 4 * q4;
+        u32x2 part[2];
+#pragma unroll
+        for (int rd = 0; rd < 2; ++rd) {
+          const int key = 16 * c2 + 8 * rd + 4 * (grp >> 1) + ekey;
+          const uint8_t* at = vt + key * T::kRow + (T::vpiece(key, d >> 3) << 4) + ((d >> 2) & 1) * 8;
+          part[rd] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16p*)at));
+        }
+        o[db] = E::mfma(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]}, pb, o[db]);
+      }
+    }
+  }
+
+  // Zero where every accumulator is finite, NaN otherwise.
+  __device__ __forceinline__ float finite_probe() const {
+    float f = 0.f;
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) f = __builtin_fmaf(o[db][x], 0.f, f);
+    return f;
+  }
+};
+
+// One K or V tile of a sequence on its way from global memory to LDS through registers: NT threads,
+// KT keys.  Rows past the sequence and dims past D arrive as zeros.
+template <int KC, int KT, int NT>
+struct Stage {
+  using T = Dims<KC>;
+  static constexpr int kPiecesAll = KT * T::kPieces;
+  static constexpr int kN = (kPiecesAll + NT - 1) / NT;
+  uint32_t off[kN];                                          // global byte offset of each piece, in the tile
+  const char* base;
+  int64_t row;                                               // bytes between rows
+  int dbytes;
+  u32x4 data[kN];
+
+  __device__ __forceinline__ void init(const void* p, int64_t stride, int t, int D) {
+    base = (const char*)p;
+    row = stride * 2;
+    dbytes = D * 2;
+#pragma unroll
+    for (int u = 0; u < kN; ++u) {
+      const int idx = u * NT + t, key = idx / T::kPieces, piece = idx % T::kPieces;
+      off[u] = idx < kPiecesAll && piece * 8 < D ? (uint32_t)(key * row) + piece * 16 : 0x7ffffff0u;
+    }
+  }
+  // tile starting at key j0, keys j0 .. lk - 1 exist (j0 < lk)
+  __device__ __forceinline__ void load(int j0, int lk) {
+    const int n = min(KT, lk - j0);
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + j0 * row, (n - 1) * row + dbytes);
+#pragma unroll
+    for (int u = 0; u < kN; ++u)
+      data[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[u], 0, 0));
+  }
+  template <bool V>
+  __device__ __forceinline__ void store(uint8_t* lds, int t) const {
+#pragma unroll
+    for (int u = 0; u < kN; ++u) {
+      const int idx = u * NT + t, key = idx / T::kPieces, piece = idx % T::kPieces;
+      if (kPiecesAll % NT == 0 || idx < kPiecesAll)
+        st16(lds + key * T::kRow + ((V ? T::vpiece(key, piece) : T::kpiece(key, piece)) << 4), data[u]);
+    }
+  }
+};
+
+// Workgroups of NW waves, 32 rows each, over shared K/V tiles of 64 keys: two LDS buffers and
+// one barrier a tile; the tile after the next is in flight to registers meanwhile.  Tiles go from
+// the last that the rows see to the first, the partly visible ones first.
+template <class E, int KC, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
+  using T = Dims<KC>;
+  constexpr int kTile = 64 * T::kRow, R = 32 * NW;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];     // two buffers of K, V
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
+  const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+  const int slice = rest % pl.slices, idx = rest / pl.slices;
+  Seq s;
+  int tile, ntiles;
+  if (!find_tile<R>(a, idx, s, tile, ntiles)) return;
+  tile = ntiles - 1 - tile;                                  // causal: the longest rows first
+  const int G = a.H / a.Hkv, rows = s.lq * G, r0 = tile * R + wave * 32;
+  const int row = min(r0 + li, rows - 1);                    // rows past the end repeat the last
+  const int seen = last_key(s, a.causal, min(tile * R + R, rows) - 1, G) + 1;   // keys the workgroup's last row sees
+  const int n_all = (seen + 63) / 64;
+  const int t_lo = (int)((int64_t)n_all * slice / pl.slices), t_hi = (int)((int64_t)n_all * (slice + 1) / pl.slices);
+
+  RowState<E, KC> st;
+  st.init(a, s, row, hk, pl.c0);
+  const int mine = last_key(s, a.causal, row, G);
+  // of this wave's rows: the fewest and the most keys
+  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0, rows - 1), G));
+  const int high = r0 < rows ? __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0 + 31, rows - 1), G)) : -1;
+
+  if (t_lo < t_hi) {
+    Stage<KC, 64, 64 * NW> ks, vs;
+    ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], tid, a.D);
+    vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], tid, a.D);
+    ks.load(64 * (t_hi - 1), s.lk);
+    vs.load(64 * (t_hi - 1), s.lk);
+    ks.template store<false>(smem, tid);
+    vs.template store<true>(smem + kTile, tid);
+    if (t_hi - 2 >= t_lo) {
+      ks.load(64 * (t_hi - 2), s.lk);
+      vs.load(64 * (t_hi - 2), s.lk);
+    }
+    lds_only_barrier();
+    bool first = true;
+    for (int t = t_hi - 1, buf = 0; t >= t_lo; --t, buf ^= 1) {
+      if (t > t_lo) {
+        uint8_t* next = smem + (buf ^ 1) * 2 * kTile;
+        ks.template store<false>(next, tid);
+        vs.template store<true>(next + kTile, tid);
+        if (t - 1 > t_lo) {
+          ks.load(64 * (t - 2), s.lk);
+          vs.load(64 * (t - 2), s.lk);
+        }
+      }
+      if (64 * t <= high) {
+        const uint8_t* kt = smem + buf * 2 * kTile;
+        st.template tile<2>(kt, kt + kTile, 64 * t + 63 > low, mine - 64 * t, first);
+        first = false;
+      }
+      lds_only_barrier();
+    }
+  }
+  if (r0 >= rows) return;                                    // (no barrier from here on)
+  const float l = st.l + __shfl_xor(st.l, 32);
+  if (pl.slices > 1) {
+    float* po = pl.part + (((int64_t)idx * a.Hkv + hk) * pl.slices + slice) * R * (T::DP + 2);
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4)
+        *reinterpret_cast<f32x4*>(po + (wave * 32 + li) * T::DP + 32 * db + 8 * c4 + 4 * half) =
+            f32x4{st.o[db][4 * c4], st.o[db][4 * c4 + 1], st.o[db][4 * c4 + 2], st.o[db][4 * c4 + 3]};
+    if (half == 0) *reinterpret_cast<f32x2*>(po + R * T::DP + 2 * (wave * 32 + li)) = f32x2{st.m, l};
+    return;
+  }
+  const float inv = mine < 0 ? 0.f : 1.f / l;
+  // rows to be done again (see exact_row): either half's accumulators are not finite
+  const uint64_t badl = __ballot(a.causal && !(st.finite_probe() == 0.f) && r0 + li < rows);
+  uint32_t bad = (uint32_t)badl | (uint32_t)(badl >> 32);
+  uint16_t* op = (uint16_t*)a.out + (int64_t)(s.q0 + row / G) * a.o_s[0] + (int64_t)(hk * G + row % G) * a.o_s[1];
+  const bool write = r0 + li < rows && !(bad >> li & 1);
+#pragma unroll
+  for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t w[4];                                         // dims 32 db + 16 c + {0, 8} + 4 half .. +3
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = E::pack(st.o[db][8 * c + 2 * e] * inv, st.o[db][8 * c + 2 * e + 1] * inv);
+      // half 0 takes the 8 dims 16 c .., half 1 the 8 dims 16 c + 8 ..
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      const int d0 = 32 * db + 16 * c + 8 * half;
+      if (write && d0 < a.D) st16(op + d0, u32x4{x[0], y[0], x[1], y[1]});
+    }
+  for (; bad != 0; bad &= bad - 1) {
+    const int r = r0 + __builtin_ctz(bad);
+    exact_row<E>(a, s, r, hk, last_key(s, a.causal, r, G), pl.c0);
+  }
+}
+
+// 32 rows a workgroup (a new token's heads, short pieces): its 4 waves each stream a slice of the
+// keys through LDS of their own, no barrier until the slices are joined.  Bound by the reads of K
+// and V; with few rows the workgroups themselves take slices (pl.slices), joined by
+// packed_combine_kernel.
+template <class E, int KC>
+__global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
+  using T = Dims<KC>;
+  constexpr int KT = T::DP <= 64 ? 64 : 32, kTile = KT * T::kRow;
+  static_assert(2 * kTile >= 32 * T::DP * 4, "a wave's tiles hold its O");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * 2 * kTile];
+  __shared__ f32x2 ml[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+  const int slice = rest % pl.slices, idx = rest / pl.slices;
+  Seq s;
+  int tile, ntiles;
+  if (!find_tile<32>(a, idx, s, tile, ntiles)) return;
+  const int G = a.H / a.Hkv, rows = s.lq * G, r0 = tile * 32;
+  const int row = min(r0 + li, rows - 1);
+  const int seen = last_key(s, a.causal, min(r0 + 32, rows) - 1, G) + 1;
+  const int n_all = (seen + KT - 1) / KT, z = slice * 4 + wave, Z = pl.slices * 4;
+  const int t_lo = (int)((int64_t)n_all * z / Z), t_hi = (int)((int64_t)n_all * (z + 1) / Z);
+  const int mine = last_key(s, a.causal, row, G);
+  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, r0, G));
+  uint8_t* kt = smem + wave * 2 * kTile;
+  {
+    RowState<E, KC> st;
+    st.init(a, s, row, hk, pl.c0);
+    if (t_lo < t_hi) {
+      Stage<KC, KT, 64> ks, vs;
+      ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], lane, a.D);
+      vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], lane, a.D);
+      ks.load(KT * (t_hi - 1), s.lk);
+      vs.load(KT * (t_hi - 1), s.lk);
+      for (int t = t_hi - 1; t >= t_lo; --t) {
+        ks.template store<false>(kt, lane);
+        vs.template store<true>(kt + kTile, lane);
+        if (t > t_lo) {
+          ks.load(KT * (t - 1), s.lk);
+          vs.load(KT * (t - 1), s.lk);
+        }
+        st.template tile<KT / 32>(kt, kt + kTile, KT * t + KT - 1 > low, mine - KT * t, t == t_hi - 1);
+      }
+    }
+    // the slice's O over the wave's tiles, for all threads
+    const float l = st.l + __shfl_xor(st.l, 32);
+    float* po = (float*)kt;
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4)
+        *reinterpret_cast<f32x4*>(po + li * T::DP + 32 * db + 8 * c4 + 4 * half) =
+            f32x4{st.o[db][4 * c4], st.o[db][4 * c4 + 1], st.o[db][4 * c4 + 2], st.o[db][4 * c4 + 3]};
+    if (half == 0) ml[wave][li] = f32x2{st.m, l};
+  }
+  lds_only_barrier();
+  // thread (row tid / 8, dims 4 (tid % 8) + 32 db): the 4 slices of the waves
+  const int jr = tid >> 3, jd = 4 * (tid & 7);
+  float m = ml[0][jr][0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][jr][0]);
+  float l = 0.f, wt[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    wt[w] = rescale<E>(ml[w][jr][0], m, fabsf(pl.c0));
+    l += wt[w] * ml[w][jr][1];
+  }
+  f32x4 o[T::DB];
+  float probe = 0.f;
+#pragma unroll
+  for (int db = 0; db < T::DB; ++db) {
+    o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)(smem + w * 2 * kTile) + jr * T::DP + 32 * db + jd);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[db][e] += wt[w] * x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[db][e], 0.f, probe);
+  }
+  if (pl.slices > 1) {
+    float* po = pl.part + (((int64_t)idx * a.Hkv + hk) * pl.slices + slice) * 32 * (T::DP + 2);
+    if (r0 + jr < rows) {
+#pragma unroll
+      for (int db = 0; db < T::DB; ++db) *reinterpret_cast<f32x4*>(po + jr * T::DP + 32 * db + jd) = o[db];
+      if (jd == 0) *reinterpret_cast<f32x2*>(po + 32 * T::DP + 2 * jr) = f32x2{m, l};
+    }
+    return;
+  }
+  const int r = r0 + jr;
+  const uint64_t bad8 = __ballot(a.causal && !(probe == 0.f) && r < rows);   // a byte for each of the wave's 8 rows
+  if (r < rows && !(bad8 >> (lane & 56) & 0xff)) {
+    const float inv = last_key(s, a.causal, r, G) < 0 ? 0.f : 1.f / l;
+    uint16_t* op = (uint16_t*)a.out + (int64_t)(s.q0 + r / G) * a.o_s[0] + (int64_t)(hk * G + r % G) * a.o_s[1];
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+      if (32 * db + jd < a.D)
+        *reinterpret_cast<u32x2*>(op + 32 * db + jd) = u32x2{E::pack(o[db][0] * inv, o[db][1] * inv), E::pack(o[db][2] * inv, o[db][3] * inv)};
+  }
+  for (int x = 0; x < 8; ++x)
+    if (bad8 >> (8 * x) & 0xff) exact_row<E>(a, s, r0 + wave * 8 + x, hk, last_key(s, a.causal, r0 + wave * 8 + x, G), pl.c0);
+}
+
+// Joins the key slices of a row, a wave per row: o = sum_z w_z O_z / sum_z w_z l_z with w_z the worth of
+// slice z's reference point against the largest.  R: rows of a tile.
+template <class E, int DP, int R>
+__global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int quad = blockIdx.x % (R / 4), rest = blockIdx.x / (R / 4), hk = rest % a.Hkv, idx = rest / a.Hkv;
+  Seq s;
+  int tile, ntiles;
+  if (!find_tile<R>(a, idx, s, tile, ntiles)) return;
+  if (R > 32) tile = ntiles - 1 - tile;                      // as packed_tile_kernel takes them
+  const int G = a.H / a.Hkv, in = quad * 4 + wave, r = tile * R + in;
+  if (r >= s.lq * G) return;
+  const float* part = pl.part + ((int64_t)idx * a.Hkv + hk) * pl.slices * R * (DP + 2);
+  constexpr int64_t kStep = R * (DP + 2);
+  float m = -FLT_MAX, l = 0.f;
+  if (lane < pl.slices) {                                    // slices <= 64
+    const f32x2 v = *reinterpret_cast<const f32x2*>(part + lane * kStep + R * DP + 2 * in);
+    m = v[0];
+    l = v[1];
+  }
+  float mx = m;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+  const float w = lane < pl.slices ? rescale<E>(m, mx, fabsf(pl.c0)) : 0.f;
+  const float sum = wave_sum(w * l);
+  const int d = 2 * lane;
+  f32x2 o = {0.f, 0.f};
+  if (d < DP) {
+    const float* po = part + in * DP + d;
+#pragma unroll 4
+    for (int z = 0; z < pl.slices; ++z) {
+      const f32x2 v = *reinterpret_cast<const f32x2*>(po + z * kStep);
+      const float wz = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z));
+      o[0] += wz * v[0];
+      o[1] += wz * v[1];
+    }
+  }
+  const int last = last_key(s, a.causal, r, G);
+  if (a.causal && __any(!(__builtin_fmaf(o[0], 0.f, o[1] * 0.f) == 0.f))) {
+    exact_row<E>(a, s, r, hk, last, pl.c0);
+    return;
+  }
+  const float inv = last < 0 ? 0.f : 1.f / sum;
+  if (d < a.D)
+    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + (int64_t)(s.q0 + r / G) * a.o_s[0] + (int64_t)(hk * G + r % G) * a.o_s[1] + d) =
+        E::pack(o[0] * inv, o[1] * inv);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Route {
+  int nw;            // waves of packed_tile_kernel's workgroups; 0: packed_stream_kernel
+  int kc, dp;
+  PackedPlan pl;
+  int64_t wgs;
+};
+
+int route(const sf_packed_attention_args* a, Route& r) {
+  if (a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->D <= 0 || a->Tq < 0 || a->Tk < 0) {
+    sf_set_error("packed attention: sizes must be positive (B=%d H=%d Hkv=%d D=%d Tq=%lld Tk=%lld)", a->B, a->H, a->Hkv, a->D,
+                 (long long)a->Tq, (long long)a->Tk);
+    return 1;
+  }
+  if (a->H % a->Hkv != 0) { sf_set_error("packed attention: %d heads do not share %d key heads evenly", a->H, a->Hkv); return 1; }
+  if (a->D > 128 || a->D % 8 != 0) { sf_set_error("packed attention: head dim %d is not a multiple of 8 up to 128", a->D); return 1; }
+  if (a->dtype != SF_DTYPE_BF16 && a->dtype != SF_DTYPE_F16) { sf_set_error("packed attention: element type %d", a->dtype); return 1; }
+  if (!(fabsf(a->scale) <= 1e30f)) { sf_set_error("packed attention: scale %g is not finite or above 1e30", (double)a->scale); return 1; }
+  const int G = a->H / a->Hkv;
+  if (a->Tk > INT32_MAX || a->Tq * G > INT32_MAX) {
+    sf_set_error("packed attention: %lld query rows or %lld keys exceed 2^31 - 1", (long long)(a->Tq * G), (long long)a->Tk);
+    return 1;
+  }
+  if (a->Tq > 0 && (a->q == nullptr || a->out == nullptr || (a->Tk > 0 && (a->k == nullptr || a->v == nullptr)))) {
+    sf_set_error("packed attention: q, k, v and out must be non-null"); return 1;
+  }
+  if (a->cu_q == nullptr || a->cu_k == nullptr) { sf_set_error("packed attention: cu_q and cu_k must be non-null"); return 1; }
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) {
+    sf_set_error("packed attention: q, k, v and out must be 16-byte aligned"); return 1;
+  }
+  for (int i = 0; i < 2; ++i)
+    if (a->q_s[i] % 8 || a->k_s[i] % 8 || a->v_s[i] % 8 || a->o_s[i] % 8) {
+      sf_set_error("packed attention: strides must be multiples of 8 elements"); return 1;
+    }
+  for (const int64_t st : {a->k_s[0], a->v_s[0]})
+    if (st < a->D || st >= 1 << 24) {
+      sf_set_error("packed attention: key and value row strides must lie in [D, 2^24)"); return 1;
+    }
+  r.kc = a->D <= 32 ? 2 : a->D <= 48 ? 3 : a->D <= 64 ? 4 : a->D <= 96 ? 6 : 8;
+  r.dp = 32 * ((r.kc + 1) / 2);
+  const int64_t rows = a->Tq * G;
+  const int64_t keys = (a->Tk + a->B - 1) / a->B;            // of a sequence, on average
+  r.nw = rows > 64ll * a->B ? 4 : 0;
+  const int R = r.nw ? 32 * r.nw : 32;
+  // tiles end at sequence ends: sum_b ceil(rows_b / R) <= rows / R + B
+  const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
+  const int64_t base = tiles * a->Hkv;
+  // few workgroups: slices of the keys, at least 4 tiles (a wave's 2) long each
+  const int64_t want = (512 + base - 1) / base, most = r.nw ? keys / 512 : keys / 512;
+  int64_t slices = want < most ? want : most;
+  slices = slices < 1 ? 1 : slices > 64 ? 64 : slices;
+  float c0 = a->scale * SF_LOG2E;
+  if (fabsf(c0) < FLT_MIN) c0 = FLT_MIN;                     // all logits equal; a masked one stays -inf
+  r.pl = PackedPlan{(int)tiles, (int)slices, c0, nullptr};
+  r.wgs = base * slices;
+  if (r.wgs > INT32_MAX || tiles * a->Hkv * (R / 4) > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
+  return 0;
+}
+
+size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
+  if (r.pl.slices <= 1) return 0;
+  const int R = r.nw ? 32 * r.nw : 32;
+  return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float);
+}
+
+template <class E, int KC>
+int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
+  const dim3 grid((unsigned)r.wgs);
+  if (r.nw == 4) hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4>), grid, dim3(256), 0, st, *a, r.pl);
+  else hipLaunchKernelGGL((packed_stream_kernel<E, KC>), grid, dim3(256), 0, st, *a, r.pl);
+  const int rc = sf_check_launch(r.nw ? "packed_tile_kernel" : "packed_stream_kernel");
+  if (rc || r.pl.slices <= 1) return rc;
+  const int R = r.nw ? 32 * r.nw : 32;
+  const dim3 gc((unsigned)(r.pl.tiles * a->Hkv * (R / 4)));
+  constexpr int DP = Dims<KC>::DP;
+  if (r.nw == 4) hipLaunchKernelGGL((packed_combine_kernel<E, DP, 128>), gc, dim3(256), 0, st, *a, r.pl);
+  else hipLaunchKernelGGL((packed_combine_kernel<E, DP, 32>), gc, dim3(256), 0, st, *a, r.pl);
+  return sf_check_launch("packed_combine_kernel");
+}
+
+template <class E>
+int launch_type(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
+  switch (r.kc) {
+    case 2: return launch<E, 2>(a, r, st);
+    case 3: return launch<E, 3>(a, r, st);
+    case 4: return launch<E, 4>(a, r, st);
+    case 6: return launch<E, 6>(a, r, st);
+    default: return launch<E, 8>(a, r, st);
+  }
+}
+
+}  // namespace
+
+extern "C" size_t sf_hip_packed_attention_workspace_bytes(const sf_packed_attention_args* a) {
+  Route r;
+  if (a == nullptr || a->Tq == 0 || route(a, r)) return 0;
+  return part_bytes(a, r);
+}
+
+extern "C" int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (a == nullptr) { sf_set_error("packed attention: null args"); return 1; }
+  Route r;
+  if (a->Tq == 0 && a->B > 0) return 0;                      // nothing to write
+  if (route(a, r)) return 1;
+  const size_t need = part_bytes(a, r);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
+    sf_set_error("packed attention: needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
+    return 1;
+  }
+  r.pl.part = static_cast<float*>(workspace);
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return a->dtype == SF_DTYPE_BF16 ? launch_type<Bf16>(a, r, st) : launch_type<Fp16>(a, r, st);
+}
