@@ -153,6 +153,10 @@ __device__ __forceinline__ int last_key(const Seq& s, int causal, int r, int G) 
   return causal ? max(min(r / G + s.lk - s.lq, s.lk - 1), -1) : s.lk - 1;
 }
 
+// Offset of pieces that do not exist.  A tile's last byte lies below it (row strides below 2^25 bytes, 64
+// rows), and so does what the rows' steps add to it below 2^32.
+constexpr uint32_t kOutside = 0x80000000u;
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t bytes) {
   // raw buffer, 32-bit data: loads past `bytes` return zeros
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
@@ -231,50 +235,50 @@ struct RowState {
     c0 = fabsf(scale_c0);
   }
 
-  // One tile of 32 NB keys in LDS.  `last`: the last key of the tile that the lane's row sees (tiles
-  // where a row sees less than all: partial).  first: no tile before this one.
+  // S^T = K Q^T of a tile of 32 NB keys in LDS: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4.
   template <int NB>
-  __device__ __forceinline__ void tile(const uint8_t* kt, const uint8_t* vt, bool partial, int last, bool first) {
+  __device__ __forceinline__ void products(const uint8_t* kt, f32x16 (&s)[NB]) const {
     const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
-    f32x16 s[NB];
-    // S^T = K Q^T: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KC; ++kk) {
+    for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
         const int key = 32 * kb + li;
         s[kb] = E::mfma(ld16(kt + key * T::kRow + (T::kpiece(key, 2 * kk + half) << 4)), q[kk], s[kb]);
       }
+    // the reads run kAhead operands before the products that take them
+    constexpr int kAhead = NB * KC < 4 ? NB * KC : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int x = 0; x < NB * KC - kAhead; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+  }
+
+  // The rest of a tile, its V rows in LDS.  `last`: the last key of the tile that the lane's row sees
+  // (partial: tiles where a row sees less than all).
+  template <int NB>
+  __device__ __forceinline__ void weigh(f32x16 (&s)[NB], const uint8_t* vt, bool partial, int last) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
     if (partial) {
+      last -= 4 * half;                                      // (so that the keys are constants)
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          s[kb][x] = 32 * kb + 8 * (x >> 2) + 4 * half + (x & 3) > last ? -INFINITY : s[kb][x];
+          s[kb][x] = 32 * kb + 8 * (x >> 2) + (x & 3) > last ? -INFINITY : s[kb][x];
     }
     // Weights against a reference point that stays where an earlier tile put it, until a tile's
-    // weights sum to more than the limit: no running maximum, exp or rescale of O in the others.
+    // weights sum to more than the limit (as those of the first do): no running maximum, exp or
+    // rescale of O in the others.
     uint32_t p[8 * NB];
-    float sum = 0.f;
-    for (bool raise = first;; raise = true) {
-      if (raise) {
-        float mx = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[kb][x]);
-        mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-        const float w = rescale<E>(m, mx, c0);
-        m = mx;
-        l *= w;
-#pragma unroll
-        for (int db = 0; db < T::DB; ++db)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[db][x] *= w;
-      }
+    auto weights = [&]() __attribute__((always_inline)) {
       const Ref<E> ref(m, c0);
       float t0 = 0.f, t1 = 0.f;
 #pragma unroll
@@ -288,8 +292,24 @@ struct RowState {
           p[8 * kb + e] = E::pack(w0, w1);
           if (e & 1) t1 = E::sum2(p[8 * kb + e], t1); else t0 = E::sum2(p[8 * kb + e], t0);
         }
-      sum = t0 + t1;
-      if (raise || !__any(!(sum <= E::kMassLimit))) break;
+      return t0 + t1;
+    };
+    float sum = weights();
+    if (__any(!(sum <= E::kMassLimit))) {
+      float mx = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[kb][x]);
+      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+      const float w = rescale<E>(m, mx, c0);
+      m = mx;
+      l *= w;
+#pragma unroll
+      for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[db][x] *= w;
+      sum = weights();
     }
     l += sum;
     // O^T += V^T P^T; a 16-lane group of the transposing read takes 4 keys x 16 dims
@@ -310,6 +330,14 @@ struct RowState {
         o[db] = E::mfma(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]}, pb, o[db]);
       }
     }
+    constexpr int kProducts = 2 * NB * T::DB, kAhead = kProducts < 4 ? kProducts : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 1);
+#pragma unroll
+    for (int x = 0; x < kProducts - kAhead; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 1);
   }
 
   // Zero where every accumulator is finite, NaN otherwise.
@@ -330,7 +358,10 @@ struct Stage {
   using T = Dims<KC>;
   static constexpr int kPiecesAll = KT * T::kPieces;
   static constexpr int kN = (kPiecesAll + NT - 1) / NT;
-  uint32_t off[kN];                                          // global byte offset of each piece, in the tile
+  // a thread's pieces lie whole rows apart: one offset, and kStep rows from piece to piece
+  static constexpr bool kSteps = NT % T::kPieces == 0;
+  static constexpr int kStep = NT / T::kPieces;
+  uint32_t off[kSteps ? 1 : kN];                             // global byte offsets in the tile
   const char* base;
   int64_t row;                                               // bytes between rows
   int dbytes;
@@ -341,18 +372,21 @@ struct Stage {
     row = stride * 2;
     dbytes = D * 2;
 #pragma unroll
-    for (int u = 0; u < kN; ++u) {
+    for (int u = 0; u < (kSteps ? 1 : kN); ++u) {
       const int idx = u * NT + t, key = idx / T::kPieces, piece = idx % T::kPieces;
-      off[u] = idx < kPiecesAll && piece * 8 < D ? (uint32_t)(key * row) + piece * 16 : 0x7ffffff0u;
+      off[u] = idx < kPiecesAll && piece * 8 < D ? (uint32_t)(key * row) + piece * 16 : kOutside;
     }
   }
-  // tile starting at key j0, keys j0 .. lk - 1 exist (j0 < lk)
-  __device__ __forceinline__ void load(int j0, int lk) {
+  // tile starting at key j0, keys j0 .. lk - 1 exist (j0 < lk); zeros, and nothing read, where the tile
+  // is not `there`: no branch around the loads, so that their registers have one value on every path
+  __device__ __forceinline__ void load(int j0, int lk, bool there) {
     const int n = min(KT, lk - j0);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + j0 * row, (n - 1) * row + dbytes);
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + j0 * row, there ? (n - 1) * row + dbytes : 0);
+    uint32_t step = (uint32_t)(kStep * row);
+    asm volatile("" : "+s"(step));                           // (formed per tile: kept over the loop, the sums cost registers)
 #pragma unroll
     for (int u = 0; u < kN; ++u)
-      data[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[u], 0, 0));
+      data[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(kSteps ? off[0] + u * step : off[u]), 0, 0));
   }
   template <bool V>
   __device__ __forceinline__ void store(uint8_t* lds, int t) const {
@@ -399,33 +433,39 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
     Stage<KC, 64, 64 * NW> ks, vs;
     ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], tid, a.D);
     vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], tid, a.D);
-    ks.load(64 * (t_hi - 1), s.lk);
-    vs.load(64 * (t_hi - 1), s.lk);
+    ks.load(64 * (t_hi - 1), s.lk, true);
+    vs.load(64 * (t_hi - 1), s.lk, true);
     ks.template store<false>(smem, tid);
     vs.template store<true>(smem + kTile, tid);
-    if (t_hi - 2 >= t_lo) {
-      ks.load(64 * (t_hi - 2), s.lk);
-      vs.load(64 * (t_hi - 2), s.lk);
-    }
+    ks.load(64 * (t_hi - 2), s.lk, t_hi - 2 >= t_lo);
+    vs.load(64 * (t_hi - 2), s.lk, t_hi - 2 >= t_lo);
     lds_only_barrier();
-    bool first = true;
-    for (int t = t_hi - 1, buf = 0; t >= t_lo; --t, buf ^= 1) {
-      if (t > t_lo) {
-        uint8_t* next = smem + (buf ^ 1) * 2 * kTile;
-        ks.template store<false>(next, tid);
-        vs.template store<true>(next + kTile, tid);
-        if (t - 1 > t_lo) {
-          ks.load(64 * (t - 2), s.lk);
-          vs.load(64 * (t - 2), s.lk);
-        }
-      }
-      if (64 * t <= high) {
-        const uint8_t* kt = smem + buf * 2 * kTile;
-        st.template tile<2>(kt, kt + kTile, 64 * t + 63 > low, mine - 64 * t, first);
-        first = false;
-      }
+    int t = t_hi - 1, buf = 0;
+    auto refill = [&]() __attribute__((always_inline)) {     // the next tile to the other buffer, the one after it on its way
+      uint8_t* next = smem + (buf ^ 1) * 2 * kTile;
+      ks.template store<false>(next, tid);
+      vs.template store<true>(next + kTile, tid);
+      ks.load(64 * (t - 2), s.lk, t - 1 > t_lo);
+      vs.load(64 * (t - 2), s.lk, t - 1 > t_lo);
+    };
+    auto step = [&](auto partial) __attribute__((always_inline)) {
+      refill();
+      const uint8_t* kt = smem + buf * 2 * kTile;
+      f32x16 sc[2];
+      st.template products<2>(kt, sc);
+      st.template weigh<2>(sc, kt + kTile, decltype(partial)::value, mine - 64 * t);
       lds_only_barrier();
+      --t;
+      buf ^= 1;
+    };
+    for (; t >= t_lo && 64 * t > high;) {                    // tiles that none of this wave's rows sees
+      refill();
+      lds_only_barrier();
+      --t;
+      buf ^= 1;
     }
+    while (t >= t_lo && 64 * t + 63 > low) step(std::true_type{});
+    while (t >= t_lo) step(std::false_type{});
   }
   if (r0 >= rows) return;                                    // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
@@ -466,15 +506,15 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
 }
 
 // 32 rows a workgroup (a new token's heads, short pieces): its 4 waves each stream a slice of the
-// keys through LDS of their own, no barrier until the slices are joined.  Bound by the reads of K
-// and V; with few rows the workgroups themselves take slices (pl.slices), joined by
-// packed_combine_kernel.
+// keys, no barrier until the slices are joined: K straight into the registers of the matrix operand,
+// V through registers to LDS of the wave's own.  Bound by the reads of K and V; with few rows the
+// workgroups themselves take slices (pl.slices), joined by packed_combine_kernel.
 template <class E, int KC>
 __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
-  constexpr int KT = T::DP <= 64 ? 64 : 32, kTile = KT * T::kRow;
-  static_assert(2 * kTile >= 32 * T::DP * 4, "a wave's tiles hold its O");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * 2 * kTile];
+  constexpr int KT = T::DP <= 64 ? 64 : 32, NB = KT / 32, kTile = KT * T::kRow;
+  constexpr int kWave = kTile > 32 * T::DP * 4 ? kTile : 32 * T::DP * 4;   // V tile, later the wave's O
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kWave];
   __shared__ f32x2 ml[4][32];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -490,29 +530,48 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   const int t_lo = (int)((int64_t)n_all * z / Z), t_hi = (int)((int64_t)n_all * (z + 1) / Z);
   const int mine = last_key(s, a.causal, row, G);
   const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, r0, G));
-  uint8_t* kt = smem + wave * 2 * kTile;
+  uint8_t* vt = smem + wave * kWave;
   {
     RowState<E, KC> st;
     st.init(a, s, row, hk, pl.c0);
     if (t_lo < t_hi) {
-      Stage<KC, KT, 64> ks, vs;
-      ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], lane, a.D);
+      const char* kbase = (const char*)((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1]);
+      const int64_t krow = a.k_s[0] * 2;
+      const uint32_t koff = (uint32_t)(li * krow) + 16 * half;
+      u32x4 kf[NB][KC];                                      // keys 32 kb + li, dims 16 kk + 8 half .. +7
+      auto load_k = [&](int j0, bool there) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t r = rows_rsrc(kbase + j0 * krow, there ? (min(KT, s.lk - j0) - 1) * krow + a.D * 2 : 0);
+        uint32_t o = koff, oh = half ? kOutside : koff;      // steps that both halves have, that the first has
+        asm volatile("" : "+v"(o), "+v"(oh));                // (formed per tile: kept over the loop, the sums cost registers)
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int kk = 0; kk < KC; ++kk)
+            kf[kb][kk] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                r, (int)((16 * kk + 8 < a.D ? o : 16 * kk < a.D ? oh : kOutside) + kb * 32 * (uint32_t)krow + 32 * kk), 0, 0));
+      };
+      Stage<KC, KT, 64> vs;
       vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], lane, a.D);
-      ks.load(KT * (t_hi - 1), s.lk);
-      vs.load(KT * (t_hi - 1), s.lk);
+      load_k(KT * (t_hi - 1), true);
+      vs.load(KT * (t_hi - 1), s.lk, true);
       for (int t = t_hi - 1; t >= t_lo; --t) {
-        ks.template store<false>(kt, lane);
-        vs.template store<true>(kt + kTile, lane);
-        if (t > t_lo) {
-          ks.load(KT * (t - 1), s.lk);
-          vs.load(KT * (t - 1), s.lk);
+        f32x16 sc[NB];
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sc[kb][x] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < KC; ++kk) sc[kb] = E::mfma(kf[kb][kk], st.q[kk], sc[kb]);
         }
-        st.template tile<KT / 32>(kt, kt + kTile, KT * t + KT - 1 > low, mine - KT * t, t == t_hi - 1);
+        vs.template store<true>(vt, lane);
+        load_k(KT * (t - 1), t > t_lo);
+        vs.load(KT * (t - 1), s.lk, t > t_lo);
+        st.template weigh<NB>(sc, vt, KT * t + KT - 1 > low, mine - KT * t);
       }
     }
     // the slice's O over the wave's tiles, for all threads
     const float l = st.l + __shfl_xor(st.l, 32);
-    float* po = (float*)kt;
+    float* po = (float*)vt;
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
@@ -540,7 +599,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
     o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)(smem + w * 2 * kTile) + jr * T::DP + 32 * db + jd);
+      const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)(smem + w * kWave) + jr * T::DP + 32 * db + jd);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[db][e] += wt[w] * x[e];
     }
@@ -595,14 +654,17 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
   for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
   const float w = lane < pl.slices ? rescale<E>(m, mx, fabsf(pl.c0)) : 0.f;
   const float sum = wave_sum(w * l);
+  __shared__ float worth[4][64];
+  worth[wave][lane] = w;
+  asm volatile("" ::: "memory");                             // (a wave's LDS accesses are in order)
   const int d = 2 * lane;
   f32x2 o = {0.f, 0.f};
   if (d < DP) {
     const float* po = part + in * DP + d;
-#pragma unroll 4
+#pragma unroll 8
     for (int z = 0; z < pl.slices; ++z) {
       const f32x2 v = *reinterpret_cast<const f32x2*>(po + z * kStep);
-      const float wz = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), z));
+      const float wz = worth[wave][z];
       o[0] += wz * v[0];
       o[1] += wz * v[1];
     }
