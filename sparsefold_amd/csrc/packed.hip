@@ -66,6 +66,7 @@ struct Fp16 {
 template <class E>
 struct Ref {
   float c, mc;
+  Ref() = default;
   __device__ __forceinline__ Ref(float m, float c0) : c(fabsf(m * c0) < E::kHuge ? c0 : __uint_as_float(__float_as_uint(c0) & 0xff800000u)), mc(fminf(fmaxf(m * c, -FLT_MAX), FLT_MAX)) {}            // (finite: a logit of -inf weighs nothing)
 };
 // What sums against m are worth against mnew (the larger logit of the two).
@@ -78,9 +79,16 @@ __device__ __forceinline__ float rescale(float m, float mnew, float c0) {
 struct PackedPlan {
   int tiles;         // bound on the row tiles of one key head
   int slices;        // key slices (workgroups per row tile)
+  int pieces;        // blocks of packed_combine_kernel per row tile
   float c0;          // scale log2 e
+  int G;             // query heads of a key head
+  double inv_g;      // 1 / G
   float* part;       // slices > 1: per (tile, head, slice) unnormalised O [R][DP], then (m, l) [R][2]
+  int4* found;       // slices > 1: per tile, its sequence and its index there, for the join: (q0, lq, lk, tile), (k0, ...)
 };
+
+// r / G without a division: (r + 0.5) / G is at least 0.5 / G away from a whole number.
+__device__ __forceinline__ int token_of(const PackedPlan& pl, int r) { return (int)(((double)r + 0.5) * pl.inv_g); }
 
 // Tile sizes.  KC: 16-dim steps of q.k that hold data; DP: head dim padded to whole 32-dim blocks.
 template <int KC>
@@ -116,14 +124,17 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, const int32_t* len,
 // Tile `idx` of the sequences' row tiles of R rows each, laid end to end: its sequence and its index
 // there, or false past the last.  All lanes of the wave take part; the results are uniform.
 template <int R>
-__device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, int idx, Seq& s, int& tile, int& ntiles) {
-  const int lane = threadIdx.x & 63, G = a.H / a.Hkv;
+__device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, const PackedPlan& pl, int idx, Seq& s, int& tile, int& ntiles) {
+  const int lane = threadIdx.x & 63;
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
-    int start = 0, n = 0;
-    if (b < a.B) seq_range(a.cu_q, a.len_q, b, a.Tq, start, n);
-    const int nt = (int)(((int64_t)n * G + R - 1) / R);
+    int start = 0, n = 0, k0 = 0, lk = 0;
+    if (b < a.B) {
+      seq_range(a.cu_q, a.len_q, b, a.Tq, start, n);
+      seq_range(a.cu_k, a.len_k, b, a.Tk, k0, lk);
+    }
+    const int nt = (int)(((uint32_t)n * (uint32_t)pl.G + R - 1) / R);      // (rows fit 31 bits)
     int incl = nt;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -135,12 +146,10 @@ __device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, int
       const int src = __builtin_ctzll(past);
       s.q0 = __builtin_amdgcn_readlane(start, src);
       s.lq = __builtin_amdgcn_readlane(n, src);
+      s.k0 = __builtin_amdgcn_readlane(k0, src);
+      s.lk = __builtin_amdgcn_readlane(lk, src);
       ntiles = __builtin_amdgcn_readlane(nt, src);
       tile = idx - base - (__builtin_amdgcn_readlane(incl, src) - ntiles);
-      int k0, lk;
-      seq_range(a.cu_k, a.len_k, b0 + src, a.Tk, k0, lk);
-      s.k0 = __builtin_amdgcn_readfirstlane(k0);
-      s.lk = __builtin_amdgcn_readfirstlane(lk);
       return true;
     }
     base += __builtin_amdgcn_readlane(incl, 63);
@@ -148,9 +157,23 @@ __device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, int
   return false;
 }
 
+// Leaves what find_tile found to packed_combine_kernel (lq = 0: no tile).
+__device__ __forceinline__ void note_tile(const PackedPlan& pl, int idx, bool mine, bool there, const Seq& s, int tile) {
+  if (pl.slices > 1 && mine) {
+    pl.found[2 * idx] = there ? int4{s.q0, s.lq, s.lk, tile} : int4{0, 0, 0, 0};
+    pl.found[2 * idx + 1] = int4{there ? s.k0 : 0, 0, 0, 0};
+  }
+}
+
 // Last key that row r of the sequence sees (-1: none).
-__device__ __forceinline__ int last_key(const Seq& s, int causal, int r, int G) {
-  return causal ? max(min(r / G + s.lk - s.lq, s.lk - 1), -1) : s.lk - 1;
+__device__ __forceinline__ int last_key(const Seq& s, int causal, int r, const PackedPlan& pl) {
+  return causal ? max(min(token_of(pl, r) + s.lk - s.lq, s.lk - 1), -1) : s.lk - 1;
+}
+
+// Element offset of row r in q or out: token, head.
+__device__ __forceinline__ int64_t row_at(const Seq& s, const PackedPlan& pl, int hk, int r, const int64_t (&stride)[2]) {
+  const int token = token_of(pl, r);
+  return (int64_t)(s.q0 + token) * stride[0] + (int64_t)(hk * pl.G + r - token * pl.G) * stride[1];
 }
 
 // Offset of pieces that do not exist.  A tile's last byte lies below it (row strides below 2^25 bytes, 64
@@ -166,11 +189,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, in
 // each for the products, lanes over the dims for the sums.  For rows whose fast result is not
 // finite: there a NaN or infinite value of a key that the row does not see meets a weight of zero.
 template <class E>
-__device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, const Seq& s, int r, int hk, int last, float c0) {
-  const int lane = threadIdx.x & 63, G = a.H / a.Hkv, D = a.D;
-  const int64_t token = s.q0 + r / G;
-  const int h = hk * G + r % G;
-  const uint16_t* q = (const uint16_t*)a.q + token * a.q_s[0] + (int64_t)h * a.q_s[1];
+__device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
+  const int lane = threadIdx.x & 63, D = a.D, last = last_key(s, a.causal, r, pl);
+  const float c0 = pl.c0;
+  const uint16_t* q = (const uint16_t*)a.q + row_at(s, pl, hk, r, a.q_s);
   const uint16_t* k = (const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1];
   const uint16_t* v = (const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1];
   float m = -FLT_MAX, l = 0.f, o[2] = {0.f, 0.f};
@@ -198,7 +220,7 @@ __device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, con
       if (lane + 64 < D) o[1] += px * E::to_float(vr[lane + 64]);
     }
   }
-  uint16_t* out = (uint16_t*)a.out + token * a.o_s[0] + (int64_t)h * a.o_s[1];
+  uint16_t* out = (uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s);
   if (lane < D) out[lane] = last < 0 ? 0 : E::from_float(o[0] / l);
   if (lane + 64 < D) out[lane + 64] = last < 0 ? 0 : E::from_float(o[1] / l);
 }
@@ -211,17 +233,18 @@ struct RowState {
   u32x4 q[KC];                                               // Q operand: dims 16 kk + 8 half .. +7
   f32x16 o[T::DB];
   float m, l, c0;
+  Ref<E> ref;                                                // of m
 
-  __device__ __forceinline__ void init(const sf_packed_attention_args& a, const Seq& s, int r, int hk, float scale_c0) {
-    const int G = a.H / a.Hkv, half = (threadIdx.x >> 5) & 1;
-    const uint16_t* qp = (const uint16_t*)a.q + (int64_t)(s.q0 + r / G) * a.q_s[0] + (int64_t)(hk * G + r % G) * a.q_s[1];
+  __device__ __forceinline__ void init(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
+    const int half = (threadIdx.x >> 5) & 1;
+    const uint16_t* qp = (const uint16_t*)a.q + row_at(s, pl, hk, r, a.q_s);
 #pragma unroll
     for (int kk = 0; kk < KC; ++kk) {
       const int d0 = 16 * kk + 8 * half;
       q[kk] = d0 < a.D ? ld16(qp + d0) : u32x4{0, 0, 0, 0};
     }
     // a negative scale turns the queries over, so that the largest product has the largest logit
-    if (scale_c0 < 0.f)
+    if (pl.c0 < 0.f)
 #pragma unroll
       for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
@@ -232,70 +255,62 @@ struct RowState {
       for (int x = 0; x < 16; ++x) o[db][x] = 0.f;
     m = -FLT_MAX;
     l = 0.f;
-    c0 = fabsf(scale_c0);
+    c0 = fabsf(pl.c0);
+    ref = Ref<E>(m, c0);
   }
 
   // S^T = K Q^T of a tile of 32 NB keys in LDS: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4.
-  template <int NB>
-  __device__ __forceinline__ void products(const uint8_t* kt, f32x16 (&s)[NB]) const {
-    const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
+  // The operands are read kAhead products before they are taken; `between(x)` is issued after product x.
+  template <int NB, class F>
+  __device__ __forceinline__ void products(const uint8_t* kt, f32x16 (&s)[NB], F between) const {
+    const int half = (threadIdx.x >> 5) & 1, li = threadIdx.x & 31;
+    constexpr int kAll = NB * KC, kAhead = kAll < 4 ? kAll : 4;
+    const auto operand = [&](int x) __attribute__((always_inline)) {
+      const int key = 32 * (x % NB) + li;
+      return ld16(kt + key * T::kRow + (T::kpiece(key, 2 * (x / NB) + half) << 4));
+    };
+    u32x4 k[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) k[x] = operand(x);
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < KC; ++kk)
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb) {
-        const int key = 32 * kb + li;
-        s[kb] = E::mfma(ld16(kt + key * T::kRow + (T::kpiece(key, 2 * kk + half) << 4)), q[kk], s[kb]);
-      }
-    // the reads run kAhead operands before the products that take them
-    constexpr int kAhead = NB * KC < 4 ? NB * KC : 4;
-    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-    for (int x = 0; x < NB * KC - kAhead; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    for (int x = 0; x < kAll; ++x) {
+      s[x % NB] = E::mfma(k[x % kAhead], q[x / NB], s[x % NB]);
+      if (x + kAhead < kAll) k[x % kAhead] = operand(x + kAhead);
+      between(x);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
   }
 
-  // The rest of a tile, its V rows in LDS.  `last`: the last key of the tile that the lane's row sees
-  // (partial: tiles where a row sees less than all).
+  // Weight 0 for the keys past `last`, of the tile.
   template <int NB>
-  __device__ __forceinline__ void weigh(f32x16 (&s)[NB], const uint8_t* vt, bool partial, int last) {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    if (partial) {
-      last -= 4 * half;                                      // (so that the keys are constants)
+  __device__ __forceinline__ void hide(f32x16 (&s)[NB], int last) const {
+    last -= 4 * ((threadIdx.x >> 5) & 1);                    // (so that the keys are constants)
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int x = 0; x < 16; ++x)
-          s[kb][x] = 32 * kb + 8 * (x >> 2) + (x & 3) > last ? -INFINITY : s[kb][x];
-    }
-    // Weights against a reference point that stays where an earlier tile put it, until a tile's
-    // weights sum to more than the limit (as those of the first do): no running maximum, exp or
-    // rescale of O in the others.
-    uint32_t p[8 * NB];
-    auto weights = [&]() __attribute__((always_inline)) {
-      const Ref<E> ref(m, c0);
-      float t0 = 0.f, t1 = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w0 = fast_exp2(__builtin_fmaf(s[kb][2 * e], ref.c, -ref.mc));
-          const float w1 = fast_exp2(__builtin_fmaf(s[kb][2 * e + 1], ref.c, -ref.mc));
-          // rounded to 16 bits for the matrix product; the sum takes the rounded weights, so that
-          // they still average to one
-          p[8 * kb + e] = E::pack(w0, w1);
-          if (e & 1) t1 = E::sum2(p[8 * kb + e], t1); else t0 = E::sum2(p[8 * kb + e], t0);
-        }
-      return t0 + t1;
-    };
-    float sum = weights();
-    if (__any(!(sum <= E::kMassLimit))) {
+      for (int x = 0; x < 16; ++x) s[kb][x] = 32 * kb + 8 * (x >> 2) + (x & 3) > last ? -INFINITY : s[kb][x];
+  }
+
+  // Weights against a reference point that stays where an earlier tile put it, until a tile's weights
+  // sum to more than the limit (as those of the first do): no running maximum, exp or rescale of O in
+  // the others.  Pair x of the tile's weights: rounded to 16 bits for the matrix product; the sum
+  // takes the rounded weights, so that they still average to one.
+  template <int NB>
+  __device__ __forceinline__ void weight_pair(const f32x16 (&s)[NB], int x, uint32_t (&p)[8 * NB], float (&sum)[2]) const {
+    const float w0 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7)], ref.c, -ref.mc));
+    const float w1 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7) + 1], ref.c, -ref.mc));
+    p[x] = E::pack(w0, w1);
+    sum[x & 1] = E::sum2(p[x], sum[x & 1]);
+  }
+
+  // The tile's sum of weights accepted, or the reference point moved and the weights formed again.
+  template <int NB>
+  __device__ __forceinline__ void settle(const f32x16 (&s)[NB], uint32_t (&p)[8 * NB], float (&sum)[2]) {
+    if (__any(!(sum[0] + sum[1] <= E::kMassLimit))) {
       float mx = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
@@ -309,35 +324,54 @@ struct RowState {
       for (int db = 0; db < T::DB; ++db)
 #pragma unroll
         for (int x = 0; x < 16; ++x) o[db][x] *= w;
-      sum = weights();
+      ref = Ref<E>(m, c0);
+      sum[0] = sum[1] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum);
     }
-    l += sum;
-    // O^T += V^T P^T; a 16-lane group of the transposing read takes 4 keys x 16 dims
-    const int grp = lane >> 4, ekey = (lane & 15) >> 2, q4 = lane & 3;
+    l += sum[0] + sum[1];
+  }
+
+  // V^T operand x = c2 DB + db of a tile: keys 16 c2 + 8 (e / 4) + 4 half + e % 4 (the order of P^T), dim
+  // 32 db + li.  A 16-lane group of the transposing read takes 4 keys x 16 dims.
+  static __device__ __forceinline__ u32x4 value_operand(const uint8_t* vt, int x) {
+    const int lane = threadIdx.x & 63, grp = lane >> 4, ekey = (lane & 15) >> 2, q4 = lane & 3;
+    const int c2 = x / T::DB, d = 32 * (x % T::DB) + 16 * (grp & 1) + 4 * q4;
+    u32x2 part[2];
 #pragma unroll
-    for (int c2 = 0; c2 < 2 * NB; ++c2) {
-      const u32x4 pb = {p[4 * c2], p[4 * c2 + 1], p[4 * c2 + 2], p[4 * c2 + 3]};
-#pragma unroll
-      for (int db = 0; db < T::DB; ++db) {
-        const int d = 32 * db + 16 * (grp & 1) + 4 * q4;
-        u32x2 part[2];
-#pragma unroll
-        for (int rd = 0; rd < 2; ++rd) {
-          const int key = 16 * c2 + 8 * rd + 4 * (grp >> 1) + ekey;
-          const uint8_t* at = vt + key * T::kRow + (T::vpiece(key, d >> 3) << 4) + ((d >> 2) & 1) * 8;
-          part[rd] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16p*)at));
-        }
-        o[db] = E::mfma(u32x4{part[0][0], part[0][1], part[1][0], part[1][1]}, pb, o[db]);
-      }
+    for (int rd = 0; rd < 2; ++rd) {
+      const int key = 16 * c2 + 8 * rd + 4 * (grp >> 1) + ekey;
+      const uint8_t* at = vt + key * T::kRow + (T::vpiece(key, d >> 3) << 4) + ((d >> 2) & 1) * 8;
+      part[rd] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16p*)at));
     }
-    constexpr int kProducts = 2 * NB * T::DB, kAhead = kProducts < 4 ? kProducts : 4;
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 1);
+    return u32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
+  }
+
+  // O^T += V^T P^T, the operands read kAhead products before they are taken.  `between(x)` is issued
+  // after product x.
+  template <int NB, class F>
+  __device__ __forceinline__ void gather(const uint32_t (&p)[8 * NB], const uint8_t* vt, F between) {
+    constexpr int kAll = 2 * NB * T::DB, kAhead = kAll < 4 ? kAll : 4;
+    u32x4 v[kAhead];
 #pragma unroll
-    for (int x = 0; x < kProducts - kAhead; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    for (int x = 0; x < kAhead; ++x) v[x] = value_operand(vt, x);
+#pragma unroll
+    for (int x = 0; x < kAll; ++x) {
+      const int c2 = x / T::DB, db = x % T::DB;
+      o[db] = E::mfma(v[x % kAhead], u32x4{p[4 * c2], p[4 * c2 + 1], p[4 * c2 + 2], p[4 * c2 + 3]}, o[db]);
+      if (x + kAhead < kAll) v[x % kAhead] = value_operand(vt, x + kAhead);
+      between(x);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 1);
+  }
+
+  // A tile's weights in one go.
+  template <int NB>
+  __device__ __forceinline__ void weights(const f32x16 (&s)[NB], uint32_t (&p)[8 * NB]) {
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum);
+    settle<NB>(s, p, sum);
   }
 
   // Zero where every accumulator is finite, NaN otherwise.
@@ -406,7 +440,7 @@ template <class E, int KC, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
   constexpr int kTile = 64 * T::kRow, R = 32 * NW;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];     // two buffers of K, V
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];     // two buffers of K, V
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
@@ -414,58 +448,69 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
   const int slice = rest % pl.slices, idx = rest / pl.slices;
   Seq s;
   int tile, ntiles;
-  if (!find_tile<R>(a, idx, s, tile, ntiles)) return;
+  const bool there = find_tile<R>(a, pl, idx, s, tile, ntiles);
+  note_tile(pl, idx, hk + slice == 0 && tid == 0, there, s, ntiles - 1 - tile);
+  if (!there) return;
   tile = ntiles - 1 - tile;                                  // causal: the longest rows first
-  const int G = a.H / a.Hkv, rows = s.lq * G, r0 = tile * R + wave * 32;
+  const int rows = s.lq * pl.G, r0 = tile * R + wave * 32;
   const int row = min(r0 + li, rows - 1);                    // rows past the end repeat the last
-  const int seen = last_key(s, a.causal, min(tile * R + R, rows) - 1, G) + 1;   // keys the workgroup's last row sees
+  const int seen = last_key(s, a.causal, min(tile * R + R, rows) - 1, pl) + 1;   // keys the workgroup's last row sees
   const int n_all = (seen + 63) / 64;
-  const int t_lo = (int)((int64_t)n_all * slice / pl.slices), t_hi = (int)((int64_t)n_all * (slice + 1) / pl.slices);
+  const int per = (n_all + pl.slices - 1) / pl.slices, t_lo = min(slice * per, n_all), t_hi = min(t_lo + per, n_all);
 
   RowState<E, KC> st;
-  st.init(a, s, row, hk, pl.c0);
-  const int mine = last_key(s, a.causal, row, G);
+  st.init(a, pl, s, row, hk);
+  const int mine = last_key(s, a.causal, row, pl);
   // of this wave's rows: the fewest and the most keys
-  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0, rows - 1), G));
-  const int high = r0 < rows ? __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0 + 31, rows - 1), G)) : -1;
+  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0, rows - 1), pl));
+  const int high = r0 < rows ? __builtin_amdgcn_readfirstlane(last_key(s, a.causal, min(r0 + 31, rows - 1), pl)) : -1;
 
   if (t_lo < t_hi) {
     Stage<KC, 64, 64 * NW> ks, vs;
     ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], tid, a.D);
     vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], tid, a.D);
-    ks.load(64 * (t_hi - 1), s.lk, true);
-    vs.load(64 * (t_hi - 1), s.lk, true);
-    ks.template store<false>(smem, tid);
-    vs.template store<true>(smem + kTile, tid);
-    ks.load(64 * (t_hi - 2), s.lk, t_hi - 2 >= t_lo);
-    vs.load(64 * (t_hi - 2), s.lk, t_hi - 2 >= t_lo);
+    int t = t_hi - 1;
+    ks.load(64 * t, s.lk, true);
+    vs.load(64 * t, s.lk, true);
+    // tile t in buffer t & 1
+    const auto kt = [&](int buf) __attribute__((always_inline)) { return smem + buf * 2 * kTile; };
+    const auto vt = [&](int buf) __attribute__((always_inline)) { return smem + buf * 2 * kTile + kTile; };
+    ks.template store<false>(kt(t & 1), tid);
+    vs.template store<true>(vt(t & 1), tid);
+    ks.load(64 * (t - 1), s.lk, t - 1 >= t_lo);
+    vs.load(64 * (t - 1), s.lk, t - 1 >= t_lo);
     lds_only_barrier();
-    int t = t_hi - 1, buf = 0;
-    auto refill = [&]() __attribute__((always_inline)) {     // the next tile to the other buffer, the one after it on its way
-      uint8_t* next = smem + (buf ^ 1) * 2 * kTile;
-      ks.template store<false>(next, tid);
-      vs.template store<true>(next + kTile, tid);
-      ks.load(64 * (t - 2), s.lk, t - 1 > t_lo);
-      vs.load(64 * (t - 2), s.lk, t - 1 > t_lo);
-    };
-    auto step = [&](auto partial) __attribute__((always_inline)) {
-      refill();
-      const uint8_t* kt = smem + buf * 2 * kTile;
-      f32x16 sc[2];
-      st.template products<2>(kt, sc);
-      st.template weigh<2>(sc, kt + kTile, decltype(partial)::value, mine - 64 * t);
+    for (; t >= t_lo && 64 * t > high; --t) {                // tiles that none of this wave's rows sees
+      ks.template store<false>(kt(~t & 1), tid);
+      vs.template store<true>(vt(~t & 1), tid);
+      ks.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
+      vs.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
       lds_only_barrier();
-      --t;
-      buf ^= 1;
-    };
-    for (; t >= t_lo && 64 * t > high;) {                    // tiles that none of this wave's rows sees
-      refill();
-      lds_only_barrier();
-      --t;
-      buf ^= 1;
     }
-    while (t >= t_lo && 64 * t + 63 > low) step(std::true_type{});
-    while (t >= t_lo) step(std::false_type{});
+    // (the buffers as constants: LDS addresses are formed once)
+    auto step = [&](auto buffer) __attribute__((always_inline)) {
+      constexpr int B = decltype(buffer)::value;
+      f32x16 sc[2];
+      // meanwhile the next tile goes to the other buffer, and the one after it is asked for
+      st.template products<2>(kt(B), sc, [&](int x) __attribute__((always_inline)) {
+        if (x == 0) ks.template store<false>(kt(B ^ 1), tid);
+        if (x == 1) vs.template store<true>(vt(B ^ 1), tid);
+        if (x == 2) ks.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
+        if (x == 3) vs.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
+      });
+      if (64 * t + 63 > low) st.template hide<2>(sc, mine - 64 * t);
+      uint32_t p[16];
+      st.template weights<2>(sc, p);
+      st.template gather<2>(p, vt(B), [](int) {});
+      lds_only_barrier();
+      --t;
+    };
+    if (t >= t_lo && (t & 1)) step(std::integral_constant<int, 1>{});
+    while (t >= t_lo) {
+      step(std::integral_constant<int, 0>{});
+      if (t < t_lo) break;
+      step(std::integral_constant<int, 1>{});
+    }
   }
   if (r0 >= rows) return;                                    // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
@@ -484,7 +529,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
   // rows to be done again (see exact_row): either half's accumulators are not finite
   const uint64_t badl = __ballot(a.causal && !(st.finite_probe() == 0.f) && r0 + li < rows);
   uint32_t bad = (uint32_t)badl | (uint32_t)(badl >> 32);
-  uint16_t* op = (uint16_t*)a.out + (int64_t)(s.q0 + row / G) * a.o_s[0] + (int64_t)(hk * G + row % G) * a.o_s[1];
+  uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, row, a.o_s);
   const bool write = r0 + li < rows && !(bad >> li & 1);
 #pragma unroll
   for (int db = 0; db < T::DB; ++db)
@@ -501,7 +546,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
     }
   for (; bad != 0; bad &= bad - 1) {
     const int r = r0 + __builtin_ctz(bad);
-    exact_row<E>(a, s, r, hk, last_key(s, a.causal, r, G), pl.c0);
+    exact_row<E>(a, pl, s, r, hk);
   }
 }
 
@@ -522,18 +567,20 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   const int slice = rest % pl.slices, idx = rest / pl.slices;
   Seq s;
   int tile, ntiles;
-  if (!find_tile<32>(a, idx, s, tile, ntiles)) return;
-  const int G = a.H / a.Hkv, rows = s.lq * G, r0 = tile * 32;
+  const bool there = find_tile<32>(a, pl, idx, s, tile, ntiles);
+  note_tile(pl, idx, hk + slice == 0 && tid == 0, there, s, tile);
+  if (!there) return;
+  const int rows = s.lq * pl.G, r0 = tile * 32;
   const int row = min(r0 + li, rows - 1);
-  const int seen = last_key(s, a.causal, min(r0 + 32, rows) - 1, G) + 1;
-  const int n_all = (seen + KT - 1) / KT, z = slice * 4 + wave, Z = pl.slices * 4;
-  const int t_lo = (int)((int64_t)n_all * z / Z), t_hi = (int)((int64_t)n_all * (z + 1) / Z);
-  const int mine = last_key(s, a.causal, row, G);
-  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, r0, G));
+  const int seen = last_key(s, a.causal, min(r0 + 32, rows) - 1, pl) + 1;
+  const int n_all = (seen + KT - 1) / KT, Z = pl.slices * 4;
+  const int per = (n_all + Z - 1) / Z, t_lo = min((slice * 4 + wave) * per, n_all), t_hi = min(t_lo + per, n_all);
+  const int mine = last_key(s, a.causal, row, pl);
+  const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, r0, pl));
   uint8_t* vt = smem + wave * kWave;
   {
     RowState<E, KC> st;
-    st.init(a, s, row, hk, pl.c0);
+    st.init(a, pl, s, row, hk);
     if (t_lo < t_hi) {
       const char* kbase = (const char*)((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1]);
       const int64_t krow = a.k_s[0] * 2;
@@ -566,7 +613,10 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
         vs.template store<true>(vt, lane);
         load_k(KT * (t - 1), t > t_lo);
         vs.load(KT * (t - 1), s.lk, t > t_lo);
-        st.template weigh<NB>(sc, vt, KT * t + KT - 1 > low, mine - KT * t);
+        if (KT * t + KT - 1 > low) st.template hide<NB>(sc, mine - KT * t);
+        uint32_t p[8 * NB];
+        st.template weights<NB>(sc, p);
+        st.template gather<NB>(p, vt, [](int) {});
       }
     }
     // the slice's O over the wave's tiles, for all threads
@@ -618,66 +668,116 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   const int r = r0 + jr;
   const uint64_t bad8 = __ballot(a.causal && !(probe == 0.f) && r < rows);   // a byte for each of the wave's 8 rows
   if (r < rows && !(bad8 >> (lane & 56) & 0xff)) {
-    const float inv = last_key(s, a.causal, r, G) < 0 ? 0.f : 1.f / l;
-    uint16_t* op = (uint16_t*)a.out + (int64_t)(s.q0 + r / G) * a.o_s[0] + (int64_t)(hk * G + r % G) * a.o_s[1];
+    const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / l;
+    uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
       if (32 * db + jd < a.D)
         *reinterpret_cast<u32x2*>(op + 32 * db + jd) = u32x2{E::pack(o[db][0] * inv, o[db][1] * inv), E::pack(o[db][2] * inv, o[db][3] * inv)};
   }
   for (int x = 0; x < 8; ++x)
-    if (bad8 >> (8 * x) & 0xff) exact_row<E>(a, s, r0 + wave * 8 + x, hk, last_key(s, a.causal, r0 + wave * 8 + x, G), pl.c0);
+    if (bad8 >> (8 * x) & 0xff) exact_row<E>(a, pl, s, r0 + wave * 8 + x, hk);
 }
 
-// Joins the key slices of a row, a wave per row: o = sum_z w_z O_z / sum_z w_z l_z with w_z the worth of
-// slice z's reference point against the largest.  R: rows of a tile.
+// Joins the key slices: o = sum_z w_z O_z / sum_z w_z l_z with w_z the worth of slice z's reference point
+// against the largest.  LR lanes of 4 dims take a row.  R: rows of a tile; pl.pieces blocks share a
+// tile.  From packed_stream_kernel (R = 32: few rows, up to 64 slices) a block takes a row at a time, its
+// lane groups the slices z, z + GROUPS, .., joined through LDS; from packed_tile_kernel (few slices) a
+// group takes a row and a block 32 of them.
 template <class E, int DP, int R>
 __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int quad = blockIdx.x % (R / 4), rest = blockIdx.x / (R / 4), hk = rest % a.Hkv, idx = rest / a.Hkv;
-  Seq s;
-  int tile, ntiles;
-  if (!find_tile<R>(a, idx, s, tile, ntiles)) return;
-  if (R > 32) tile = ntiles - 1 - tile;                      // as packed_tile_kernel takes them
-  const int G = a.H / a.Hkv, in = quad * 4 + wave, r = tile * R + in;
-  if (r >= s.lq * G) return;
-  const float* part = pl.part + ((int64_t)idx * a.Hkv + hk) * pl.slices * R * (DP + 2);
+  constexpr int LR = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, GROUPS = 256 / LR;
+  constexpr bool kOneRow = R == 32;
+  constexpr int ROWS = kOneRow ? 1 : 32, PASSES = kOneRow ? 1 : ROWS / GROUPS;
   constexpr int64_t kStep = R * (DP + 2);
-  float m = -FLT_MAX, l = 0.f;
-  if (lane < pl.slices) {                                    // slices <= 64
-    const f32x2 v = *reinterpret_cast<const f32x2*>(part + lane * kStep + R * DP + 2 * in);
-    m = v[0];
-    l = v[1];
-  }
-  float mx = m;
+  __shared__ f32x4 so[kOneRow ? GROUPS : 1][LR];
+  __shared__ f32x2 sml[GROUPS];
+  const int tid = threadIdx.x, lane = tid & 63, group = tid / LR, d = 4 * (tid % LR);
+  const int piece = blockIdx.x % pl.pieces, rest = blockIdx.x / pl.pieces, hk = rest % a.Hkv, idx = rest / a.Hkv;
+  const int4 f0 = pl.found[2 * idx];
+  const Seq s = {f0.x, f0.y, pl.found[2 * idx + 1].x, f0.z};
+  const int rows = s.lq * pl.G, r0 = f0.w * R;
+  const float* part = pl.part + ((int64_t)idx * a.Hkv + hk) * pl.slices * kStep;
+  const float c0 = fabsf(pl.c0);
+  for (int in0 = piece * ROWS; in0 < R && r0 + in0 < rows; in0 += pl.pieces * ROWS) {      // (uniform over the block)
+    f32x4 o[PASSES];
+    float sum[PASSES];
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-  const float w = lane < pl.slices ? rescale<E>(m, mx, fabsf(pl.c0)) : 0.f;
-  const float sum = wave_sum(w * l);
-  __shared__ float worth[4][64];
-  worth[wave][lane] = w;
-  asm volatile("" ::: "memory");                             // (a wave's LDS accesses are in order)
-  const int d = 2 * lane;
-  f32x2 o = {0.f, 0.f};
-  if (d < DP) {
-    const float* po = part + in * DP + d;
-#pragma unroll 8
-    for (int z = 0; z < pl.slices; ++z) {
-      const f32x2 v = *reinterpret_cast<const f32x2*>(po + z * kStep);
-      const float wz = worth[wave][z];
-      o[0] += wz * v[0];
-      o[1] += wz * v[1];
+    for (int x = 0; x < PASSES; ++x) {
+      const int in = kOneRow ? in0 : in0 + x * GROUPS + group;
+      const int z0 = kOneRow ? group : 0, dz = kOneRow ? GROUPS : 1;
+      const float* ml = part + R * DP + 2 * in;
+      const float* po = part + in * DP + d;
+      float m = -FLT_MAX, l = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      if (r0 + in < rows && d < DP) {
+        for (int z = z0; z < pl.slices; z += 4 * dz) {
+          f32x2 v[4];
+          f32x4 ov[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const bool in_range = z + y * dz < pl.slices;
+            const int64_t at = (in_range ? z + y * dz : z) * kStep;
+            v[y] = *reinterpret_cast<const f32x2*>(ml + at);
+            ov[y] = *reinterpret_cast<const f32x4*>(po + at);
+            if (!in_range) v[y] = f32x2{-FLT_MAX, 0.f};
+            if (!in_range) ov[y] = f32x4{0.f, 0.f, 0.f, 0.f};   // (whatever it weighs: it may not be finite)
+          }
+          float mx = m;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) mx = fmaxf(mx, v[y][0]);
+          const float w0 = rescale<E>(m, mx, c0);
+          m = mx;
+          l *= w0;
+          acc *= w0;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float w = rescale<E>(v[y][0], mx, c0);
+            l += w * v[y][1];
+            acc += w * ov[y];
+          }
+        }
+      }
+      if (kOneRow) {                                         // the groups' shares of the row
+        so[group][tid % LR] = acc;
+        if (d == 0) sml[group] = f32x2{m, l};
+        __syncthreads();
+        m = -FLT_MAX;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, sml[g][0]);
+        l = 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const float w = rescale<E>(sml[g][0], m, c0);
+          l += w * sml[g][1];
+          acc += w * so[g][tid % LR];
+        }
+        __syncthreads();                                     // (the shares may be overwritten)
+      }
+      o[x] = acc;
+      sum[x] = l;
+    }
+    if (kOneRow && tid >= 64) continue;
+#pragma unroll
+    for (int x = 0; x < PASSES; ++x) {
+      const int in = kOneRow ? in0 : in0 + x * GROUPS + group, r = r0 + in;
+      const bool mine = r < rows && d < a.D && (!kOneRow || tid < LR);
+      float probe = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[x][e], 0.f, probe);
+      const uint64_t bad = __ballot(a.causal && mine && !(probe == 0.f));
+      const uint64_t lanes = ((1ull << LR) - 1) << (lane / LR * LR);
+      if (mine && !(bad & lanes)) {
+        const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / sum[x];
+        *reinterpret_cast<u32x2*>((uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s) + d) =
+            u32x2{E::pack(o[x][0] * inv, o[x][1] * inv), E::pack(o[x][2] * inv, o[x][3] * inv)};
+      }
+#pragma unroll
+      for (int g = 0; g < 64 / LR; ++g)
+        if (bad >> (g * LR) & ((1ull << LR) - 1)) exact_row<E>(a, pl, s, kOneRow ? r : r0 + in0 + x * GROUPS + tid / 64 * (64 / LR) + g, hk);
     }
   }
-  const int last = last_key(s, a.causal, r, G);
-  if (a.causal && __any(!(__builtin_fmaf(o[0], 0.f, o[1] * 0.f) == 0.f))) {
-    exact_row<E>(a, s, r, hk, last, pl.c0);
-    return;
-  }
-  const float inv = last < 0 ? 0.f : 1.f / sum;
-  if (d < a.D)
-    *reinterpret_cast<uint32_t*>((uint16_t*)a.out + (int64_t)(s.q0 + r / G) * a.o_s[0] + (int64_t)(hk * G + r % G) * a.o_s[1] + d) =
-        E::pack(o[0] * inv, o[1] * inv);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -700,8 +800,8 @@ int route(const sf_packed_attention_args* a, Route& r) {
   if (a->dtype != SF_DTYPE_BF16 && a->dtype != SF_DTYPE_F16) { sf_set_error("packed attention: element type %d", a->dtype); return 1; }
   if (!(fabsf(a->scale) <= 1e30f)) { sf_set_error("packed attention: scale %g is not finite or above 1e30", (double)a->scale); return 1; }
   const int G = a->H / a->Hkv;
-  if (a->Tk > INT32_MAX || a->Tq * G > INT32_MAX) {
-    sf_set_error("packed attention: %lld query rows or %lld keys exceed 2^31 - 1", (long long)(a->Tq * G), (long long)a->Tk);
+  if (a->Tk > 1 << 30 || a->Tq > (1 << 30) / G) {
+    sf_set_error("packed attention: %lld queries of %d heads a key head, or %lld keys, exceed 2^30", (long long)a->Tq, G, (long long)a->Tk);
     return 1;
   }
   if (a->Tq > 0 && (a->q == nullptr || a->out == nullptr || (a->Tk > 0 && (a->k == nullptr || a->v == nullptr)))) {
@@ -722,41 +822,65 @@ int route(const sf_packed_attention_args* a, Route& r) {
   r.kc = a->D <= 32 ? 2 : a->D <= 48 ? 3 : a->D <= 64 ? 4 : a->D <= 96 ? 6 : 8;
   r.dp = 32 * ((r.kc + 1) / 2);
   const int64_t rows = a->Tq * G;
-  const int64_t keys = (a->Tk + a->B - 1) / a->B;            // of a sequence, on average
-  r.nw = rows > 64ll * a->B ? 4 : 0;
+  // keys that a row of an average sequence sees, on average
+  int64_t seen = (a->Tk + a->B - 1) / a->B;
+  if (a->causal) seen -= seen < a->Tq / a->B ? seen / 2 : a->Tq / a->B / 2;
+  // Up to 64 rows a sequence stream their keys.  Above, tiles of 128 rows; of 256 (half the reads of K and V)
+  // where head dims above 64 meet long rows and two workgroups a CU: prompt of 8192, 32 / 8 heads of 128, 128 and 256
+  // rows 548 / 512 us, 2048 (256 workgroups) 55 / 75; 8 of 512 41 / 45; 8192, 16 heads of 64 170 / 172.
+  r.nw = rows <= 64ll * a->B ? 0 : r.kc > 4 && seen >= 1024 && rows / 256 * a->Hkv >= 512 ? 8 : 4;
   const int R = r.nw ? 32 * r.nw : 32;
   // tiles end at sequence ends: sum_b ceil(rows_b / R) <= rows / R + B
   const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
-  const int64_t base = tiles * a->Hkv;
-  // few workgroups: slices of the keys, at least 4 tiles (a wave's 2) long each
-  const int64_t want = (512 + base - 1) / base, most = r.nw ? keys / 512 : keys / 512;
-  int64_t slices = want < most ? want : most;
+  const int64_t full = (rows + R - 1) / R, wgs = (full > a->B ? full : a->B) * a->Hkv;
+  int64_t slices;
+  if (r.nw) {
+    // Few workgroups: slices of the keys.  Two workgroups a CU where a slice keeps 1024 keys, else one, and
+    // no slice below 512 (prompt of 512 over 8192 keys, 32 / 8 heads of 128, 1 / 2 / 4 slices: 152 / 95 / 85 us;
+    // 128 over 8192, 1 / 4 / 8 / 16: 144 / 50 / 37 / 42; 1024 over 1024, 16 heads of 64, 1 / 2: 18.3 / 20.6).
+    slices = 512 / wgs;
+    if (slices > 1 && seen / slices < 1024) slices = 256 / wgs;
+    if (slices > seen / 512) slices = seen / 512;
+    if (r.nw == 8) slices = 1;                               // (512 workgroups and more)
+  } else {
+    const int64_t least = r.dp > 64 ? 128 : 256;
+    slices = 256 / wgs;
+    if (slices > seen / least) slices = seen / least;
+  }
   slices = slices < 1 ? 1 : slices > 64 ? 64 : slices;
+  // rows of a tile join in blocks of 32, or -- packed_stream_kernel -- one by one, as many blocks as a
+  // sequence has rows on average
+  int64_t pieces = r.nw ? r.nw : (rows + a->B - 1) / a->B;
+  if (pieces > 32) pieces = 32;
   float c0 = a->scale * SF_LOG2E;
   if (fabsf(c0) < FLT_MIN) c0 = FLT_MIN;                     // all logits equal; a masked one stays -inf
-  r.pl = PackedPlan{(int)tiles, (int)slices, c0, nullptr};
-  r.wgs = base * slices;
-  if (r.wgs > INT32_MAX || tiles * a->Hkv * (R / 4) > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
+  r.pl = PackedPlan{(int)tiles, (int)slices, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr};
+  r.wgs = tiles * a->Hkv * slices;
+  if (r.wgs > INT32_MAX || tiles * a->Hkv * 32 > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
   return 0;
 }
 
 size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
   if (r.pl.slices <= 1) return 0;
   const int R = r.nw ? 32 * r.nw : 32;
-  return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float);
+  return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float) + (size_t)r.pl.tiles * 2 * sizeof(int4);
 }
 
 template <class E, int KC>
 int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
   const dim3 grid((unsigned)r.wgs);
-  if (r.nw == 4) hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4>), grid, dim3(256), 0, st, *a, r.pl);
-  else hipLaunchKernelGGL((packed_stream_kernel<E, KC>), grid, dim3(256), 0, st, *a, r.pl);
+  if (r.nw == 0) {
+    hipLaunchKernelGGL((packed_stream_kernel<E, KC>), grid, dim3(256), 0, st, *a, r.pl);
+  } else if (r.nw == 4) {
+    hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4>), grid, dim3(256), 0, st, *a, r.pl);
+  } else if constexpr (KC > 4) {
+    hipLaunchKernelGGL((packed_tile_kernel<E, KC, 8>), grid, dim3(512), 0, st, *a, r.pl);
+  }
   const int rc = sf_check_launch(r.nw ? "packed_tile_kernel" : "packed_stream_kernel");
   if (rc || r.pl.slices <= 1) return rc;
-  const int R = r.nw ? 32 * r.nw : 32;
-  const dim3 gc((unsigned)(r.pl.tiles * a->Hkv * (R / 4)));
-  constexpr int DP = Dims<KC>::DP;
-  if (r.nw == 4) hipLaunchKernelGGL((packed_combine_kernel<E, DP, 128>), gc, dim3(256), 0, st, *a, r.pl);
+  const dim3 gc((unsigned)(r.pl.tiles * a->Hkv * r.pl.pieces));
+  constexpr int DP = Dims<KC>::DP;                           // (tiles of 256 rows are never sliced)
+  if (r.nw) hipLaunchKernelGGL((packed_combine_kernel<E, DP, 128>), gc, dim3(256), 0, st, *a, r.pl);
   else hipLaunchKernelGGL((packed_combine_kernel<E, DP, 32>), gc, dim3(256), 0, st, *a, r.pl);
   return sf_check_launch("packed_combine_kernel");
 }
@@ -791,6 +915,7 @@ extern "C" int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, vo
     return 1;
   }
   r.pl.part = static_cast<float*>(workspace);
+  r.pl.found = reinterpret_cast<int4*>(r.pl.part + r.wgs * (r.nw ? 32 * r.nw : 32) * (r.dp + 2));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == SF_DTYPE_BF16 ? launch_type<Bf16>(a, r, st) : launch_type<Fp16>(a, r, st);
 }

@@ -113,6 +113,34 @@ def test_key_slices(dtype, D, n, m):
   assert torch.equal(out, ops.packed_attention(q, k, v, offsets([n]), offsets([m]), causal=True))
 
 
+@pytest.mark.parametrize("dtype,D,lens,heads,causal", [("bf16", 128, [4100], (32, 8), True), ("fp16", 96, [1100, 2300, 7, 1500], (48, 24), False),
+                                                       ("bf16", 80, [5000, 3333], (24, 6), True)])
+def test_long_rows(dtype, D, lens, heads, causal):
+  """Enough long rows for the widest tiles; every 97th row and the last ones."""
+  H, Hk = heads
+  q, k, v = make(lens, lens, H, Hk, D, TYPES[dtype], D)
+  out = ops.packed_attention(q, k, v, offsets(lens), causal=causal)
+  assert torch.isfinite(out.float()).all()
+  at = 0
+  for n in lens:
+    rows = torch.tensor(sorted(set(range(0, n, 97)) | set(range(max(n - 40, 0), n))))
+    for h in range(0, H, 5):
+      kk, vv = k[at:at + n, h // (H // Hk)][:, None], v[at:at + n, h // (H // Hk)][:, None]
+      for r in rows.split(64):
+        # the sampled rows one by one as sequences of one query over the keys they see
+        s = (q[at + r.to(DEV), h].double() @ kk[:, 0].double().T) / math.sqrt(D)
+        seen = torch.arange(n, device=DEV)[None] <= r.to(DEV)[:, None] if causal else torch.ones(len(r), n, dtype=torch.bool, device=DEV)
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        want, a = p @ vv[:, 0].double(), p @ vv[:, 0].double().abs()
+        u = torch.finfo(TYPES[dtype]).eps / 2
+        size = (q[at + r.to(DEV), h].double().abs() @ kk[:, 0].double().abs().T / math.sqrt(D)).amax(-1, keepdim=True)
+        tol = 2 * (u + (D + 8) * 2.0 ** -23 * size + n * 2.0 ** -24) * a + u * want.abs()
+        if dtype == "fp16":
+          tol = tol + n * 2.0 ** -25 * vv.double().abs().amax()
+        assert ((out[at + r.to(DEV), h].double() - want).abs() <= tol).all()
+    at += n
+
+
 @pytest.mark.parametrize("n", [1, 40, 300])
 def test_caches_with_free_rows(n):
   """Keys in caches of 600 rows each, the free rows NaN; queries of a padded batch."""
