@@ -601,17 +601,16 @@ def _no_grad(what: str, *ts) -> None:
         raise ValueError(f"{what}: has no backward pass; detach the inputs or call it under torch.no_grad()")
 
 
-def _on_device(t: torch.Tensor):
-  """Context that makes t's device current for a launch (None where it is already)."""
-  return None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(fn, t: torch.Tensor, what: str, *args) -> None:
-  ctx = _on_device(t)
-  if ctx is None:
+  """``fn(*args, stream)`` with t's device current."""
+  index = t.get_device()
+  if index == _current_device():
     _lib.check(fn(*args, _stream(t)), what)
   else:
-    with ctx:
+    with torch.cuda.device(index):
       _lib.check(fn(*args, _stream(t)), what)
 
 
@@ -619,8 +618,10 @@ def _strides2(t: torch.Tensor) -> tuple[int, int]:
   """Row and head strides of ``[T, H, D]``; those of a single row or head, which torch leaves
   arbitrary, as if packed."""
   T, H, D = t.shape
-  sh = t.stride(1) if H > 1 else D
-  return (t.stride(0) if T > 1 else max(H * sh, H * D)), sh
+  st, sh, _ = t.stride()
+  if H <= 1:
+    sh = D
+  return (st if T > 1 else max(H * sh, H * D)), sh
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int, int]:
@@ -641,7 +642,7 @@ def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _offsets32(t: torch.Tensor, name: str, n: int | None, what: str) -> torch.Tensor:
-  if t.dtype != torch.int32 or t.ndim != 1 or (n is not None and t.numel() != n):
+  if t.dtype is not torch.int32 or t.ndim != 1 or (n is not None and t.shape[0] != n):
     raise ValueError(f"{what}: {name} must be int32 [{'sequences + 1' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
   return t if t.is_contiguous() else t.contiguous()
 
@@ -670,20 +671,21 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   what = "packed_attention"
   _no_grad(what, q, k, v)
   dev = _require_cuda(q, k, v, cu_q, cu_k, len_q, len_k, out)
-  _require(q.ndim == 3 and k.ndim == 3 and v.ndim == 3, "packed_attention: q, k and v must be [tokens, heads, dim]")
-  Tq, H, D = q.shape
-  Tk, Hkv = k.shape[0], k.shape[1]
-  if k.shape[2] != D or v.shape != k.shape:
-    raise ValueError(f"packed_attention: shapes q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+  qs, ks = q.shape, k.shape
+  _require(len(qs) == 3 and len(ks) == 3 and v.ndim == 3, "packed_attention: q, k and v must be [tokens, heads, dim]")
+  Tq, H, D = qs
+  Tk, Hkv, Dk = ks
+  if Dk != D or v.shape != ks:
+    raise ValueError(f"packed_attention: shapes q{tuple(qs)} k{tuple(ks)} v{tuple(v.shape)}")
   if H == 0 or Hkv == 0 or H % Hkv != 0:
     raise ValueError(f"packed_attention: {H} query heads do not share {Hkv} key heads evenly")
   if D % 8 != 0 or not 0 < D <= 128:
     raise ValueError(f"packed_attention: head dim {D} is not a multiple of 8 up to 128")
   dtype = q.dtype
-  if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
+  if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
     raise ValueError(f"packed_attention: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
   cu_q = _offsets32(cu_q, "cu_q", None, what)
-  B = cu_q.numel() - 1
+  B = cu_q.shape[0] - 1
   _require(B >= 1, "packed_attention: cu_q needs at least two offsets")
   if cu_k is None:
     cu_k, len_k = cu_q, (len_q if len_k is None else len_k)
@@ -694,33 +696,35 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   if len_k is not None:
     len_k = _offsets32(len_k, "len_k", B, what)
   scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-  _require(abs(scale) <= 1e30, f"packed_attention: scale {scale} is not finite or above 1e30")
+  if not abs(scale) <= 1e30:
+    raise ValueError(f"packed_attention: scale {scale} is not finite or above 1e30")
 
-  def rows(t, keys):
-    st, sh = _strides2(t)
-    if t.stride(2) != 1 or st % 8 or sh % 8 or t.data_ptr() % 16 or (keys and not D <= st < 1 << 24):
+  def rows(t, least):
+    st, sh, sd = t.stride()
+    if t.shape[1] == 1:                                        # (a single head's or row's stride means nothing)
+      sh = D
+    if t.shape[0] <= 1:
+      st = t.shape[1] * max(sh, D)
+    ptr = t.data_ptr()
+    if sd != 1 or (st | sh | ptr >> 1) % 8 or not least <= st < 1 << 24:
       t = torch.empty(t.shape, dtype=dtype, device=dev).copy_(t)
-      st, sh = t.shape[1] * D, D
-    return t, (st, sh)
+      st, sh, ptr = t.shape[1] * D, D, t.data_ptr()
+    return t, ptr, (st, sh)
 
   if out is None:
-    out = torch.empty((Tq, H, D), dtype=dtype, device=dev)
+    out = torch.empty(qs, dtype=dtype, device=dev)
     so = (H * D, D)
   else:
     so = _strides2(out) if out.ndim == 3 else (0, 0)
-    if tuple(out.shape) != (Tq, H, D) or out.dtype != dtype or out.stride(2) != 1 or so[0] % 8 or so[1] % 8 or out.data_ptr() % 16:
+    if out.shape != qs or out.dtype != dtype or out.stride(2) != 1 or so[0] % 8 or so[1] % 8 or out.data_ptr() % 16:
       raise ValueError(f"packed_attention: out must be {dtype} {(Tq, H, D)} in 16-byte aligned rows")
     if not (_disjoint(out, q) and _disjoint(out, k) and _disjoint(out, v)):
       raise ValueError("packed_attention: out overlaps an input")
-  a = _lib.PackedAttentionArgs()
-  a.B, a.H, a.Hkv, a.D, a.Tq, a.Tk = B, H, Hkv, D, Tq, Tk
-  a.scale, a.causal, a.dtype = scale, int(bool(causal)), _ELEMENT_TYPES[dtype]
-  q, (a.q_s[0], a.q_s[1]) = rows(q, False)
-  k, (a.k_s[0], a.k_s[1]) = rows(k, True)
-  v, (a.v_s[0], a.v_s[1]) = rows(v, True)
-  a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-  a.o_s[0], a.o_s[1] = so
-  a.cu_q, a.cu_k, a.len_q, a.len_k = cu_q.data_ptr(), cu_k.data_ptr(), _vp(len_q), _vp(len_k)
+  q, qp, sq = rows(q, 0)
+  k, kp, sk = rows(k, D)
+  v, vp, sv = rows(v, D)
+  a = _lib.PackedAttentionArgs(B, H, Hkv, D, Tq, Tk, scale, int(bool(causal)), _ELEMENT_TYPES[dtype], qp, sq, kp, sk, vp, sv,
+                               out.data_ptr(), so, cu_q.data_ptr(), cu_k.data_ptr(), _vp(len_q), _vp(len_k))
   lib = _lib.load()
   ref = C.byref(a)
   need = lib.sf_hip_packed_attention_workspace_bytes(ref)
@@ -763,75 +767,81 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
 def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, norm=0, eps=0.0, weights=(None,) * 4):
   _no_grad(what, q, k, freqs, *weights)
   dev = _require_cuda(q, k, positions, freqs, out_q, out_k, *weights)
-  if q.ndim < 3 or (k is not None and (k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
-    raise ValueError(f"{what}: q must be [..., H, D] and k [..., Hk, D], got {tuple(q.shape)}"
-                     f"{'' if k is None else ' and ' + str(tuple(k.shape))}")
-  lead, H, D = q.shape[:-2], q.shape[-2], q.shape[-1]
+  qs, ks = q.shape, None if k is None else k.shape
+  nd = len(qs)
+  if nd < 3 or (ks is not None and (len(ks) != nd or ks[-1] != qs[-1] or (ks[0] != qs[0] if nd == 3 else ks[:-2] != qs[:-2]))):
+    raise ValueError(f"{what}: q must be [..., H, D] and k [..., Hk, D], got {tuple(qs)}{'' if ks is None else ' and ' + str(tuple(ks))}")
+  H, D = qs[-2], qs[-1]
   dtype = q.dtype
   if dtype not in _ELEMENT_TYPES or (k is not None and k.dtype != dtype):
     raise ValueError(f"{what}: q and k must be bfloat16, float16 or float32 alike, got {dtype}{'' if k is None else f' and {k.dtype}'}")
-  if H == 0 or (k is not None and k.shape[-2] == 0) or not 0 < D <= 256:
+  if H == 0 or (ks is not None and ks[-2] == 0) or not 0 < D <= 256:
     raise ValueError(f"{what}: heads must be there and head dims lie in 1 .. 256, got {tuple(q.shape)}")
-  if freqs.dtype != torch.float64 or freqs.ndim != 1 or not 1 <= freqs.numel() <= D // 2:
+  pairs = freqs.numel()
+  if freqs.dtype != torch.float64 or freqs.ndim != 1 or not 1 <= pairs <= D // 2:
     raise ValueError(f"{what}: freqs must be float64 [R / 2], 1 to {D // 2} of them, got {freqs.dtype} {tuple(freqs.shape)}")
-  if positions.dtype not in (torch.int32, torch.int64):
-    raise ValueError(f"{what}: positions must be int32 or int64, got {positions.dtype}")
-  if positions.shape != lead:
+  pdtype = positions.dtype
+  if pdtype is not torch.int32 and pdtype is not torch.int64:
+    raise ValueError(f"{what}: positions must be int32 or int64, got {pdtype}")
+  flat = nd == 3
+  if positions.ndim != 1 or not flat or positions.shape[0] != qs[0]:
     try:
-      positions = positions.expand(lead)
+      positions = positions.expand(qs[:-2])
     except RuntimeError:
-      raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit tokens {tuple(lead)}") from None
+      raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit tokens {tuple(qs[:-2])}") from None
+    positions = positions.reshape(-1)
   if not math.isfinite(magnitude):
     raise ValueError(f"{what}: magnitude {magnitude} is not finite")
 
   def three(t):
-    t3 = t if t.ndim == 3 else t.reshape(-1, t.shape[-2], D)
-    return t3 if t3.stride(2) == 1 or D == 1 else t3.contiguous()
+    t3 = t if flat else t.reshape(-1, t.shape[-2], D)
+    return t3 if D == 1 or t3.stride(2) == 1 else t3.contiguous()
 
-  def result(given, like, name):
-    if given is None:
-      o = torch.empty(like.shape, dtype=dtype, device=dev)
-      return o, three(o)
-    if given.shape != like.shape or given.dtype != dtype or (given.stride(-1) != 1 and D > 1):
+  def given(o, like, name):
+    if o.shape != like.shape or o.dtype != dtype or (D > 1 and o.stride(-1) != 1):
       raise ValueError(f"{what}: {name} must be {dtype} {tuple(like.shape)} with a unit last stride")
     try:
-      return given, given if given.ndim == 3 else given.view(-1, given.shape[-2], D)
+      return o if flat else o.view(-1, o.shape[-2], D)
     except RuntimeError:
       raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
 
-  q3 = three(q)
-  k3 = None if k is None else three(k)
-  oq, oq3 = result(out_q, q, "out_q")
-  ok = ok3 = None
-  if k is not None:
-    ok, ok3 = result(out_k, k, "out_k")
-  elif out_k is not None:
+  if k is None and out_k is not None:
     raise ValueError(f"{what}: out_k without k")
-  if out_q is not None or out_k is not None:
-    same = lambda a, b: a.data_ptr() == b.data_ptr() and _strides2(a) == _strides2(b) and a.shape == b.shape
-    pairs = [(oq3, q3, True)]
-    if k is not None:
-      pairs += [(ok3, k3, True), (oq3, k3, False), (ok3, q3, False), (oq3, ok3, False)]
-    for a, b, own in pairs:
+  in_place = out_q is not None or out_k is not None
+  q3 = three(q)
+  sq = _strides2(q3)
+  T = q3.shape[0]
+  if out_q is None:
+    out_q = torch.empty(qs, dtype=dtype, device=dev)
+    oq3, so = out_q, (H * D, D)
+  else:
+    oq3 = given(out_q, q, "out_q")
+    so = _strides2(oq3)
+  Hk, k3, ok3, kp, sk, okp, sok = 0, None, None, None, (0, 0), None, (0, 0)
+  if k is not None:
+    Hk, k3 = ks[-2], three(k)
+    kp, sk = k3.data_ptr(), _strides2(k3)
+    if out_k is None:
+      out_k = torch.empty(ks, dtype=dtype, device=dev)
+      ok3, sok = out_k, (Hk * D, D)
+    else:
+      ok3 = given(out_k, k, "out_k")
+      sok = _strides2(ok3)
+    okp = ok3.data_ptr()
+  if in_place:
+    same = lambda a, b: a.data_ptr() == b.data_ptr() and a.shape == b.shape and _strides2(a) == _strides2(b)
+    oq, ok = oq3.view(-1, H, D) if oq3.ndim != 3 else oq3, ok3.view(-1, Hk, D) if ok3 is not None and ok3.ndim != 3 else ok3
+    meets = [(oq, q3, True)] if k is None else [(oq, q3, True), (ok, k3, True), (oq, k3, False), (ok, q3, False), (oq, ok, False)]
+    for a, b, own in meets:
       if not (_disjoint(a, b) or (own and same(a, b))):
         raise ValueError(f"{what}: outputs may be their own input in place, and overlap nothing else")
-  a = _lib.RotaryArgs()
-  a.T, a.H, a.Hk, a.D, a.R = q3.shape[0], H, 0 if k is None else k.shape[-2], D, 2 * freqs.numel()
-  a.interleaved, a.dtype, a.norm = int(bool(interleaved)), _ELEMENT_TYPES[dtype], norm
-  a.eps, a.magnitude = eps, magnitude
-  positions = positions if positions.ndim == 1 and positions.is_contiguous() else positions.reshape(-1).contiguous()
-  freqs = freqs.contiguous()
-  a.q, a.q_out = q3.data_ptr(), oq3.data_ptr()
-  a.q_s[0], a.q_s[1] = _strides2(q3)
-  a.qo_s[0], a.qo_s[1] = _strides2(oq3)
-  if k is not None:
-    a.k, a.k_out = k3.data_ptr(), ok3.data_ptr()
-    a.k_s[0], a.k_s[1] = _strides2(k3)
-    a.ko_s[0], a.ko_s[1] = _strides2(ok3)
-  a.positions, a.positions_64, a.freqs = positions.data_ptr(), int(positions.dtype == torch.int64), freqs.data_ptr()
-  a.q_weight, a.k_weight, a.q_bias, a.k_bias = (_vp(w) for w in weights)
+  positions, freqs = positions.contiguous(), freqs.contiguous()
+  qw, kw, qb, kb = weights
+  a = _lib.RotaryArgs(T, H, Hk, D, 2 * pairs, int(bool(interleaved)), _ELEMENT_TYPES[dtype], norm, eps, magnitude, q3.data_ptr(), sq,
+                      kp, sk, oq3.data_ptr(), so, okp, sok, positions.data_ptr(), int(pdtype is torch.int64), freqs.data_ptr(),
+                      _vp(qw), _vp(qb), _vp(kw), _vp(kb))
   _launch(_lib.load().sf_hip_rotary_fwd, q3, "sf_hip_rotary_fwd", C.byref(a))
-  return oq, ok
+  return out_q, out_k
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor, *,
@@ -867,9 +877,14 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
   if not 0.0 <= eps < math.inf:
     raise ValueError(f"{what}: eps {eps} is not finite and >= 0")
   weights = (q_weight, k_weight, q_bias, k_bias)
+  ready = []
   for w in weights:
-    if w is not None and tuple(w.shape) != (q.shape[-1],):
-      raise ValueError(f"{what}: weights and biases must be [{q.shape[-1]}], got {tuple(w.shape)}")
-  _no_grad(what, *weights)
-  return _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, _NORMS[norm], float(eps),
-                 tuple(_f32(w) for w in weights))
+    if w is not None:
+      if w.ndim != 1 or w.shape[0] != q.shape[-1]:
+        raise ValueError(f"{what}: weights and biases must be [{q.shape[-1]}], got {tuple(w.shape)}")
+      if w.requires_grad:
+        _no_grad(what, w)
+      if w.dtype is not torch.float32 or not w.is_contiguous():
+        w = _f32(w)
+    ready.append(w)
+  return _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, _NORMS[norm], float(eps), ready)

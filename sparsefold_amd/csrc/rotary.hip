@@ -41,8 +41,8 @@ struct RotF32 {
 template <class E, int V>
 struct Piece {
   typedef typename E::raw vec __attribute__((ext_vector_type(V)));
-  static __device__ __forceinline__ void load(const typename E::raw* p, float* f) {
-    const vec v = *reinterpret_cast<const vec*>(p);
+  static __device__ __forceinline__ vec load(const typename E::raw* p) { return *reinterpret_cast<const vec*>(p); }
+  static __device__ __forceinline__ void widen(const vec& v, float* f) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = E::to_float(v[e]);
   }
@@ -55,7 +55,9 @@ struct Piece {
 };
 template <class E>
 struct Piece<E, 1> {
-  static __device__ __forceinline__ void load(const typename E::raw* p, float* f) { f[0] = E::to_float(*p); }
+  typedef typename E::raw vec;
+  static __device__ __forceinline__ vec load(const typename E::raw* p) { return *p; }
+  static __device__ __forceinline__ void widen(const vec& v, float* f) { f[0] = E::to_float(v); }
   static __device__ __forceinline__ void store(typename E::raw* p, const float* f) { *p = E::from_float(f[0]); }
 };
 
@@ -85,10 +87,22 @@ template <class E, int V, int UPL, int NORM, bool INTERLEAVED>
 __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_args a, const RotaryPlan pl) {
   typedef typename E::raw raw;
   __shared__ f32x2 table[kWaves][kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float affine[NORM == 2 ? 4 : NORM == 1 ? 2 : 1][2 * kMaxPairs];   // weights of q, k, biases of q, k
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
   const int64_t token = task / pl.chunks;
-  if (token >= a.T) return;                                  // (waves meet no barrier)
+  if (NORM != 0) {                                           // read from memory once for all waves
+    for (int d = threadIdx.x; d < a.D; d += 64 * kWaves) {
+      affine[0][d] = a.q_weight != nullptr ? a.q_weight[d] : 1.f;
+      affine[1][d] = a.k_weight != nullptr ? a.k_weight[d] : 1.f;
+      if (NORM == 2) {
+        affine[2][d] = a.q_bias != nullptr ? a.q_bias[d] : 0.f;
+        affine[3][d] = a.k_bias != nullptr ? a.k_bias[d] : 0.f;
+      }
+    }
+    __syncthreads();
+  }
+  if (token >= a.T) return;                                  // (no barrier from here on)
   const int first = (int)(task - token * pl.chunks) * pl.per_wave, end = min(first + pl.per_wave, a.H + a.Hk);
   const int half_r = a.R >> 1;
 
@@ -103,6 +117,7 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
   }
   asm volatile("" ::: "memory");                             // a wave's LDS accesses are in order
 
+  constexpr bool kInPiece = INTERLEAVED && V > 1;            // a pair's two dims lie in one piece
   // ---- this lane's units: V pairs each, or 2 V dims behind the rotated ones ----
   const int sub = lane & (pl.lph - 1), group = lane / pl.lph, step = 64 / pl.lph;
   const int rotating = half_r / V, units = rotating + (a.D - a.R + 2 * V - 1) / (2 * V);
@@ -115,13 +130,17 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
 #pragma unroll
     for (int e = 0; e < V; ++e) cs[x][e] = f32x2{1.f, 0.f};
     if (u < rotating) {
-      at[x][0] = INTERLEAVED ? 2 * V * u : V * u;
-      at[x][1] = INTERLEAVED ? 2 * V * u + V : half_r + V * u;
+      // the pieces of neighbouring lanes are neighbours: whole lines an instruction, in either layout
+      at[x][0] = kInPiece ? V * u : INTERLEAVED ? 2 * u : V * u;
+      at[x][1] = kInPiece ? half_r + V * u : INTERLEAVED ? 2 * u + 1 : half_r + V * u;
 #pragma unroll
-      for (int e = 0; e < V; ++e) cs[x][e] = table[wave][V * u + e];
+      for (int e = 0; e < V; ++e) {
+        const int pair = !kInPiece ? V * u + e : e < V / 2 ? at[x][0] / 2 + e : at[x][1] / 2 + e - V / 2;
+        cs[x][e] = table[wave][pair];
+      }
     } else if (u < units) {
-      at[x][0] = a.R + 2 * V * (u - rotating);
-      if (at[x][0] + V < a.D) at[x][1] = at[x][0] + V;
+      at[x][0] = a.R + V * (u - rotating);
+      if (at[x][0] + V * (units - rotating) < a.D) at[x][1] = at[x][0] + V * (units - rotating);
     }
   }
 
@@ -135,8 +154,6 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
     const int64_t src_h = which ? a.k_s[1] : a.q_s[1], dst_h = which ? a.ko_s[1] : a.qo_s[1];
     float w[UPL][2][V], b[UPL][2][V];
     if (NORM != 0) {
-      const float* wp = which ? a.k_weight : a.q_weight;
-      const float* bp = which ? a.k_bias : a.q_bias;
 #pragma unroll
       for (int x = 0; x < UPL; ++x)
 #pragma unroll
@@ -144,27 +161,38 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const int d = max(at[x][p], 0) + e;
-            w[x][p][e] = wp != nullptr ? wp[d] : 1.f;
-            b[x][p][e] = NORM == 2 && bp != nullptr ? bp[d] : 0.f;
+            w[x][p][e] = affine[which][d];
+            b[x][p][e] = NORM == 2 ? affine[NORM == 2 ? 2 + which : 0][d] : 0.f;
           }
     }
+    // the next heads' loads are on their way while these are worked on
+    typename Piece<E, V>::vec next[UPL][2];
+    auto fetch = [&](int h) __attribute__((always_inline)) {
+      const raw* sp = src + (int64_t)min(h, h1 - 1) * src_h;
+#pragma unroll
+      for (int x = 0; x < UPL; ++x)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+          if (at[x][p] >= 0) next[x][p] = Piece<E, V>::load(sp + at[x][p]);
+    };
+    fetch(h0 + group);
 #pragma unroll 1
     for (int hb = h0; hb < h1; hb += step) {
       const int h = hb + group;
       const bool ok = h < h1;
-      const raw* sp = src + (int64_t)min(h, h1 - 1) * src_h;
       float f[UPL][2][V];
 #pragma unroll
       for (int x = 0; x < UPL; ++x)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           if (at[x][p] >= 0) {
-            Piece<E, V>::load(sp + at[x][p], f[x][p]);
+            Piece<E, V>::widen(next[x][p], f[x][p]);
           } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) f[x][p][e] = 0.f;
           }
         }
+      if (hb + step < h1) fetch(h + step);
       if (NORM != 0) {
         auto head_sum = [&](float v) __attribute__((always_inline)) {
           for (int o = 1; o < pl.lph; o <<= 1) v += __shfl_xor(v, o);
