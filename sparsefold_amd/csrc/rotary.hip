@@ -291,8 +291,10 @@ extern "C" int sf_hip_rotary_fwd(const sf_rotary_args* a, void* stream) {
   const int heads = a->H + a->Hk, at_once = 64 / pl.lph;
   pl.per_wave = heads;
   pl.chunks = (heads + pl.per_wave - 1) / pl.per_wave;
-  // few tokens: their heads spread over waves until the GPU is filled
-  while (pl.per_wave > at_once && a->T * pl.chunks < 4096) {
+  // few tokens: their heads spread over waves until the GPU is filled; without a norm, whose waves have
+  // more to set up, also where it gets another round (8192 tokens, 32 + 8 heads of 128 in fp16, 1 / 5 waves a
+  // token: 36.4 / 33.3 us; with a norm, bf16, 16384 tokens, 1 / 2: 71 / 78)
+  while (pl.per_wave > at_once && a->T * pl.chunks < (a->norm == SF_NORM_NONE ? 32768 : 4096)) {
     pl.per_wave = (pl.per_wave / 2 + at_once - 1) / at_once * at_once;
     pl.chunks = (heads + pl.per_wave - 1) / pl.per_wave;
   }
