@@ -185,9 +185,39 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, in
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
+// A weight of zero does not keep a NaN or an infinity out of a sum, so a tile that some of its rows see in
+// part can leave in a row's result what only keys hidden from it hold.  Such rows are done again by
+// exact_row.  That is slow, so a result that is not finite for a reason of its own is told apart
+// first: every hidden value near is finite, or the row's last key has a NaN in the very dims.
+
+// Whether keys first .. end - 1 of the key head hold a value that is not finite; by a wave, uniform.
+template <class E>
+__device__ __forceinline__ bool hidden_not_finite(const sf_packed_attention_args& a, const Seq& s, int hk, int first, int end) {
+  const int lane = threadIdx.x & 63;
+  float f = 0.f;
+  for (int j = max(first, 0); j < end; ++j) {
+    const uint16_t* v = (const uint16_t*)a.v + (int64_t)(s.k0 + j) * a.v_s[0] + (int64_t)hk * a.v_s[1];
+    if (lane < a.D) f = __builtin_fmaf(E::to_float(v[lane]), 0.f, f);
+    if (lane + 64 < a.D) f = __builtin_fmaf(E::to_float(v[lane + 64]), 0.f, f);
+  }
+  return __any(!(f == 0.f));
+}
+
+// Of a row's dims d .. d + 3: whether one is not finite that is no NaN in the row's last key (-1: it has none).
+template <class E>
+__device__ __forceinline__ bool unexplained(const sf_packed_attention_args& a, const Seq& s, int hk, int last, int d, const float (&o)[4]) {
+  bool doubt = false;
+  for (int e = 0; e < 4; ++e) {
+    if (__builtin_fmaf(o[e], 0.f, 0.f) == 0.f || d + e >= a.D) continue;
+    const uint16_t* v = (const uint16_t*)a.v + (int64_t)(s.k0 + max(last, 0)) * a.v_s[0] + (int64_t)hk * a.v_s[1];
+    const float x = last < 0 ? 0.f : E::to_float(v[d + e]);
+    doubt |= x == x;
+  }
+  return doubt;
+}
+
 // One row exactly, by a wave, straight from its definition: keys 0 .. last in chunks of 64, a lane
-// each for the products, lanes over the dims for the sums.  For rows whose fast result is not
-// finite: there a NaN or infinite value of a key that the row does not see meets a weight of zero.
+// each for the products, lanes over the dims for the sums.
 template <class E>
 __device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
   const int lane = threadIdx.x & 63, D = a.D, last = last_key(s, a.causal, r, pl);
@@ -527,7 +557,19 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
   }
   const float inv = mine < 0 ? 0.f : 1.f / l;
   // rows to be done again (see exact_row): either half's accumulators are not finite
-  const uint64_t badl = __ballot(a.causal && !(st.finite_probe() == 0.f) && r0 + li < rows);
+  uint64_t badl = __ballot(a.causal && !(st.finite_probe() == 0.f) && r0 + li < rows);
+  if (badl != 0) {
+    bool doubt = false;
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const float o[4] = {st.o[db][4 * c4], st.o[db][4 * c4 + 1], st.o[db][4 * c4 + 2], st.o[db][4 * c4 + 3]};
+        doubt |= unexplained<E>(a, s, hk, mine, 32 * db + 8 * c4 + 4 * half, o);
+      }
+    badl &= __ballot(doubt);
+    if (badl != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (high | 63) + 1))) badl = 0;
+  }
   uint32_t bad = (uint32_t)badl | (uint32_t)(badl >> 32);
   uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, row, a.o_s);
   const bool write = r0 + li < rows && !(bad >> li & 1);
@@ -666,7 +708,15 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
     return;
   }
   const int r = r0 + jr;
-  const uint64_t bad8 = __ballot(a.causal && !(probe == 0.f) && r < rows);   // a byte for each of the wave's 8 rows
+  uint64_t bad8 = __ballot(a.causal && !(probe == 0.f) && r < rows);         // a byte for each of the wave's 8 rows
+  if (bad8 != 0) {
+    bool doubt = false;
+#pragma unroll
+    for (int db = 0; db < T::DB; ++db)
+      doubt |= unexplained<E>(a, s, hk, last_key(s, a.causal, min(r, rows - 1), pl), 32 * db + jd, {o[db][0], o[db][1], o[db][2], o[db][3]});
+    bad8 &= __ballot(doubt);
+    if (bad8 != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (seen - 1 | 63) + 1))) bad8 = 0;
+  }
   if (r < rows && !(bad8 >> (lane & 56) & 0xff)) {
     const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / l;
     uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s);
@@ -766,7 +816,12 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
       float probe = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[x][e], 0.f, probe);
-      const uint64_t bad = __ballot(a.causal && mine && !(probe == 0.f));
+      uint64_t bad = __ballot(a.causal && mine && !(probe == 0.f));
+      if (bad != 0) {
+        const int r32 = r0 + (in0 & ~31), low = last_key(s, a.causal, r32, pl), high = last_key(s, a.causal, min(r32 + 31, rows - 1), pl);
+        bad &= __ballot(unexplained<E>(a, s, hk, last_key(s, a.causal, min(r, rows - 1), pl), d, {o[x][0], o[x][1], o[x][2], o[x][3]}));
+        if (bad != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (high | 63) + 1))) bad = 0;
+      }
       const uint64_t lanes = ((1ull << LR) - 1) << (lane / LR * LR);
       if (mine && !(bad & lanes)) {
         const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / sum[x];

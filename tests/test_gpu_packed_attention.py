@@ -188,6 +188,28 @@ def test_later_keys_have_no_influence(n, D, bad):
   check(out[:p], q[:p], k[:p], v[:p], [p], [p], True)
 
 
+@pytest.mark.parametrize("n,D", [(20, 64), (200, 64), (2000, 128)])
+def test_values_that_are_not_finite_everywhere(n, D):
+  """NaN or infinite in one dim of all values: that dim alone, with the value it has."""
+  q, k, v = make([n], [n], 4, 2, D, torch.bfloat16, n)
+  clean = ops.packed_attention(q, k, v, offsets([n]), causal=True)
+  for bad in (math.nan, math.inf, -math.inf):
+    dirty = v.clone()
+    dirty[..., 5] = bad
+    out = ops.packed_attention(q, k, dirty, offsets([n]), causal=True)
+    assert torch.equal(out[..., 5].float().cpu(), torch.full((n, 4), bad)) or (bad != bad and torch.isnan(out[..., 5].float()).all())
+    rest = [d for d in range(D) if d != 5]
+    # (rows done again are summed in another order)
+    u = 2.0 ** -8
+    assert ((out[..., rest] - clean[..., rest]).float().abs() <= 6 * u * v.float().abs().amax()).all()
+
+
+def test_nothing_but_nan():
+  q, k, v = make([4000], [4000], 8, 8, 64, torch.bfloat16)
+  assert torch.isnan(ops.packed_attention(q, k, torch.full_like(v, math.nan), offsets([4000]), causal=True).float()).all()
+  assert torch.isnan(ops.packed_attention(torch.full_like(q, math.nan), k, v, offsets([4000]), causal=True).float()).all()
+
+
 def test_later_values_have_no_influence_over_key_slices():
   n, m, p = 5, 4000, 3998
   q, k, v = make([n], [m], 2, 1, 128, torch.bfloat16)
