@@ -127,8 +127,6 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
   for (int x = 0; x < UPL; ++x) {
     const int u = sub + 64 * x;
     at[x][0] = at[x][1] = -1;
-#pragma unroll
-    for (int e = 0; e < V; ++e) cs[x][e] = f32x2{1.f, 0.f};
     if (u < rotating) {
       // the pieces of neighbouring lanes are neighbours: whole lines an instruction, in either layout
       at[x][0] = kInPiece ? V * u : INTERLEAVED ? 2 * u : V * u;
@@ -230,13 +228,15 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
 #pragma unroll
       for (int x = 0; x < UPL; ++x) {
         float* z = &f[x][0][0];                              // 2 V values: the pieces one after the other
+        if (sub + 64 * x < rotating) {                       // (others stay: a turn by 0 would mix an infinity in)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float& za = INTERLEAVED ? z[2 * e] : z[e];
-          float& zb = INTERLEAVED ? z[2 * e + 1] : z[V + e];
-          const float va = za, vb = zb;
-          za = va * cs[x][e][0] - vb * cs[x][e][1];
-          zb = vb * cs[x][e][0] + va * cs[x][e][1];
+          for (int e = 0; e < V; ++e) {
+            float& za = INTERLEAVED ? z[2 * e] : z[e];
+            float& zb = INTERLEAVED ? z[2 * e + 1] : z[V + e];
+            const float va = za, vb = zb;
+            za = va * cs[x][e][0] - vb * cs[x][e][1];
+            zb = vb * cs[x][e][0] + va * cs[x][e][1];
+          }
         }
         raw* dp = dst + (int64_t)h * dst_h;
 #pragma unroll
@@ -263,8 +263,8 @@ void launch(const sf_rotary_args* a, const RotaryPlan& pl, dim3 grid, hipStream_
 
 extern "C" int sf_hip_rotary_fwd(const sf_rotary_args* a, void* stream) {
   if (a == nullptr) { sf_set_error("rotary: null args"); return 1; }
-  if (a->T < 0 || a->H <= 0 || a->Hk < 0 || a->D <= 0 || a->D > 256) {
-    sf_set_error("rotary: sizes T=%lld H=%d Hk=%d D=%d (heads positive, D <= 256)", (long long)a->T, a->H, a->Hk, a->D); return 1;
+  if (a->T < 0 || a->H <= 0 || a->Hk < 0 || a->H > 1 << 24 || a->Hk > 1 << 24 || a->D <= 0 || a->D > 256) {
+    sf_set_error("rotary: sizes T=%lld H=%d Hk=%d D=%d (heads positive, up to 2^24; D <= 256)", (long long)a->T, a->H, a->Hk, a->D); return 1;
   }
   if (a->R < 2 || a->R > a->D || a->R % 2 != 0) { sf_set_error("rotary: rotated dims %d are not even and within 2 .. %d", a->R, a->D); return 1; }
   if (a->dtype != SF_DTYPE_BF16 && a->dtype != SF_DTYPE_F16 && a->dtype != SF_DTYPE_F32) { sf_set_error("rotary: element type %d", a->dtype); return 1; }

@@ -173,6 +173,38 @@ def test_values_that_are_not_finite_stay_in_their_head():
     assert bad[1, 1] and bad[2, 0] and bad.sum() == 2
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims", [(128, 64), (96, 48), (64, 24), (40, 2), (255, 30), (130, 4)], ids=lambda d: "x".join(map(str, d)))
+def test_dims_behind_the_rotated_ones_are_copied(dims, interleaved, dtype):
+  """Bit for bit, infinities, NaN and negative zeros among them, and the rotated dims know nothing of them."""
+  D, R = dims
+  q, k = rand(7, 5, D, dtype=TYPES[dtype]), rand(7, 2, D, dtype=TYPES[dtype], seed=1)
+  pos, f = torch.arange(7, device=DEV), ops.rotary_frequencies(R, device=DEV)
+  want = ops.rotary(q, k, pos, f, interleaved=interleaved, magnitude=1.5)
+  for t in (q, k):
+    t[::2, :, R::3], t[1::2, :, R + 1::3], t[:, 1:, D - 1] = math.inf, -0.0, -math.inf
+    t[3, 0, R:] = math.nan
+  got = ops.rotary(q, k, pos, f, interleaved=interleaved, magnitude=1.5)
+  for t, w, g in zip((q, k), want, got):
+    assert torch.equal(g[..., :R], w[..., :R])
+    assert torch.equal(torch.isnan(g[..., R:]), torch.isnan(t[..., R:]))
+    assert torch.equal(g[..., R:].nan_to_num(nan=5.0), t[..., R:].nan_to_num(nan=5.0))
+    assert torch.equal(torch.signbit(g[..., R:])[~torch.isnan(t[..., R:])], torch.signbit(t[..., R:])[~torch.isnan(t[..., R:])])
+
+
+def test_a_graph_that_saved_what_is_overwritten_refuses():
+  w = torch.ones(64, device=DEV, requires_grad=True)
+  q = rand(4, 2, 64)
+  y = (q * w).sum()
+  ops.rotary(q, None, torch.arange(4, device=DEV), ops.rotary_frequencies(64, device=DEV), out_q=q)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    y.backward()
+  with torch.inference_mode():
+    q = rand(4, 2, 64)
+    ops.rotary(q, None, torch.arange(4, device=DEV), ops.rotary_frequencies(64, device=DEV), out_q=q)
+
+
 def test_no_tokens():
   q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=DEV)
   oq, _ = ops.rotary(q, None, torch.empty(0, dtype=torch.int32, device=DEV), ops.rotary_frequencies(64, device=DEV))
