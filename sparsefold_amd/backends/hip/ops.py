@@ -641,6 +641,20 @@ def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
   return sa == sb and ea <= sa and eb <= sa and eb <= (pa - pb) % sa <= sa - ea
 
 
+def _separate(t: torch.Tensor) -> bool:
+  """Whether the rows and heads of a ``[T, H, D]`` view lie apart, row-major or head-major."""
+  st, sh = _strides2(t)
+  T, H, D = t.shape
+  return t.numel() == 0 or (sh >= D and st >= (H - 1) * sh + D) or (st >= D and sh >= (T - 1) * st + D)
+
+
+def _written(*ts) -> None:
+  """Tells autograd that the caller's tensors were written: a graph that saved their old values refuses to use them."""
+  for t in ts:
+    if t is not None and not t.is_inference():
+      torch.autograd.graph.increment_version(t)
+
+
 def _offsets32(t: torch.Tensor, name: str, n: int | None, what: str) -> torch.Tensor:
   if t.dtype is not torch.int32 or t.ndim != 1 or (n is not None and t.shape[0] != n):
     raise ValueError(f"{what}: {name} must be int32 [{'sequences + 1' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
@@ -669,7 +683,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   be captured.  They must not decrease; wrong ones give wrong results but no access outside the
   tensors.  ``out`` may not overlap an input."""
   what = "packed_attention"
-  _no_grad(what, q, k, v)
+  _no_grad(what, q, k, v, out)
   dev = _require_cuda(q, k, v, cu_q, cu_k, len_q, len_k, out)
   qs, ks = q.shape, k.shape
   _require(len(qs) == 3 and len(ks) == 3 and v.ndim == 3, "packed_attention: q, k and v must be [tokens, heads, dim]")
@@ -677,8 +691,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   Tk, Hkv, Dk = ks
   if Dk != D or v.shape != ks:
     raise ValueError(f"packed_attention: shapes q{tuple(qs)} k{tuple(ks)} v{tuple(v.shape)}")
-  if H == 0 or Hkv == 0 or H % Hkv != 0:
-    raise ValueError(f"packed_attention: {H} query heads do not share {Hkv} key heads evenly")
+  if H == 0 or Hkv == 0 or H % Hkv != 0 or H > 1 << 24:
+    raise ValueError(f"packed_attention: {H} query heads do not share {Hkv} key heads evenly, or exceed 2^24")
   if D % 8 != 0 or not 0 < D <= 128:
     raise ValueError(f"packed_attention: head dim {D} is not a multiple of 8 up to 128")
   dtype = q.dtype
@@ -686,7 +700,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     raise ValueError(f"packed_attention: q, k and v must all be bfloat16 or all float16, got {q.dtype}, {k.dtype}, {v.dtype}")
   cu_q = _offsets32(cu_q, "cu_q", None, what)
   B = cu_q.shape[0] - 1
-  _require(B >= 1, "packed_attention: cu_q needs at least two offsets")
+  _require(1 <= B < 1 << 30, "packed_attention: cu_q needs at least two offsets, and below 2^30")
   if cu_k is None:
     cu_k, len_k = cu_q, (len_q if len_k is None else len_k)
   else:
@@ -711,13 +725,15 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
       st, sh, ptr = t.shape[1] * D, D, t.data_ptr()
     return t, ptr, (st, sh)
 
+  given = out
   if out is None:
     out = torch.empty(qs, dtype=dtype, device=dev)
     so = (H * D, D)
   else:
     so = _strides2(out) if out.ndim == 3 else (0, 0)
-    if out.shape != qs or out.dtype != dtype or out.stride(2) != 1 or so[0] % 8 or so[1] % 8 or out.data_ptr() % 16:
-      raise ValueError(f"packed_attention: out must be {dtype} {(Tq, H, D)} in 16-byte aligned rows")
+    if (out.shape != qs or out.dtype != dtype or out.stride(2) != 1 or so[0] % 8 or so[1] % 8 or out.data_ptr() % 16
+        or not _separate(out)):
+      raise ValueError(f"packed_attention: out must be {dtype} {(Tq, H, D)} in 16-byte aligned rows, apart from each other")
     if not (_disjoint(out, q) and _disjoint(out, k) and _disjoint(out, v)):
       raise ValueError("packed_attention: out overlaps an input")
   q, qp, sq = rows(q, 0)
@@ -730,6 +746,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   need = lib.sf_hip_packed_attention_workspace_bytes(ref)
   ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
   _launch(lib.sf_hip_packed_attention_fwd, q, "sf_hip_packed_attention_fwd", ref, _vp(ws), need)
+  _written(given)
   return out
 
 
@@ -765,7 +782,7 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
 
 
 def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, norm=0, eps=0.0, weights=(None,) * 4):
-  _no_grad(what, q, k, freqs, *weights)
+  _no_grad(what, q, k, freqs, out_q, out_k, *weights)
   dev = _require_cuda(q, k, positions, freqs, out_q, out_k, *weights)
   qs, ks = q.shape, None if k is None else k.shape
   nd = len(qs)
@@ -775,8 +792,8 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
   dtype = q.dtype
   if dtype not in _ELEMENT_TYPES or (k is not None and k.dtype != dtype):
     raise ValueError(f"{what}: q and k must be bfloat16, float16 or float32 alike, got {dtype}{'' if k is None else f' and {k.dtype}'}")
-  if H == 0 or (ks is not None and ks[-2] == 0) or not 0 < D <= 256:
-    raise ValueError(f"{what}: heads must be there and head dims lie in 1 .. 256, got {tuple(q.shape)}")
+  if not 0 < H <= 1 << 24 or (ks is not None and not 0 < ks[-2] <= 1 << 24) or not 0 < D <= 256:
+    raise ValueError(f"{what}: heads must lie in 1 .. 2^24 and head dims lie in 1 .. 256, got {tuple(q.shape)}")
   pairs = freqs.numel()
   if freqs.dtype != torch.float64 or freqs.ndim != 1 or not 1 <= pairs <= D // 2:
     raise ValueError(f"{what}: freqs must be float64 [R / 2], 1 to {D // 2} of them, got {freqs.dtype} {tuple(freqs.shape)}")
@@ -801,13 +818,16 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
     if o.shape != like.shape or o.dtype != dtype or (D > 1 and o.stride(-1) != 1):
       raise ValueError(f"{what}: {name} must be {dtype} {tuple(like.shape)} with a unit last stride")
     try:
-      return o if flat else o.view(-1, o.shape[-2], D)
+      o = o if flat else o.view(-1, o.shape[-2], D)
     except RuntimeError:
       raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
+    if not _separate(o):
+      raise ValueError(f"{what}: {name} must hold every element once")
+    return o
 
   if k is None and out_k is not None:
     raise ValueError(f"{what}: out_k without k")
-  in_place = out_q is not None or out_k is not None
+  given_q, given_k = out_q, out_k
   q3 = three(q)
   sq = _strides2(q3)
   T = q3.shape[0]
@@ -828,7 +848,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
       ok3 = given(out_k, k, "out_k")
       sok = _strides2(ok3)
     okp = ok3.data_ptr()
-  if in_place:
+  if given_q is not None or given_k is not None:
     same = lambda a, b: a.data_ptr() == b.data_ptr() and a.shape == b.shape and _strides2(a) == _strides2(b)
     oq, ok = oq3.view(-1, H, D) if oq3.ndim != 3 else oq3, ok3.view(-1, Hk, D) if ok3 is not None and ok3.ndim != 3 else ok3
     meets = [(oq, q3, True)] if k is None else [(oq, q3, True), (ok, k3, True), (oq, k3, False), (ok, q3, False), (oq, ok, False)]
@@ -841,6 +861,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
                       kp, sk, oq3.data_ptr(), so, okp, sok, positions.data_ptr(), int(pdtype is torch.int64), freqs.data_ptr(),
                       _vp(qw), _vp(qb), _vp(kw), _vp(kb))
   _launch(_lib.load().sf_hip_rotary_fwd, q3, "sf_hip_rotary_fwd", C.byref(a))
+  _written(given_q, given_k)
   return out_q, out_k
 
 

@@ -96,6 +96,36 @@ def test_attention_refuses_overlaps_and_gradients():
     ops.packed_attention(leaf, k, v, cu)
 
 
+def test_outputs_that_hold_an_element_twice_are_refused():
+  for out in (torch.zeros(1, 4, 32, dtype=BF).expand(6, 4, 32), torch.zeros(6, 1, 32, dtype=BF).expand(6, 4, 32),
+              torch.zeros(448, dtype=BF).as_strided((6, 4, 32), (64, 32, 1))):
+    with pytest.raises(ValueError, match="apart from each other"):
+      ops.packed_attention(**attention_args(out=out))
+    q = torch.zeros(6, 4, 32, dtype=BF)
+    with pytest.raises(ValueError, match="every element once"):
+      ops.rotary(q, None, torch.arange(6), ops.rotary_frequencies(32), out_q=out)
+    with pytest.raises(ValueError, match="every element once"):
+      ops.rotary(out, None, torch.arange(6), ops.rotary_frequencies(32), out_q=out)
+  with pytest.raises(_Launched):                     # head-major
+    ops.packed_attention(**attention_args(out=torch.zeros(4, 6, 32, dtype=BF).transpose(0, 1)))
+
+
+def test_outputs_that_expect_a_gradient_are_refused():
+  leaf = torch.zeros(6, 4, 32, dtype=BF, requires_grad=True)
+  with pytest.raises(ValueError, match="no backward"):
+    ops.packed_attention(**attention_args(out=leaf))
+  with pytest.raises(ValueError, match="no backward"):
+    ops.rotary(torch.zeros(6, 4, 32, dtype=BF), None, torch.arange(6), ops.rotary_frequencies(32), out_q=leaf)
+
+
+def test_more_heads_than_fit_are_refused():
+  many = torch.zeros(1, 1, 8, dtype=BF).expand(1, (1 << 24) + 1, 8)
+  with pytest.raises(ValueError, match="2\\^24"):
+    ops.packed_attention(many, many, many, torch.tensor([0, 1], dtype=torch.int32))
+  with pytest.raises(ValueError, match="2\\^24"):
+    ops.rotary(many, None, torch.arange(1), ops.rotary_frequencies(8))
+
+
 def rotary_args(**kw):
   a = dict(q=torch.zeros(5, 4, 32, dtype=BF), k=torch.zeros(5, 2, 32, dtype=BF), positions=torch.arange(5), freqs=ops.rotary_frequencies(32))
   a.update(kw)
@@ -258,3 +288,21 @@ def test_bound_of_the_row_tiles(R):
       for G in (1, 3, 8):
         rows = sum(lens) * G
         assert sum(-(-n * G // R) for n in lens) <= tiles_bound(rows, B, R) or rows == 0
+
+
+@pytest.mark.parametrize("B", [1, 2, 63, 64, 65, 257, 4096, 4097, 20000])
+def test_search_of_a_tile(B):
+  """The search over the tiles before each sequence, 64 of them a step: the sequence that holds the tile."""
+  g = torch.Generator().manual_seed(B)
+  for top in (1, 4):
+    tiles = torch.randint(0, top + 1, (B,), generator=g)
+    starts = [0] + tiles.cumsum(0).tolist()
+    for idx in range(0, starts[-1], 1 + starts[-1] // 500):
+      b, n = 0, B
+      while n > 1:
+        step = -(-n // 64)
+        at = [lane * step < n and starts[b + min(lane * step, n - 1)] <= idx for lane in range(64)]
+        assert at == sorted(at, reverse=True)
+        skip = max(sum(at) - 1, 0) * step
+        b, n = b + skip, min(step, n - skip)
+      assert starts[b] <= idx < starts[b + 1]
