@@ -85,7 +85,13 @@ struct PackedPlan {
   double inv_g;      // 1 / G
   float* part;       // slices > 1: per (tile, head, slice) unnormalised O [R][DP], then (m, l) [R][2]
   int4* found;       // slices > 1: per tile, its sequence and its index there, for the join: (q0, lq, lk, tile), (k0, ...)
+  int* starts;       // more than kScanned sequences: the tiles before each, from packed_starts_kernel; else null
 };
+
+// Up to as many sequences every workgroup counts the tiles itself, 64 sequences a step; above, one workgroup
+// counts them for all, a launch of its own (sequences of 20 tokens, 8 heads of 64, counted by each / for all: 130 of
+// them 20.8 / 22.7 us, 256 37.7 / 31.2, 512 90 / 55, 8192 12370 / 797).
+constexpr int kScanned = 192;
 
 // r / G without a division: (r + 0.5) / G is at least 0.5 / G away from a whole number.
 __device__ __forceinline__ int token_of(const PackedPlan& pl, int r) { return (int)(((double)r + 0.5) * pl.inv_g); }
@@ -126,6 +132,23 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, const int32_t* len,
 template <int R>
 __device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, const PackedPlan& pl, int idx, Seq& s, int& tile, int& ntiles) {
   const int lane = threadIdx.x & 63;
+  if (pl.starts != nullptr) {
+    if (idx >= pl.starts[a.B]) return false;
+    // the last sequence that starts at or before idx, among n from b on: 64 of them a step
+    int b = 0, n = a.B;
+    while (n > 1) {
+      const int step = (n + 63) / 64;
+      const bool at = lane * step < n && pl.starts[b + min(lane * step, n - 1)] <= idx;
+      const int skip = max(__popcll(__ballot(at)) - 1, 0) * step;
+      b += skip;
+      n = min(step, n - skip);
+    }
+    seq_range(a.cu_q, a.len_q, b, a.Tq, s.q0, s.lq);
+    seq_range(a.cu_k, a.len_k, b, a.Tk, s.k0, s.lk);
+    ntiles = (int)(((uint32_t)s.lq * (uint32_t)pl.G + R - 1) / R);
+    tile = idx - pl.starts[b];
+    return tile < ntiles;
+  }
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
@@ -155,6 +178,45 @@ __device__ __forceinline__ bool find_tile(const sf_packed_attention_args& a, con
     base += __builtin_amdgcn_readlane(incl, 63);
   }
   return false;
+}
+
+// starts[b]: row tiles of the sequences before b, starts[B] those of all.  One workgroup.
+__global__ __launch_bounds__(1024) void packed_starts_kernel(const sf_packed_attention_args a, const PackedPlan pl, int R) {
+  constexpr int kEach = 4;
+  __shared__ int64_t waves[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t base = 0;                                          // (offsets that overlap may count more than 31 bits hold)
+  for (int64_t b0 = 0; b0 < a.B; b0 += 1024 * kEach) {
+    const int64_t b = b0 + kEach * threadIdx.x;
+    int64_t nt[kEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      int start, n = 0;
+      if (b + e < a.B) seq_range(a.cu_q, a.len_q, (int)(b + e), a.Tq, start, n);
+      nt[e] = ((uint32_t)n * (uint32_t)pl.G + R - 1) / R;
+      sum += nt[e];
+    }
+    int64_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t up = __shfl_up((long long)incl, o);
+      incl += lane >= o ? up : 0;
+    }
+    if (lane == 63) waves[wave] = incl;
+    __syncthreads();
+    int64_t before = base + incl - sum;
+    for (int w = 0; w < 16; ++w) {
+      before += w < wave ? waves[w] : 0;
+      base += waves[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (b + e < a.B) pl.starts[b + e] = (int)min(before, (int64_t)INT32_MAX);
+      before += nt[e];
+    }
+  }
+  if (threadIdx.x == 0) pl.starts[a.B] = (int)min(base, (int64_t)INT32_MAX);
 }
 
 // Leaves what find_tile found to packed_combine_kernel (lq = 0: no tile).
@@ -470,7 +532,7 @@ template <class E, int KC, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
   constexpr int kTile = 64 * T::kRow, R = 32 * NW;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];     // two buffers of K, V
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];       // two buffers of K, V
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
@@ -902,21 +964,22 @@ int route(const sf_packed_attention_args* a, Route& r) {
     slices = 256 / wgs;
     if (slices > seen / least) slices = seen / least;
   }
-  slices = slices < 1 ? 1 : slices > 64 ? 64 : slices;
+  slices = slices < 1 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;
   // rows of a tile join in blocks of 32, or -- packed_stream_kernel -- one by one, as many blocks as a
   // sequence has rows on average
   int64_t pieces = r.nw ? r.nw : (rows + a->B - 1) / a->B;
   if (pieces > 32) pieces = 32;
   float c0 = a->scale * SF_LOG2E;
   if (fabsf(c0) < FLT_MIN) c0 = FLT_MIN;                     // all logits equal; a masked one stays -inf
-  r.pl = PackedPlan{(int)tiles, (int)slices, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr};
+  r.pl = PackedPlan{(int)tiles, (int)slices, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr, nullptr};
   r.wgs = tiles * a->Hkv * slices;
   if (r.wgs > INT32_MAX || tiles * a->Hkv * 32 > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
   return 0;
 }
 
 size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
-  if (r.pl.slices <= 1) return 0;
+  const size_t starts = a->B > kScanned ? ((size_t)a->B + 1) * sizeof(int) : 0;
+  if (r.pl.slices <= 1) return starts;                       // (so many sequences fill the GPU)
   const int R = r.nw ? 32 * r.nw : 32;
   return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float) + (size_t)r.pl.tiles * 2 * sizeof(int4);
 }
@@ -924,6 +987,10 @@ size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
 template <class E, int KC>
 int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
   const dim3 grid((unsigned)r.wgs);
+  if (r.pl.starts != nullptr) {
+    hipLaunchKernelGGL(packed_starts_kernel, dim3(1), dim3(1024), 0, st, *a, r.pl, r.nw ? 32 * r.nw : 32);
+    if (sf_check_launch("packed_starts_kernel")) return 1;
+  }
   if (r.nw == 0) {
     hipLaunchKernelGGL((packed_stream_kernel<E, KC>), grid, dim3(256), 0, st, *a, r.pl);
   } else if (r.nw == 4) {
@@ -970,6 +1037,7 @@ extern "C" int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, vo
     return 1;
   }
   r.pl.part = static_cast<float*>(workspace);
+  if (a->B > kScanned) r.pl.starts = static_cast<int*>(workspace);
   r.pl.found = reinterpret_cast<int4*>(r.pl.part + r.wgs * (r.nw ? 32 * r.nw : 32) * (r.dp + 2));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == SF_DTYPE_BF16 ? launch_type<Bf16>(a, r, st) : launch_type<Fp16>(a, r, st);

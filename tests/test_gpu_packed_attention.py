@@ -361,6 +361,46 @@ def test_other_streams_at_once():
     check(out, q, k, v, [1], [6000], True)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sequences,top", [(192, 30), (193, 30), (300, 400), (4097, 20), (9000, 3)])
+def test_many_sequences(sequences, top, causal):
+  """Beyond 192 sequences a launch of its own counts their tiles; empty ones, a few long ones, lengths in use."""
+  g = torch.Generator().manual_seed(sequences)
+  room = torch.randint(0, top + 1, (sequences,), generator=g)
+  room[::7], room[5], room[-1] = 0, 300, 1
+  used = (torch.rand(sequences, generator=g) * (room + 1)).int().clamp(max=room.int())
+  q, k, v = make(room.tolist(), room.tolist(), 2, 1, 32, torch.bfloat16, top)
+  cu, n = offsets(room.tolist()), used.to(DEV)
+  out = torch.full_like(q, 7.0)
+  assert ops.packed_attention(q, k, v, cu, causal=causal, out=out) is out
+  every = range(sequences) if sequences <= 300 else list(range(0, sequences, 97)) + [5, 6, sequences - 1]
+  starts = [0] + room.cumsum(0).tolist()
+  for b in every:
+    rows = slice(starts[b], starts[b + 1])
+    check(out[rows], q[rows], k[rows], v[rows], [room[b].item()], [room[b].item()], causal)
+  out.fill_(7.0)
+  ops.packed_attention(q, k, v, cu, len_q=n, causal=causal, out=out)
+  free = torch.ones(len(q), dtype=torch.bool)
+  for b in range(sequences):
+    free[starts[b]:starts[b] + used[b]] = False
+  assert (out[free.to(DEV)] == 7.0).all()
+  for b in every:
+    rows = slice(starts[b], starts[b] + used[b])
+    check(out[rows], q[rows], k[rows], v[rows], [used[b].item()], [used[b].item()], causal)
+
+
+def test_many_wrong_offsets():
+  """Overlapping, decreasing and too large ones, more tiles than the launch has: no access outside."""
+  q, k, v = make([64], [64], 2, 2, 32, torch.bfloat16)
+  cu = torch.tensor([0, 1 << 30, -1] * 200 + [10, 64], dtype=torch.int32, device=DEV)
+  room = torch.full((192, 2, 32), 7.0, dtype=torch.bfloat16, device=DEV)
+  ops.packed_attention(q, k, v, cu, torch.full_like(cu, 64).index_fill_(0, torch.zeros(1, dtype=torch.long, device=DEV), 0), out=room[64:128])
+  assert (room[:64] == 7.0).all() and (room[128:] == 7.0).all()
+  # a row belongs to several sequences, only the first of them with keys: its result, or zeros
+  got, (want, tol) = room[64:128].cpu().double(), definition(q, k, v, False, 1 / math.sqrt(32))
+  assert (((got - want).abs() <= tol) | (got == 0)).all()
+
+
 def test_empty_batch():
   q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=DEV)
   assert ops.packed_attention(q, q, q, offsets([0, 0])).shape == (0, 4, 64)
