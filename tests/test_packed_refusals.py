@@ -306,3 +306,44 @@ def test_search_of_a_tile(B):
         skip = max(sum(at) - 1, 0) * step
         b, n = b + skip, min(step, n - skip)
       assert starts[b] <= idx < starts[b + 1]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B", [2, 5, 20, 64])
+def test_order_of_the_row_tiles(B, causal):
+  """The search for the tile with the idx-th most keys: each tile once, keys falling in steps of 64."""
+  g = torch.Generator().manual_seed(B)
+  draw = lambda top: int(torch.randint(0, top, (1,), generator=g))
+  for G, R in ((1, 128), (3, 128), (8, 256), (2, 32)):
+    lk = [(0, 1, draw(900))[draw(3)] for _ in range(B)]
+    lq = [(n, draw(600))[draw(2)] for n in lk]
+    tiles = [-(-n * G // R) for n in lq]
+
+    def longer(b, u):
+      if u < 0:
+        return tiles[b]
+      if not causal:
+        return tiles[b] if lk[b] > 64 * u else 0
+      token = 64 * u - (lk[b] - lq[b])
+      return tiles[b] if token <= 0 else 0 if token >= lq[b] else tiles[b] - token * G // R
+
+    def keys(b, t):
+      return max(0, (min((t + 1) * R, lq[b] * G) - 1) // G + lk[b] - lq[b] + 1) if causal else lk[b]
+
+    order = []
+    for idx in range(sum(tiles)):
+      step, u = 1, -1
+      while any(n > 64 * step for n in lk):
+        step *= 2
+      while step > 0:
+        u += step if sum(longer(b, u + step) for b in range(B)) > idx else 0
+        step //= 2
+      above = [longer(b, u + 1) for b in range(B)]
+      rank, b = idx - sum(above), 0
+      while rank >= longer(b, u) - above[b]:
+        rank -= longer(b, u) - above[b]
+        b += 1
+      order.append((b, tiles[b] - 1 - above[b] - rank))
+    assert sorted(order) == [(b, t) for b in range(B) for t in range(tiles[b])]
+    steps = [-(-keys(b, t) // 64) for b, t in order]
+    assert steps == sorted(steps, reverse=True)
