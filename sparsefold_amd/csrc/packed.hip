@@ -78,13 +78,14 @@ __device__ __forceinline__ float rescale(float m, float mnew, float c0) {
 
 struct PackedPlan {
   int tiles;         // bound on the row tiles of one key head
-  int slices;        // key slices (workgroups per row tile)
+  int slices;        // key slices (workgroups) of every row tile, where there is no share
+  int share;         // packed_stream_kernel: slices of all row tiles of a key head together, dealt out by their keys (0: slices)
   int pieces;        // blocks of packed_combine_kernel per row tile
   float c0;          // scale log2 e
   int G;             // query heads of a key head
   double inv_g;      // 1 / G
-  float* part;       // slices > 1: per (tile, head, slice) unnormalised O [R][DP], then (m, l) [R][2]
-  int4* found;       // slices > 1: per tile, its sequence and its index there, for the join: (q0, lq, lk, tile), (k0, ...)
+  float* part;       // of split tiles, per (slice, key head) unnormalised O [R][DP], then (m, l) [R][2]
+  int4* found;       // per tile, for the join: (q0, lq, lk, tile of the sequence), (k0, its first slice, slices, -); lq = 0: none
   int* starts;       // more than kScanned sequences: the tiles before each, from packed_starts_kernel; else null
 };
 
@@ -127,23 +128,29 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, const int32_t* len,
   n = (int)(e - s);
 }
 
-// Sums over lanes 0 .. own; every lane calls.  Rows of 16 lanes by shifts, then the sums of the rows before.
-__device__ __forceinline__ int row_sums(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);            // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+// Sums of int or float over lanes 0 .. own, and over all; every lane calls.  Rows of 16 lanes by shifts, then the rows.
+template <class V>
+__device__ __forceinline__ V row_sums(V v) {
+  v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
+  v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x112, 0xF, 0xF, false));
+  v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x114, 0xF, 0xF, false));
+  v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x118, 0xF, 0xF, false));
   return v;
+}
+template <class V>
+__device__ __forceinline__ V row_sum(V v, int lane) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 __device__ __forceinline__ int lanes_before_and_own(int v) {
   const int lane = threadIdx.x & 63;
   v = row_sums(v);
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+  const int r0 = row_sum(v, 15), r1 = r0 + row_sum(v, 31), r2 = r1 + row_sum(v, 47);
   return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
-__device__ __forceinline__ int lanes_sum(int v) {
+template <class V>
+__device__ __forceinline__ V lanes_sum(V v) {
   v = row_sums(v);
-  return __builtin_amdgcn_readlane(v, 15) + __builtin_amdgcn_readlane(v, 31) + __builtin_amdgcn_readlane(v, 47) + __builtin_amdgcn_readlane(v, 63);
+  return (row_sum(v, 15) + row_sum(v, 31)) + (row_sum(v, 47) + row_sum(v, 63));
 }
 
 // Tile `idx` of the sequences' row tiles of R rows each, laid end to end: its sequence and its index
@@ -270,12 +277,59 @@ __global__ __launch_bounds__(1024) void packed_starts_kernel(const sf_packed_att
   if (threadIdx.x == 0) pl.starts[a.B] = (int)min(base, (int64_t)INT32_MAX);
 }
 
-// Leaves what find_tile found to packed_combine_kernel (lq = 0: no tile).
-__device__ __forceinline__ void note_tile(const PackedPlan& pl, int idx, bool mine, bool there, const Seq& s, int tile) {
-  if (pl.slices > 1 && mine) {
-    pl.found[2 * idx] = there ? int4{s.q0, s.lq, s.lk, tile} : int4{0, 0, 0, 0};
-    pl.found[2 * idx + 1] = int4{there ? s.k0 : 0, 0, 0, 0};
+// Leaves to packed_combine_kernel what tile `slot` is.
+__device__ __forceinline__ void note_tile(const PackedPlan& pl, int slot, bool there, const Seq& s, int tile, int first, int slices) {
+  pl.found[2 * slot] = there ? int4{s.q0, s.lq, s.lk, tile} : int4{0, 0, 0, 0};
+  pl.found[2 * slot + 1] = there ? int4{s.k0, first, slices, 0} : int4{0, 0, 0, 0};
+}
+
+// Slice `item` of all, where the tiles of up to 64 sequences (a lane each) share pl.share slices by their keys, in
+// slices of c units of `unit` keys: the smallest c that needs no more than the share, one slice a tile aside.  c is at
+// least all units / share, which needs share + tiles at most (the launch's bound), and at most all units / (share - tiles).
+// False past the last; `slot` is the tile's number among all, past the last slice one that no tile has.
+__device__ __forceinline__ bool find_slice(const sf_packed_attention_args& a, const PackedPlan& pl, int unit, int item, Seq& s, int& tile,
+                                           int& slot, int& slice, int& slices) {
+  const int lane = threadIdx.x & 63;
+  int start = 0, n = 0, k0 = 0, lk = 0;
+  if (lane < a.B) {
+    seq_range(a.cu_q, a.len_q, lane, a.Tq, start, n);
+    seq_range(a.cu_k, a.len_k, lane, a.Tk, k0, lk);
   }
+  const int nt = (int)(((uint32_t)n * (uint32_t)pl.G + 31) / 32), units = (lk + unit - 1) / unit;
+  const int tiles = lanes_before_and_own(nt), all = __builtin_amdgcn_readlane(tiles, 63);
+  slot = item;
+  if (all > pl.tiles) return false;                          // (offsets that do not increase)
+  const float total = lanes_sum((float)nt * (float)units);
+  const auto over = [&](int n) __attribute__((always_inline)) {                // ceil(total / n)
+    // (whole numbers up to 2^23 are exact; above, the quotient is kept from falling short)
+    return total < 8388608.f ? max(((uint32_t)total + n - 1) / n, 1u) : (uint32_t)fminf(ceilf(total / (float)n * 1.000001f), 1e9f);
+  };
+  const auto split = [&](uint32_t c) __attribute__((always_inline)) { return (int)max((units + c - 1) / c, 1u); };
+  uint32_t c = over(pl.share);
+  const bool fits = pl.share <= all || lanes_sum(nt * split(c)) <= pl.share;
+  for (uint32_t high = fits ? c : over(pl.share - all); c < high;) {
+    const uint32_t mid = (c + high) / 2;
+    if (lanes_sum(nt * split(mid)) <= pl.share) high = mid;
+    else c = mid + 1;
+  }
+  const int z = split(c);
+  const int items = lanes_before_and_own(nt * z);
+  const uint64_t past = __ballot(items > item);
+  if (past == 0) {
+    slot = all + item - __builtin_amdgcn_readlane(items, 63);
+    return false;
+  }
+  const int src = __builtin_ctzll(past);
+  s.q0 = __builtin_amdgcn_readlane(start, src);
+  s.lq = __builtin_amdgcn_readlane(n, src);
+  s.k0 = __builtin_amdgcn_readlane(k0, src);
+  s.lk = __builtin_amdgcn_readlane(lk, src);
+  slices = __builtin_amdgcn_readlane(z, src);
+  const int r = item - __builtin_amdgcn_readlane(items - nt * z, src);
+  tile = r / slices;
+  slice = r - tile * slices;
+  slot = __builtin_amdgcn_readlane(tiles - nt, src) + tile;
+  return true;
 }
 
 // Last key that row r of the sequence sees (-1: none).
@@ -601,7 +655,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
     there = find_tile<R>(a, pl, idx, s, tile, ntiles);
     tile = ntiles - 1 - tile;
   }
-  note_tile(pl, idx, hk + slice == 0 && tid == 0, there, s, tile);
+  if (pl.slices > 1 && hk + slice + tid == 0) note_tile(pl, idx, there, s, tile, idx * pl.slices, pl.slices);
   if (!there) return;
   const int rows = s.lq * pl.G, r0 = tile * R + wave * 32;
   const int row = min(r0 + li, rows - 1);                    // rows past the end repeat the last
@@ -666,7 +720,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
   if (r0 >= rows) return;                                    // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
   if (pl.slices > 1) {
-    float* po = pl.part + (((int64_t)idx * a.Hkv + hk) * pl.slices + slice) * R * (T::DP + 2);
+    float* po = pl.part + (int64_t)blockIdx.x * R * (T::DP + 2);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
@@ -726,17 +780,27 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   __shared__ f32x2 ml[4][32];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
-  const int slice = rest % pl.slices, idx = rest / pl.slices;
+  const int hk = blockIdx.x % a.Hkv, item = blockIdx.x / a.Hkv;
   Seq s;
-  int tile, ntiles;
-  const bool there = find_tile<32>(a, pl, idx, s, tile, ntiles);
-  note_tile(pl, idx, hk + slice == 0 && tid == 0, there, s, tile);
-  if (!there) return;
+  int tile, slice, slices;
+  if (pl.share > 0) {
+    int slot;
+    const bool there = find_slice(a, pl, 4 * KT, item, s, tile, slot, slice, slices);
+    if (hk + tid == 0 && slot < pl.tiles && (!there || slice == 0)) note_tile(pl, slot, there && slices > 1, s, tile, item, slices);
+    if (!there) return;
+  } else {
+    int ntiles;
+    slices = pl.slices;
+    const int idx = item / slices;
+    slice = item - idx * slices;
+    const bool there = find_tile<32>(a, pl, idx, s, tile, ntiles);
+    if (slices > 1 && hk + slice + tid == 0) note_tile(pl, idx, there, s, tile, item, slices);
+    if (!there) return;
+  }
   const int rows = s.lq * pl.G, r0 = tile * 32;
   const int row = min(r0 + li, rows - 1);
   const int seen = last_key(s, a.causal, min(r0 + 32, rows) - 1, pl) + 1;
-  const int n_all = (seen + KT - 1) / KT, Z = pl.slices * 4;
+  const int n_all = (seen + KT - 1) / KT, Z = slices * 4;
   const int per = (n_all + Z - 1) / Z, t_lo = min((slice * 4 + wave) * per, n_all), t_hi = min(t_lo + per, n_all);
   const int mine = last_key(s, a.causal, row, pl);
   const int low = __builtin_amdgcn_readfirstlane(last_key(s, a.causal, r0, pl));
@@ -819,8 +883,8 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 #pragma unroll
     for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[db][e], 0.f, probe);
   }
-  if (pl.slices > 1) {
-    float* po = pl.part + (((int64_t)idx * a.Hkv + hk) * pl.slices + slice) * 32 * (T::DP + 2);
+  if (slices > 1) {
+    float* po = pl.part + (int64_t)blockIdx.x * 32 * (T::DP + 2);
     if (r0 + jr < rows) {
 #pragma unroll
       for (int db = 0; db < T::DB; ++db) *reinterpret_cast<f32x4*>(po + jr * T::DP + 32 * db + jd) = o[db];
@@ -860,15 +924,16 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
   constexpr int LR = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, GROUPS = 256 / LR;
   constexpr bool kOneRow = R == 32;
   constexpr int ROWS = kOneRow ? 1 : 32, PASSES = kOneRow ? 1 : ROWS / GROUPS;
-  constexpr int64_t kStep = R * (DP + 2);
+  const int64_t kStep = (int64_t)a.Hkv * R * (DP + 2);      // from slice to slice
   __shared__ f32x4 so[kOneRow ? GROUPS : 1][LR];
   __shared__ f32x2 sml[GROUPS];
   const int tid = threadIdx.x, lane = tid & 63, group = tid / LR, d = 4 * (tid % LR);
   const int piece = blockIdx.x % pl.pieces, rest = blockIdx.x / pl.pieces, hk = rest % a.Hkv, idx = rest / a.Hkv;
-  const int4 f0 = pl.found[2 * idx];
-  const Seq s = {f0.x, f0.y, pl.found[2 * idx + 1].x, f0.z};
+  const int4 f0 = pl.found[2 * idx], f1 = pl.found[2 * idx + 1];
+  const Seq s = {f0.x, f0.y, f1.x, f0.z};
+  const int slices = f1.z;
   const int rows = s.lq * pl.G, r0 = f0.w * R;
-  const float* part = pl.part + ((int64_t)idx * a.Hkv + hk) * pl.slices * kStep;
+  const float* part = pl.part + ((int64_t)f1.y * a.Hkv + hk) * R * (DP + 2);
   const float c0 = fabsf(pl.c0);
   for (int in0 = piece * ROWS; in0 < R && r0 + in0 < rows; in0 += pl.pieces * ROWS) {      // (uniform over the block)
     f32x4 o[PASSES];
@@ -882,12 +947,12 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
       float m = -FLT_MAX, l = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       if (r0 + in < rows && d < DP) {
-        for (int z = z0; z < pl.slices; z += 4 * dz) {
+        for (int z = z0; z < slices; z += 4 * dz) {
           f32x2 v[4];
           f32x4 ov[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const bool in_range = z + y * dz < pl.slices;
+            const bool in_range = z + y * dz < slices;
             const int64_t at = (in_range ? z + y * dz : z) * kStep;
             v[y] = *reinterpret_cast<const f32x2*>(ml + at);
             ov[y] = *reinterpret_cast<const f32x4*>(po + at);
@@ -963,6 +1028,7 @@ struct Route {
   int kc, dp;
   PackedPlan pl;
   int64_t wgs;
+  bool joined() const { return pl.slices > 1 || pl.share > 0; }
 };
 
 int route(const sf_packed_attention_args* a, Route& r) {
@@ -1009,7 +1075,7 @@ int route(const sf_packed_attention_args* a, Route& r) {
   // tiles end at sequence ends: sum_b ceil(rows_b / R) <= rows / R + B
   const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
   const int64_t full = (rows + R - 1) / R, wgs = (full > a->B ? full : a->B) * a->Hkv;
-  int64_t slices;
+  int64_t slices, share = 0;
   if (r.nw) {
     // Few workgroups: slices of the keys.  Two workgroups a CU where a slice keeps 1024 keys, else one, and
     // no slice below 512 (prompt of 512 over 8192 keys, 32 / 8 heads of 128, 1 / 2 / 4 slices: 152 / 95 / 85 us;
@@ -1022,23 +1088,27 @@ int route(const sf_packed_attention_args* a, Route& r) {
     const int64_t least = r.dp > 64 ? 128 : 256;
     slices = 256 / wgs;
     if (slices > seen / least) slices = seen / least;
+    // A workgroup a CU, slices dealt out by the keys (one token for 4 caches of 128 to 8192 keys, 32 / 8 heads of 128: 16.8
+    // us, as many slices for each 21.6; 4 caches of 4096: 20.5 / 20.1; 384 workgroups 20.2 / 25.3).  Beyond 64
+    // sequences as many for each.
+    if (slices > 1 && a->B <= 64) share = 256 / a->Hkv;
   }
-  slices = slices < 1 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;
+  slices = slices < 1 || share > 0 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;
   // rows of a tile join in blocks of 32, or -- packed_stream_kernel -- one by one, as many blocks as a
   // sequence has rows on average
   int64_t pieces = r.nw ? r.nw : (rows + a->B - 1) / a->B;
   if (pieces > 32) pieces = 32;
   float c0 = a->scale * SF_LOG2E;
   if (fabsf(c0) < FLT_MIN) c0 = FLT_MIN;                     // all logits equal; a masked one stays -inf
-  r.pl = PackedPlan{(int)tiles, (int)slices, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr, nullptr};
-  r.wgs = tiles * a->Hkv * slices;
+  r.pl = PackedPlan{(int)tiles, (int)slices, (int)share, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr, nullptr};
+  r.wgs = (share > 0 ? share + tiles : tiles * slices) * a->Hkv;
   if (r.wgs > INT32_MAX || tiles * a->Hkv * 32 > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
   return 0;
 }
 
 size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
   const size_t starts = a->B > kScanned ? ((size_t)a->B + 1) * sizeof(int) : 0;
-  if (r.pl.slices <= 1) return starts;                       // (so many sequences fill the GPU)
+  if (!r.joined()) return starts;                       // (so many sequences fill the GPU)
   const int R = r.nw ? 32 * r.nw : 32;
   return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float) + (size_t)r.pl.tiles * 2 * sizeof(int4);
 }
@@ -1058,7 +1128,7 @@ int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
     hipLaunchKernelGGL((packed_tile_kernel<E, KC, 8>), grid, dim3(512), 0, st, *a, r.pl);
   }
   const int rc = sf_check_launch(r.nw ? "packed_tile_kernel" : "packed_stream_kernel");
-  if (rc || r.pl.slices <= 1) return rc;
+  if (rc || !r.joined()) return rc;
   const dim3 gc((unsigned)(r.pl.tiles * a->Hkv * r.pl.pieces));
   constexpr int DP = Dims<KC>::DP;                           // (tiles of 256 rows are never sliced)
   if (r.nw) hipLaunchKernelGGL((packed_combine_kernel<E, DP, 128>), gc, dim3(256), 0, st, *a, r.pl);

@@ -361,6 +361,31 @@ def test_other_streams_at_once():
     check(out, q, k, v, [1], [6000], True)
 
 
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64), ("bf16", 24)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sequences,heads", [(2, (16, 2)), (7, (8, 2)), (30, (8, 1)), (64, (3, 1))])
+def test_slices_by_keys(sequences, heads, causal, dtype, D):
+  """Few rows over caches of very different lengths: long ones are split into many slices, short ones into none."""
+  g = torch.Generator().manual_seed(sequences)
+  lens_k = [(0, 1, 130, 513, 2500, 9000)[i] for i in torch.randint(0, 6, (sequences,), generator=g)]
+  lens_k[-1], lens_k[0] = 5000, 77
+  lens_q = [(0, 1, 1, 2, 5)[i] for i in torch.randint(0, 5, (sequences,), generator=g)]
+  lens_q[0], lens_q[-1] = 9, 1
+  q, k, v = make(lens_q, lens_k, *heads, D, TYPES[dtype], D)
+  if causal:                                         # what only hidden keys hold
+    end = sum(lens_k) - 1
+    v[77 - 1], v[end] = math.nan, 3.0
+  out = ops.packed_attention(q, k, v, offsets(lens_q), offsets(lens_k), causal=causal)
+  if causal:                                         # the last query of the first sequence sees the NaN
+    assert torch.isnan(out[8]).all()
+    out[8], v[77 - 1] = 0.0, 0.0
+    lens = [8] + lens_q[1:]
+    check(torch.cat([out[:8], out[9:]]), torch.cat([q[:8], q[9:]]), k, v, lens, [76] + lens_k[1:], True,
+          starts_k=[0] + [sum(lens_k[:b]) for b in range(1, sequences)])
+  else:
+    check(out, q, k, v, lens_q, lens_k)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("sequences,top", [(192, 30), (193, 30), (300, 400), (4097, 20), (9000, 3)])
 def test_many_sequences(sequences, top, causal):

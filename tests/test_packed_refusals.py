@@ -347,3 +347,46 @@ def test_order_of_the_row_tiles(B, causal):
     assert sorted(order) == [(b, t) for b in range(B) for t in range(tiles[b])]
     steps = [-(-keys(b, t) // 64) for b, t in order]
     assert steps == sorted(steps, reverse=True)
+
+
+@pytest.mark.parametrize("share", [1, 16, 32, 128, 256])
+def test_key_slices_of_different_sequences(share):
+  """Slices dealt out by keys: every tile has its own, no more than the launch, and tiles that do not exist are noted so."""
+  g = torch.Generator().manual_seed(share)
+  draw = lambda top: int(torch.randint(0, top, (1,), generator=g))
+  ceil = lambda a, b: -(-a // b)
+  for trial in range(40):
+    B, unit = 1 + draw(64), (128, 256)[draw(2)]
+    tiles = [draw(3) for _ in range(B)]
+    units = [ceil((0, 1, draw(300), draw(70000))[draw(4)], unit) for _ in range(B)]
+    bound, all_tiles = sum(tiles) + draw(5), sum(tiles)
+    total = sum(n * u for n, u in zip(tiles, units))
+    assert total < 1 << 23
+    over = lambda n: max(ceil(total, n), 1)
+    split = lambda c: [max(ceil(u, c), 1) for u in units]
+    used = lambda c: sum(n * z for n, z in zip(tiles, split(c)))
+    c = over(share)
+    high = c if share <= all_tiles or used(c) <= share else over(share - all_tiles)
+    while c < high:
+      mid = (c + high) // 2
+      c, high = (c, mid) if used(mid) <= share else (mid + 1, high)
+    z = split(c)
+    assert used(c) <= share + all_tiles and (share <= all_tiles or used(c) <= share)
+    noted, slices = set(), []
+    for item in range(share + bound):
+      b, before, slot = 0, 0, 0
+      while b < B and item >= before + tiles[b] * z[b]:
+        before, slot, b = before + tiles[b] * z[b], slot + tiles[b], b + 1
+      if b == B:
+        slot = all_tiles + item - before
+        if slot < bound:
+          assert slot not in noted
+          noted.add(slot)
+        continue
+      tile, slice_ = divmod(item - before, z[b])
+      slices.append((b, tile, slice_))
+      if slice_ == 0:
+        assert slot + tile not in noted
+        noted.add(slot + tile)
+    assert noted == set(range(bound))
+    assert slices == [(b, t, i) for b in range(B) for t in range(tiles[b]) for i in range(z[b])]
