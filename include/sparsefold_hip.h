@@ -489,8 +489,9 @@ int sf_hip_diffusion_conditioning_fwd(const sf_diffusion_conditioning_args* a, v
  * influence on its result.  Offsets are clamped to the tensors: wrong ones give wrong results, no
  * access outside them.
  * bf16 or f16, last dimension contiguous, 16-byte aligned rows (strides multiples of 8); D % 8 == 0,
- * D <= 128; k_s[0], v_s[0] in [D, 2^24).  fp32 softmax and accumulation; the weights are rounded to
- * the element type for the product with v.  out may not overlap q, k or v. */
+ * D <= 128; k_s[0], v_s[0] in [D, 2^24); Tk and Tq * G up to 2^30; B is any number of sequences.  fp32
+ * softmax and accumulation; the weights, up to 2^60 in bf16 and 2^12 in f16 before the division by their sum, are
+ * rounded to the element type for the product with v.  out holds each element once and may not overlap q, k or v. */
 typedef struct sf_packed_attention_args {
   int32_t B, H, Hkv, D;
   int64_t Tq, Tk;                               /* rows of q / out and of k / v */
@@ -514,7 +515,7 @@ int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, void* workspa
  *   radians and multiplied by `magnitude`; dims R .. D - 1 keep x'.
  * The angle is formed and reduced in 64 bits, the rest is fp32, rounded once.  q [T, H, D] and
  * k [T, Hk, D] (Hk = 0: none) share token positions; the last dimension is contiguous.  q_out may be q
- * and k_out may be k (same strides); otherwise outputs overlap no input.  D <= 256, R even, 2 <= R <= D.
+ * and k_out may be k (same strides); otherwise outputs overlap no input.  H, Hk <= 2^24, D <= 256, R even, 2 <= R <= D.
  * Weights and biases f32 [D] or NULL (1 and 0), read only where norm asks for them. */
 #define SF_NORM_NONE 0
 #define SF_NORM_RMS 1

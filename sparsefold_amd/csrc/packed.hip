@@ -14,6 +14,7 @@
 //   packed_tile_kernel    workgroups of many rows: K and V tiles of 64 keys shared through LDS
 //   packed_stream_kernel  32 rows: each wave streams its own slice of the keys
 //   packed_combine_kernel joins the slices of different workgroups
+// and one that counts row tiles before them where there are many sequences (packed_starts_kernel).
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -630,16 +631,25 @@ struct Stage {
   }
 };
 
-// Workgroups of NW waves, 32 rows each, over shared K/V tiles of 64 keys: two LDS buffers and
-// one barrier a tile; the tile after the next is in flight to registers meanwhile.  Tiles go from
-// the last that the rows see to the first, the partly visible ones first.
-template <class E, int KC, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
+// Workgroups of KG groups of NW waves: a wave has 32 rows, the groups have the same rows and take turns at the K/V
+// tiles of 64 keys.  A group has two LDS buffers and one barrier a tile; the tile after the next is in flight to
+// registers meanwhile.  Tiles go from the last that the rows see to the first, the partly visible ones
+// first.  S^T = K Q^T leaves a lane the weights of one row in the very layout that O^T += V^T P^T takes them in,
+// so they never pass through LDS; V is turned by its LDS read.
+//
+// Bound by the issue of matrix products and of the weights' vector instructions, which overlap little: 64 keys x 32 rows
+// of 128 dims take 435 and 249 ns, together 577 in a loop of registers alone (64 dims: 218, 237, 406).  A prompt of 16384,
+// 32 / 8 heads of 128, causal, bf16: 1.85 to 1.97 ms from card to card, 1.19 to 1.12 PFLOP/s (bf16 products of 8192^3:
+// 1.2 to 1.4), of 4096 136 to 144 us; 1.52 ms where all inputs are zero, which draw less power.  8192 tokens, 16
+// heads of 64: 168 us, 0.82 PFLOP/s.
+template <class E, int KC, int NW, int KG>
+__global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
   constexpr int kTile = 64 * T::kRow, R = 32 * NW;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * kTile];       // two buffers of K, V
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __attribute__((aligned(1024))) uint8_t shared[KG * 4 * kTile];          // a group: two buffers of K, V
+  const int tid = threadIdx.x % (64 * NW), lane = tid & 63, half = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW));
+  uint8_t* const smem = shared + group * 4 * kTile;
   // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
   const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
   const int slice = rest % pl.slices, idx = rest / pl.slices;
@@ -655,7 +665,7 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
     there = find_tile<R>(a, pl, idx, s, tile, ntiles);
     tile = ntiles - 1 - tile;
   }
-  if (pl.slices > 1 && hk + slice + tid == 0) note_tile(pl, idx, there, s, tile, idx * pl.slices, pl.slices);
+  if (pl.slices > 1 && hk + slice + (int)threadIdx.x == 0) note_tile(pl, idx, there, s, tile, idx * pl.slices, pl.slices);
   if (!there) return;
   const int rows = s.lq * pl.G, r0 = tile * R + wave * 32;
   const int row = min(r0 + li, rows - 1);                    // rows past the end repeat the last
@@ -674,50 +684,75 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
     Stage<KC, 64, 64 * NW> ks, vs;
     ks.init((const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1], a.k_s[0], tid, a.D);
     vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], tid, a.D);
-    int t = t_hi - 1;
-    ks.load(64 * t, s.lk, true);
-    vs.load(64 * t, s.lk, true);
-    // tile t in buffer t & 1
+    // this group's tiles t, t - KG, .. (all groups go as many steps: a last tile below t_lo is not read and has no weight)
+    int t = t_hi - 1 - group;
+    const int t_end = t_lo - group;
+    const auto buffer = [&]() __attribute__((always_inline)) { return (t >> (KG - 1)) & 1; };      // of tile t
+    ks.load(64 * t, s.lk, t >= t_lo);
+    vs.load(64 * t, s.lk, t >= t_lo);
     const auto kt = [&](int buf) __attribute__((always_inline)) { return smem + buf * 2 * kTile; };
     const auto vt = [&](int buf) __attribute__((always_inline)) { return smem + buf * 2 * kTile + kTile; };
-    ks.template store<false>(kt(t & 1), tid);
-    vs.template store<true>(vt(t & 1), tid);
-    ks.load(64 * (t - 1), s.lk, t - 1 >= t_lo);
-    vs.load(64 * (t - 1), s.lk, t - 1 >= t_lo);
+    ks.template store<false>(kt(buffer()), tid);
+    vs.template store<true>(vt(buffer()), tid);
+    ks.load(64 * (t - KG), s.lk, t - KG >= t_lo);
+    vs.load(64 * (t - KG), s.lk, t - KG >= t_lo);
     lds_only_barrier();
-    for (; t >= t_lo && 64 * t > high; --t) {                // tiles that none of this wave's rows sees
-      ks.template store<false>(kt(~t & 1), tid);
-      vs.template store<true>(vt(~t & 1), tid);
-      ks.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
-      vs.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
+    for (; t >= t_end && 64 * t > high; t -= KG) {           // tiles that none of this wave's rows sees
+      ks.template store<false>(kt(buffer() ^ 1), tid);
+      vs.template store<true>(vt(buffer() ^ 1), tid);
+      ks.load(64 * (t - 2 * KG), s.lk, t - 2 * KG >= t_lo);
+      vs.load(64 * (t - 2 * KG), s.lk, t - 2 * KG >= t_lo);
       lds_only_barrier();
     }
     // (the buffers as constants: LDS addresses are formed once)
-    auto step = [&](auto buffer) __attribute__((always_inline)) {
-      constexpr int B = decltype(buffer)::value;
+    auto step = [&](auto constant) __attribute__((always_inline)) {
+      constexpr int B = decltype(constant)::value;
       f32x16 sc[2];
       // meanwhile the next tile goes to the other buffer, and the one after it is asked for
       st.template products<2>(kt(B), sc, [&](int x) __attribute__((always_inline)) {
         if (x == 0) ks.template store<false>(kt(B ^ 1), tid);
         if (x == 1) vs.template store<true>(vt(B ^ 1), tid);
-        if (x == 2) ks.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
-        if (x == 3) vs.load(64 * (t - 2), s.lk, t - 2 >= t_lo);
+        if (x == 2) ks.load(64 * (t - 2 * KG), s.lk, t - 2 * KG >= t_lo);
+        if (x == 3) vs.load(64 * (t - 2 * KG), s.lk, t - 2 * KG >= t_lo);
       });
-      if (64 * t + 63 > low) st.template hide<2>(sc, mine - 64 * t);
+      if (64 * t + 63 > low || (KG > 1 && t < t_lo)) st.template hide<2>(sc, KG > 1 && t < t_lo ? -1 : mine - 64 * t);
       uint32_t p[16];
       st.template weights<2>(sc, p);
       st.template gather<2>(p, vt(B), [](int) {});
       lds_only_barrier();
-      --t;
+      t -= KG;
     };
-    if (t >= t_lo && (t & 1)) step(std::integral_constant<int, 1>{});
-    while (t >= t_lo) {
+    if (t >= t_end && buffer() != 0) step(std::integral_constant<int, 1>{});
+    while (t >= t_end) {
       step(std::integral_constant<int, 0>{});
-      if (t < t_lo) break;
+      if (t < t_end) break;
       step(std::integral_constant<int, 1>{});
     }
+    if constexpr (KG > 1) {
+      // the second group's sums, lane by lane, to the first
+      f32x4* const so = reinterpret_cast<f32x4*>(shared) + wave * 64 * (4 * T::DB + 1) + lane;
+      if (group == 1) {
+#pragma unroll
+        for (int x = 0; x < 4 * T::DB; ++x)
+          so[64 * x] = f32x4{st.o[x / 4][4 * (x % 4)], st.o[x / 4][4 * (x % 4) + 1], st.o[x / 4][4 * (x % 4) + 2], st.o[x / 4][4 * (x % 4) + 3]};
+        so[64 * 4 * T::DB] = f32x4{st.m, st.l, 0.f, 0.f};
+      }
+      lds_only_barrier();
+      if (group == 0) {
+        const f32x4 ml = so[64 * 4 * T::DB];
+        const float m = fmaxf(st.m, ml[0]), w0 = rescale<E>(st.m, m, st.c0), w1 = rescale<E>(ml[0], m, st.c0);
+        st.m = m;
+        st.l = st.l * w0 + ml[1] * w1;
+#pragma unroll
+        for (int x = 0; x < 4 * T::DB; ++x) {
+          const f32x4 o = so[64 * x];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st.o[x / 4][4 * (x % 4) + e] = st.o[x / 4][4 * (x % 4) + e] * w0 + o[e] * w1;
+        }
+      }
+    }
   }
-  if (r0 >= rows) return;                                    // (no barrier from here on)
+  if (r0 >= rows || group > 0) return;                       // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
   if (pl.slices > 1) {
     float* po = pl.part + (int64_t)blockIdx.x * R * (T::DP + 2);
@@ -769,8 +804,10 @@ __global__ __launch_bounds__(64 * NW, 2) void packed_tile_kernel(const sf_packed
 
 // 32 rows a workgroup (a new token's heads, short pieces): its 4 waves each stream a slice of the
 // keys, no barrier until the slices are joined: K straight into the registers of the matrix operand,
-// V through registers to LDS of the wave's own.  Bound by the reads of K and V; with few rows the
-// workgroups themselves take slices (pl.slices), joined by packed_combine_kernel.
+// V through registers to LDS of the wave's own.  With few rows the keys are split over workgroups too, joined by
+// packed_combine_kernel.  Bound by the reads of K and V: 64 tokens over caches of 2048, 32 / 8 heads of 128, 537 MB in 110
+// us, 4.9 TB/s; where there is less, by start, join and the latency of their loads: one token over 65536 keys, 16 / 2 heads, 67
+// MB in 21.7 us, of which the join is 5.
 template <class E, int KC>
 __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
@@ -918,7 +955,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 // against the largest.  LR lanes of 4 dims take a row.  R: rows of a tile; pl.pieces blocks share a
 // tile.  From packed_stream_kernel (R = 32: few rows, up to 64 slices) a block takes a row at a time, its
 // lane groups the slices z, z + GROUPS, .., joined through LDS; from packed_tile_kernel (few slices) a
-// group takes a row and a block 32 of them.
+// group takes a row and a block 32 of them.  Latency: 4 to 6 us with its launch, whatever it joins up to some MB.
 template <class E, int DP, int R>
 __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   constexpr int LR = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, GROUPS = 256 / LR;
@@ -1024,7 +1061,8 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Route {
-  int nw;            // waves of packed_tile_kernel's workgroups; 0: packed_stream_kernel
+  int nw;            // waves of rows of packed_tile_kernel's workgroups; 0: packed_stream_kernel
+  int groups;        // of such waves, that share the keys
   int kc, dp;
   PackedPlan pl;
   int64_t wgs;
@@ -1065,7 +1103,8 @@ int route(const sf_packed_attention_args* a, Route& r) {
   r.dp = 32 * ((r.kc + 1) / 2);
   const int64_t rows = a->Tq * G;
   // keys that a row of an average sequence sees, on average
-  int64_t seen = (a->Tk + a->B - 1) / a->B;
+  const int64_t keys = (a->Tk + a->B - 1) / a->B;
+  int64_t seen = keys;
   if (a->causal) seen -= seen < a->Tq / a->B ? seen / 2 : a->Tq / a->B / 2;
   // Up to 64 rows a sequence stream their keys.  Above, tiles of 128 rows; of 256 (half the reads of K and V)
   // where head dims above 64 meet long rows and two workgroups a CU: prompt of 8192, 32 / 8 heads of 128, 128 and 256
@@ -1076,14 +1115,19 @@ int route(const sf_packed_attention_args* a, Route& r) {
   const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
   const int64_t full = (rows + R - 1) / R, wgs = (full > a->B ? full : a->B) * a->Hkv;
   int64_t slices, share = 0;
+  r.groups = 1;
   if (r.nw) {
-    // Few workgroups: slices of the keys.  Two workgroups a CU where a slice keeps 1024 keys, else one, and
-    // no slice below 512 (prompt of 512 over 8192 keys, 32 / 8 heads of 128, 1 / 2 / 4 slices: 152 / 95 / 85 us;
-    // 128 over 8192, 1 / 4 / 8 / 16: 144 / 50 / 37 / 42; 1024 over 1024, 16 heads of 64, 1 / 2: 18.3 / 20.6).
-    slices = 512 / wgs;
-    if (slices > 1 && seen / slices < 1024) slices = 256 / wgs;
-    if (slices > seen / 512) slices = seen / 512;
-    if (r.nw == 8) slices = 1;                               // (512 workgroups and more)
+    // Few workgroups: two groups of waves share the keys of a workgroup, and workgroups take slices of them, no slice
+    // below 512 keys, or 256 on average where the first rows see few (causal without a cache).  Two slices want 1024
+    // keys each, for the join.  us with one group and one slice / two groups / groups and slices: prompt of 1024, 16 heads of 64,
+    // 18.5 / 15.8 / 20.7 with 2 slices; 2048 31.2 / 24.9; 4096 (512 workgroups) 61 / 52, 4 of 1024 23.3 / 25.3; 2048 of 48,
+    // all keys, 29.6 / 25.4 / 38.4; 512 over 8192, 32 / 8 heads of 128, 152 / 119 / 84 with 2, 128 over 8192 144 / 111 / 38 with 8.
+    const bool triangle = a->causal && seen * 4 < keys * 3;
+    if (r.nw == 4 && (wgs <= 256 ? seen >= 256 : wgs <= 512 && triangle && seen >= 1024)) r.groups = 2;
+    slices = 256 / wgs;
+    const int64_t most = seen / (triangle ? 256 : 512);
+    if (slices > most) slices = most;
+    if (slices < 3 && seen < 2048) slices = 1;
   } else {
     const int64_t least = r.dp > 64 ? 128 : 256;
     slices = 256 / wgs;
@@ -1123,9 +1167,10 @@ int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
   if (r.nw == 0) {
     hipLaunchKernelGGL((packed_stream_kernel<E, KC>), grid, dim3(256), 0, st, *a, r.pl);
   } else if (r.nw == 4) {
-    hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4>), grid, dim3(256), 0, st, *a, r.pl);
+    if (r.groups == 2) hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4, 2>), grid, dim3(512), 0, st, *a, r.pl);
+    else hipLaunchKernelGGL((packed_tile_kernel<E, KC, 4, 1>), grid, dim3(256), 0, st, *a, r.pl);
   } else if constexpr (KC > 4) {
-    hipLaunchKernelGGL((packed_tile_kernel<E, KC, 8>), grid, dim3(512), 0, st, *a, r.pl);
+    hipLaunchKernelGGL((packed_tile_kernel<E, KC, 8, 1>), grid, dim3(512), 0, st, *a, r.pl);
   }
   const int rc = sf_check_launch(r.nw ? "packed_tile_kernel" : "packed_stream_kernel");
   if (rc || !r.joined()) return rc;

@@ -361,6 +361,24 @@ def test_other_streams_at_once():
     check(out, q, k, v, [1], [6000], True)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 48, 64, 96, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens_q,lens_k", [([300, 65, 513], [300, 65, 513]), ([70, 200], [961, 449]), ([450, 90], [600, 10]), ([129], [4100])])
+def test_groups_of_waves_that_share_the_keys(lens_q, lens_k, causal, D, dtype):
+  """Few workgroups: odd and even numbers of key tiles, fewer keys than queries, waves without rows, slices besides."""
+  q, k, v = make(lens_q, lens_k, 4, 2, D, TYPES[dtype], D)
+  if causal:
+    v[sum(lens_k) - 1] = math.inf                    # the last key, which only the last query sees
+  out = ops.packed_attention(q, k, v, offsets(lens_q), offsets(lens_k), causal=causal)
+  if causal:
+    assert not torch.isfinite(out[-1].float()).any()
+    out[-1], v[-1] = 0.0, 0.0
+    check(out[:-1], q[:-1], k[:-1], v[:-1], lens_q[:-1] + [lens_q[-1] - 1], lens_k[:-1] + [lens_k[-1] - 1], True)
+  else:
+    check(out, q, k, v, lens_q, lens_k)
+
+
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64), ("bf16", 24)])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("sequences,heads", [(2, (16, 2)), (7, (8, 2)), (30, (8, 1)), (64, (3, 1))])
