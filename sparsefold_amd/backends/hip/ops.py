@@ -614,6 +614,11 @@ def _launch(fn, t: torch.Tensor, what: str, *args) -> None:
       _lib.check(fn(*args, _stream(t)), what)
 
 
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+  """An uninitialised packed tensor like t (half the host time of ``torch.empty`` with a shape)."""
+  return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _strides2(t: torch.Tensor) -> tuple[int, int]:
   """Row and head strides of ``[T, H, D]``; those of a single row or head, which torch leaves
   arbitrary, as if packed."""
@@ -727,7 +732,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
 
   given = out
   if out is None:
-    out = torch.empty(qs, dtype=dtype, device=dev)
+    out = _fresh(q)
     so = (H * D, D)
   else:
     so = _strides2(out) if out.ndim == 3 else (0, 0)
@@ -783,7 +788,7 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str |
 
 def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, norm=0, eps=0.0, weights=(None,) * 4):
   _no_grad(what, q, k, freqs, out_q, out_k, *weights)
-  dev = _require_cuda(q, k, positions, freqs, out_q, out_k, *weights)
+  _require_cuda(q, k, positions, freqs, out_q, out_k, *weights)
   qs, ks = q.shape, None if k is None else k.shape
   nd = len(qs)
   if nd < 3 or (ks is not None and (len(ks) != nd or ks[-1] != qs[-1] or (ks[0] != qs[0] if nd == 3 else ks[:-2] != qs[:-2]))):
@@ -832,7 +837,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
   sq = _strides2(q3)
   T = q3.shape[0]
   if out_q is None:
-    out_q = torch.empty(qs, dtype=dtype, device=dev)
+    out_q = _fresh(q)
     oq3, so = out_q, (H * D, D)
   else:
     oq3 = given(out_q, q, "out_q")
@@ -842,7 +847,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
     Hk, k3 = ks[-2], three(k)
     kp, sk = k3.data_ptr(), _strides2(k3)
     if out_k is None:
-      out_k = torch.empty(ks, dtype=dtype, device=dev)
+      out_k = _fresh(k)
       ok3, sok = out_k, (Hk * D, D)
     else:
       ok3 = given(out_k, k, "out_k")
