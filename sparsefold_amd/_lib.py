@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 from pathlib import Path
+from struct import Struct
 
 LIB_PATH = Path(__file__).resolve().parent / "libsparsefold_hip.so"
 ABI_VERSION = 12
@@ -194,6 +195,25 @@ STRUCTS = {
     "sf_packed_attention_args": PackedAttentionArgs,
     "sf_rotary_args": RotaryArgs,
 }
+
+
+def filler(struct: type[C.Structure]):
+  """``filler(S)(*values)`` is an ``S`` of the fields' values in order, arrays value by value and null pointers as 0:
+  packed in one call, a third of the time of the constructor, which the small calls notice."""
+  codes = {_i32: "i", _i64: "q", _f32: "f", _vp: "P"}
+  layout = Struct("@" + "".join(codes[getattr(t, "_type_", t)] * t._length_ if issubclass(t, C.Array) else codes[t]
+                                for _, t in struct._fields_))
+  assert layout.size <= C.sizeof(struct)
+
+  def fill(*values):
+    a = struct()
+    layout.pack_into(a, 0, *values)
+    return a
+  return fill
+
+
+packed_attention_args = filler(PackedAttentionArgs)
+rotary_args = filler(RotaryArgs)
 
 # (name, restype, argtypes) of every exported entry point.
 SIGNATURES = [

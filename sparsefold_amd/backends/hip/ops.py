@@ -41,12 +41,13 @@ def _require_cuda(*ts: torch.Tensor | None) -> torch.device:
   for t in ts:
     if t is None:
       continue
-    if not t.is_cuda:
-      raise ValueError(f"HIP kernels need device tensors, got a tensor on {t.device}")
-    if first is None:
-      first, index = t, t.get_device()
-    elif t.get_device() != index:
-      raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    i = t.get_device()                                         # (-1 on the host)
+    if i != index or i < 0:
+      if not t.is_cuda:
+        raise ValueError(f"HIP kernels need device tensors, got a tensor on {t.device}")
+      if first is not None:
+        raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+      first, index = t, i
   if first is None:
     raise ValueError("no device tensor given")
   return first.device
@@ -744,8 +745,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
   q, qp, sq = rows(q, 0)
   k, kp, sk = rows(k, D)
   v, vp, sv = rows(v, D)
-  a = _lib.PackedAttentionArgs(B, H, Hkv, D, Tq, Tk, scale, int(bool(causal)), _ELEMENT_TYPES[dtype], qp, sq, kp, sk, vp, sv,
-                               out.data_ptr(), so, cu_q.data_ptr(), cu_k.data_ptr(), _vp(len_q), _vp(len_k))
+  a = _lib.packed_attention_args(B, H, Hkv, D, Tq, Tk, scale, bool(causal), _ELEMENT_TYPES[dtype], qp, *sq, kp, *sk, vp, *sv,
+                                 out.data_ptr(), *so, cu_q.data_ptr(), cu_k.data_ptr(), _vp(len_q) or 0, _vp(len_k) or 0)
   lib = _lib.load()
   ref = C.byref(a)
   need = lib.sf_hip_packed_attention_workspace_bytes(ref)
@@ -812,8 +813,8 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
     except RuntimeError:
       raise ValueError(f"{what}: positions {tuple(positions.shape)} do not fit tokens {tuple(qs[:-2])}") from None
     positions = positions.reshape(-1)
-  if not math.isfinite(magnitude):
-    raise ValueError(f"{what}: magnitude {magnitude} is not finite")
+  if not abs(magnitude) <= 1e30:
+    raise ValueError(f"{what}: magnitude {magnitude} is not finite or above 1e30")
 
   def three(t):
     t3 = t if flat else t.reshape(-1, t.shape[-2], D)
@@ -842,7 +843,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
   else:
     oq3 = given(out_q, q, "out_q")
     so = _strides2(oq3)
-  Hk, k3, ok3, kp, sk, okp, sok = 0, None, None, None, (0, 0), None, (0, 0)
+  Hk, k3, ok3, kp, sk, okp, sok = 0, None, None, 0, (0, 0), 0, (0, 0)
   if k is not None:
     Hk, k3 = ks[-2], three(k)
     kp, sk = k3.data_ptr(), _strides2(k3)
@@ -862,9 +863,9 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
         raise ValueError(f"{what}: outputs may be their own input in place, and overlap nothing else")
   positions, freqs = positions.contiguous(), freqs.contiguous()
   qw, kw, qb, kb = weights
-  a = _lib.RotaryArgs(T, H, Hk, D, 2 * pairs, int(bool(interleaved)), _ELEMENT_TYPES[dtype], norm, eps, magnitude, q3.data_ptr(), sq,
-                      kp, sk, oq3.data_ptr(), so, okp, sok, positions.data_ptr(), int(pdtype is torch.int64), freqs.data_ptr(),
-                      _vp(qw), _vp(qb), _vp(kw), _vp(kb))
+  a = _lib.rotary_args(T, H, Hk, D, 2 * pairs, bool(interleaved), _ELEMENT_TYPES[dtype], norm, eps, magnitude, q3.data_ptr(), *sq,
+                       kp, *sk, oq3.data_ptr(), *so, okp, *sok, positions.data_ptr(), pdtype is torch.int64, freqs.data_ptr(),
+                       _vp(qw) or 0, _vp(qb) or 0, _vp(kw) or 0, _vp(kb) or 0)
   _launch(_lib.load().sf_hip_rotary_fwd, q3, "sf_hip_rotary_fwd", C.byref(a))
   _written(given_q, given_k)
   return out_q, out_k
@@ -900,8 +901,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
     raise ValueError(f"{what}: biases need norm='layer'")
   if k is None and (k_weight is not None or k_bias is not None):
     raise ValueError(f"{what}: a key weight or bias without k")
-  if not 0.0 <= eps < math.inf:
-    raise ValueError(f"{what}: eps {eps} is not finite and >= 0")
+  if not 0.0 <= eps <= 1e30:
+    raise ValueError(f"{what}: eps {eps} is not finite and >= 0, or above 1e30")
   weights = (q_weight, k_weight, q_bias, k_bias)
   ready = []
   for w in weights:

@@ -118,6 +118,13 @@ def test_outputs_that_expect_a_gradient_are_refused():
     ops.rotary(torch.zeros(6, 4, 32, dtype=BF), None, torch.arange(6), ops.rotary_frequencies(32), out_q=leaf)
 
 
+def test_scalars_past_32_bit_floats_are_refused():
+  with pytest.raises(ValueError, match="magnitude"):
+    ops.rotary(**rotary_args(magnitude=1e300))
+  with pytest.raises(ValueError, match="eps"):
+    ops.qk_norm_rotary(**rotary_args(), q_weight=None, k_weight=None, eps=1e300)
+
+
 def test_more_heads_than_fit_are_refused():
   many = torch.zeros(1, 1, 8, dtype=BF).expand(1, (1 << 24) + 1, 8)
   with pytest.raises(ValueError, match="2\\^24"):
@@ -390,3 +397,24 @@ def test_key_slices_of_different_sequences(share):
         noted.add(slot + tile)
     assert noted == set(range(bound))
     assert slices == [(b, t, i) for b in range(B) for t in range(tiles[b]) for i in range(z[b])]
+
+
+@pytest.mark.parametrize("name", ["sf_packed_attention_args", "sf_rotary_args"])
+def test_filled_structs(name):
+  """The packed fields are the constructor's."""
+  struct = _lib.STRUCTS[name]
+  fill = {"sf_packed_attention_args": _lib.packed_attention_args, "sf_rotary_args": _lib.rotary_args}[name]
+  values, flat = [], []
+  for i, (_, t) in enumerate(struct._fields_):
+    if issubclass(t, C.Array):
+      values.append((-i, 1 << 40))
+      flat += [-i, 1 << 40]
+    else:
+      values.append(i / 4 if t is C.c_float else None if t is C.c_void_p and i % 2 else i)
+      flat.append(values[-1] or 0)
+  a, b = struct(*values), fill(*flat)
+  for field, t in struct._fields_:
+    x, y = getattr(a, field), getattr(b, field)
+    assert list(x) == list(y) if issubclass(t, C.Array) else x == y
+  with pytest.raises(Exception, match="argument out of range|format requires"):
+    fill(*([1 << 40] * len(flat)))
