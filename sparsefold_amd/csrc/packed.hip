@@ -15,6 +15,7 @@
 //   packed_stream_kernel  32 rows: each wave streams its own slice of the keys
 //   packed_combine_kernel joins the slices of different workgroups
 // and one that counts row tiles before them where there are many sequences (packed_starts_kernel).
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -81,6 +82,7 @@ struct PackedPlan {
   int tiles;         // bound on the row tiles of one key head
   int slices;        // key slices (workgroups) of every row tile, where there is no share
   int share;         // packed_stream_kernel: slices of all row tiles of a key head together, dealt out by their keys (0: slices)
+  int whole;         // with a share: no slices where the longest sequence is near the mean
   int pieces;        // blocks of packed_combine_kernel per row tile
   float c0;          // scale log2 e
   int G;             // query heads of a key head
@@ -94,6 +96,9 @@ struct PackedPlan {
 // counts them for all, a launch of its own (sequences of 20 tokens, 8 heads of 64, counted by each / for all: 130 of
 // them 20.8 / 22.7 us, 256 37.7 / 31.2, 512 90 / 55, 8192 12370 / 797).
 constexpr int kScanned = 192;
+
+// Up to as many share key slices (find_slice).
+constexpr int kShared = 256;
 
 // r / G without a division: (r + 0.5) / G is at least 0.5 / G away from a whole number.
 __device__ __forceinline__ int token_of(const PackedPlan& pl, int r) { return (int)(((double)r + 0.5) * pl.inv_g); }
@@ -284,52 +289,81 @@ __device__ __forceinline__ void note_tile(const PackedPlan& pl, int slot, bool t
   pl.found[2 * slot + 1] = there ? int4{s.k0, first, slices, 0} : int4{0, 0, 0, 0};
 }
 
-// Slice `item` of all, where the tiles of up to 64 sequences (a lane each) share pl.share slices by their keys, in
+// Slice `item` of all, where the tiles of up to 64 N sequences (N a lane) share pl.share slices by their keys, in
 // slices of c units of `unit` keys: the smallest c that needs no more than the share, one slice a tile aside.  c is at
 // least all units / share, which needs share + tiles at most (the launch's bound), and at most all units / (share - tiles).
 // False past the last; `slot` is the tile's number among all, past the last slice one that no tile has.
+template <int N>
 __device__ __forceinline__ bool find_slice(const sf_packed_attention_args& a, const PackedPlan& pl, int unit, int item, Seq& s, int& tile,
                                            int& slot, int& slice, int& slices) {
   const int lane = threadIdx.x & 63;
-  int start = 0, n = 0, k0 = 0, lk = 0;
-  if (lane < a.B) {
-    seq_range(a.cu_q, a.len_q, lane, a.Tq, start, n);
-    seq_range(a.cu_k, a.len_k, lane, a.Tk, k0, lk);
+  int start[N], n[N], k0[N], lk[N], nt[N], units[N], own_tiles = 0, longest = 0;
+  float own_units = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int b = N * lane + j;
+    start[j] = n[j] = k0[j] = lk[j] = 0;
+    if (b < a.B) {
+      seq_range(a.cu_q, a.len_q, b, a.Tq, start[j], n[j]);
+      seq_range(a.cu_k, a.len_k, b, a.Tk, k0[j], lk[j]);
+    }
+    nt[j] = (int)(((uint32_t)n[j] * (uint32_t)pl.G + 31) / 32);
+    units[j] = (lk[j] + unit - 1) / unit;
+    own_tiles += nt[j];
+    own_units += (float)nt[j] * (float)units[j];
+    longest = max(longest, units[j]);
   }
-  const int nt = (int)(((uint32_t)n * (uint32_t)pl.G + 31) / 32), units = (lk + unit - 1) / unit;
-  const int tiles = lanes_before_and_own(nt), all = __builtin_amdgcn_readlane(tiles, 63);
+  const int tiles = lanes_before_and_own(own_tiles), all = __builtin_amdgcn_readlane(tiles, 63);
   slot = item;
   if (all > pl.tiles) return false;                          // (offsets that do not increase)
-  const float total = lanes_sum((float)nt * (float)units);
+  const float total = lanes_sum(own_units);
   const auto over = [&](int n) __attribute__((always_inline)) {                // ceil(total / n)
     // (whole numbers up to 2^23 are exact; above, the quotient is kept from falling short)
     return total < 8388608.f ? max(((uint32_t)total + n - 1) / n, 1u) : (uint32_t)fminf(ceilf(total / (float)n * 1.000001f), 1e9f);
   };
-  const auto split = [&](uint32_t c) __attribute__((always_inline)) { return (int)max((units + c - 1) / c, 1u); };
+  const auto split = [&](int j, uint32_t c) __attribute__((always_inline)) { return (int)max((units[j] + c - 1) / c, 1u); };
+  const auto needs = [&](uint32_t c) __attribute__((always_inline)) {          // the lane's slices
+    int v = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v += nt[j] * split(j, c);
+    return v;
+  };
   uint32_t c = over(pl.share);
-  const bool fits = pl.share <= all || lanes_sum(nt * split(c)) <= pl.share;
+  if (pl.whole && !__any((float)longest * (float)all > 1.25f * total)) c = 1u << 30;
+  const bool fits = pl.share <= all || c == 1u << 30 || lanes_sum(needs(c)) <= pl.share;
   for (uint32_t high = fits ? c : over(pl.share - all); c < high;) {
     const uint32_t mid = (c + high) / 2;
-    if (lanes_sum(nt * split(mid)) <= pl.share) high = mid;
+    if (lanes_sum(needs(mid)) <= pl.share) high = mid;
     else c = mid + 1;
   }
-  const int z = split(c);
-  const int items = lanes_before_and_own(nt * z);
+  const int own_items = needs(c), items = lanes_before_and_own(own_items);
   const uint64_t past = __ballot(items > item);
   if (past == 0) {
     slot = all + item - __builtin_amdgcn_readlane(items, 63);
     return false;
   }
   const int src = __builtin_ctzll(past);
-  s.q0 = __builtin_amdgcn_readlane(start, src);
-  s.lq = __builtin_amdgcn_readlane(n, src);
-  s.k0 = __builtin_amdgcn_readlane(k0, src);
-  s.lk = __builtin_amdgcn_readlane(lk, src);
-  slices = __builtin_amdgcn_readlane(z, src);
-  const int r = item - __builtin_amdgcn_readlane(items - nt * z, src);
+  int r = item - __builtin_amdgcn_readlane(items - own_items, src);
+  slot = __builtin_amdgcn_readlane(tiles - own_tiles, src);
+  bool found = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int ntj = __builtin_amdgcn_readlane(nt[j], src), z = __builtin_amdgcn_readlane(split(j, c), src);
+    if (!found && r < ntj * z) {
+      found = true;
+      s.q0 = __builtin_amdgcn_readlane(start[j], src);
+      s.lq = __builtin_amdgcn_readlane(n[j], src);
+      s.k0 = __builtin_amdgcn_readlane(k0[j], src);
+      s.lk = __builtin_amdgcn_readlane(lk[j], src);
+      slices = z;
+    } else if (!found) {
+      r -= ntj * z;
+      slot += ntj;
+    }
+  }
   tile = r / slices;
   slice = r - tile * slices;
-  slot = __builtin_amdgcn_readlane(tiles - nt, src) + tile;
+  slot += tile;
   return true;
 }
 
@@ -822,7 +856,8 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   int tile, slice, slices;
   if (pl.share > 0) {
     int slot;
-    const bool there = find_slice(a, pl, 4 * KT, item, s, tile, slot, slice, slices);
+    const bool there = a.B <= 64 ? find_slice<1>(a, pl, 4 * KT, item, s, tile, slot, slice, slices)
+                                 : find_slice<4>(a, pl, 4 * KT, item, s, tile, slot, slice, slices);
     if (hk + tid == 0 && slot < pl.tiles && (!there || slice == 0)) note_tile(pl, slot, there && slices > 1, s, tile, item, slices);
     if (!there) return;
   } else {
@@ -1066,6 +1101,7 @@ struct Route {
   int kc, dp;
   PackedPlan pl;
   int64_t wgs;
+  bool counted;      // packed_starts_kernel counts the tiles
   bool joined() const { return pl.slices > 1 || pl.share > 0; }
 };
 
@@ -1115,6 +1151,7 @@ int route(const sf_packed_attention_args* a, Route& r) {
   const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
   const int64_t full = (rows + R - 1) / R, wgs = (full > a->B ? full : a->B) * a->Hkv;
   int64_t slices, share = 0;
+  bool whole = false;
   r.groups = 1;
   if (r.nw) {
     // Few workgroups: two groups of waves share the keys of a workgroup, and workgroups take slices of them, no slice
@@ -1132,26 +1169,32 @@ int route(const sf_packed_attention_args* a, Route& r) {
     const int64_t least = r.dp > 64 ? 128 : 256;
     slices = 256 / wgs;
     if (slices > seen / least) slices = seen / least;
-    // A workgroup a CU, slices dealt out by the keys (one token for 4 caches of 128 to 8192 keys, 32 / 8 heads of 128: 16.8
-    // us, as many slices for each 21.6; 4 caches of 4096: 20.5 / 20.1; 384 workgroups 20.2 / 25.3).  Beyond 64
-    // sequences as many for each.
-    if (slices > 1 && a->B <= 64) share = 256 / a->Hkv;
+    // Slices dealt out by the keys, a workgroup a CU or the next multiple of that (one token for 4 caches of 128 to 8192
+    // keys, 32 / 8 heads of 128: 16.8 us, as many slices for each 21.6; 32 of them 85 / 126; 100 of 64 to 4096 93 / 141; 384
+    // workgroups in place of 256 25 / 20).  From 256 workgroups on only where sequences are uneven and long: of one length
+    // the join's launch is lost (4 caches of 4096 20.5 / 20.1, 32 of 4096 108 / 104, 32 of 1024 30 / 28).
+    if (a->B <= kShared && seen >= 2 * least && (wgs < 256 || seen >= 512)) {
+      share = 256 * (wgs / 256 + 1) / a->Hkv;
+      whole = wgs >= 256;
+    }
   }
   slices = slices < 1 || share > 0 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;
+  r.counted = a->B > kScanned && share == 0;
   // rows of a tile join in blocks of 32, or -- packed_stream_kernel -- one by one, as many blocks as a
-  // sequence has rows on average
+  // sequence has rows on average, but few where there are many tiles, most of which need no join
   int64_t pieces = r.nw ? r.nw : (rows + a->B - 1) / a->B;
   if (pieces > 32) pieces = 32;
+  if (r.nw == 0) pieces = std::max<int64_t>(std::min(pieces, 1024 / (tiles * a->Hkv)), 1);
   float c0 = a->scale * SF_LOG2E;
   if (fabsf(c0) < FLT_MIN) c0 = FLT_MIN;                     // all logits equal; a masked one stays -inf
-  r.pl = PackedPlan{(int)tiles, (int)slices, (int)share, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr, nullptr};
+  r.pl = PackedPlan{(int)tiles, (int)slices, (int)share, (int)whole, (int)pieces, c0, G, 1.0 / G, nullptr, nullptr, nullptr};
   r.wgs = (share > 0 ? share + tiles : tiles * slices) * a->Hkv;
   if (r.wgs > INT32_MAX || tiles * a->Hkv * 32 > INT32_MAX) { sf_set_error("packed attention: problem too large for the grid"); return 1; }
   return 0;
 }
 
 size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
-  const size_t starts = a->B > kScanned ? ((size_t)a->B + 1) * sizeof(int) : 0;
+  const size_t starts = r.counted ? ((size_t)a->B + 1) * sizeof(int) : 0;
   if (!r.joined()) return starts;                       // (so many sequences fill the GPU)
   const int R = r.nw ? 32 * r.nw : 32;
   return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float) + (size_t)r.pl.tiles * 2 * sizeof(int4);
@@ -1211,7 +1254,7 @@ extern "C" int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, vo
     return 1;
   }
   r.pl.part = static_cast<float*>(workspace);
-  if (a->B > kScanned) r.pl.starts = static_cast<int*>(workspace);
+  if (r.counted) r.pl.starts = static_cast<int*>(workspace);
   r.pl.found = reinterpret_cast<int4*>(r.pl.part + r.wgs * (r.nw ? 32 * r.nw : 32) * (r.dp + 2));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   return a->dtype == SF_DTYPE_BF16 ? launch_type<Bf16>(a, r, st) : launch_type<Fp16>(a, r, st);

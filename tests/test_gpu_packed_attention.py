@@ -381,7 +381,7 @@ def test_groups_of_waves_that_share_the_keys(lens_q, lens_k, causal, D, dtype):
 
 @pytest.mark.parametrize("dtype,D", [("bf16", 128), ("fp16", 64), ("bf16", 24)])
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("sequences,heads", [(2, (16, 2)), (7, (8, 2)), (30, (8, 1)), (64, (3, 1))])
+@pytest.mark.parametrize("sequences,heads", [(2, (16, 2)), (7, (8, 2)), (30, (8, 1)), (64, (3, 1)), (65, (16, 8)), (256, (4, 4))])
 def test_slices_by_keys(sequences, heads, causal, dtype, D):
   """Few rows over caches of very different lengths: long ones are split into many slices, short ones into none."""
   g = torch.Generator().manual_seed(sequences)
