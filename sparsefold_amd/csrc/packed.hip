@@ -1176,6 +1176,8 @@ int route(const sf_packed_attention_args* a, Route& r) {
     if (a->B <= kShared && seen >= 2 * least && (wgs < 256 || seen >= 512)) {
       share = 256 * (wgs / 256 + 1) / a->Hkv;
       whole = wgs >= 256;
+      // (many key heads of few rows each: the join's buffer, of 32 rows a slice, would exceed 256 MiB)
+      if (whole && (share + tiles) * a->Hkv * 32 * (r.dp + 2) > 64 << 20) share = 0;
     }
   }
   slices = slices < 1 || share > 0 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;

@@ -246,6 +246,14 @@ def test_c_attention_workspace(lib):
   assert lib.sf_hip_packed_attention_fwd(C.byref(a), None, 0, None) == 0
 
 
+@pytest.mark.parametrize("B,Hkv,need", [(1, 8, None), (64, 8, None), (128, 32, None), (256, 32, 257 * 4), (1000, 1, 1001 * 4), (100000, 4, 100001 * 4)])
+def test_c_attention_workspace_is_bounded(lib, B, Hkv, need):
+  """One token a sequence over long caches: the slices' buffer, 256 MiB at most, or the tiles before each sequence."""
+  a = packed_struct(B=B, H=2 * Hkv, Hkv=Hkv, D=128, Tq=B, Tk=B * 4096)
+  got = lib.sf_hip_packed_attention_workspace_bytes(C.byref(a))
+  assert got == need if need else 0 < got <= (256 << 20) + (1 << 16)
+
+
 def test_c_rotary_refuses(lib):
   def struct(**kw):
     a = _lib.RotaryArgs(T=5, H=4, Hk=0, D=32, R=32, dtype=0, norm=0, magnitude=1.0)
