@@ -720,12 +720,14 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     raise ValueError(f"packed_attention: scale {scale} is not finite or above 1e30")
 
   def rows(t, least):
+    ptr = t.data_ptr()
+    if t.is_contiguous() and ptr % 16 == 0 and t.shape[1] * D < 1 << 24:
+      return t, ptr, (t.shape[1] * D, D)
     st, sh, sd = t.stride()
     if t.shape[1] == 1:                                        # (a single head's or row's stride means nothing)
       sh = D
     if t.shape[0] <= 1:
       st = t.shape[1] * max(sh, D)
-    ptr = t.data_ptr()
     if sd != 1 or (st | sh | ptr >> 1) % 8 or not least <= st < 1 << 24:
       t = torch.empty(t.shape, dtype=dtype, device=dev).copy_(t)
       st, sh, ptr = t.shape[1] * D, D, t.data_ptr()
@@ -818,7 +820,8 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
 
   def three(t):
     t3 = t if flat else t.reshape(-1, t.shape[-2], D)
-    return t3 if D == 1 or t3.stride(2) == 1 else t3.contiguous()
+    t3 = t3 if t3.stride(2) == 1 else t3.contiguous()
+    return t3, _strides2(t3)
 
   def given(o, like, name):
     if o.shape != like.shape or o.dtype != dtype or (D > 1 and o.stride(-1) != 1):
@@ -834,8 +837,7 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
   if k is None and out_k is not None:
     raise ValueError(f"{what}: out_k without k")
   given_q, given_k = out_q, out_k
-  q3 = three(q)
-  sq = _strides2(q3)
+  q3, sq = (q, (H * D, D)) if flat and q.is_contiguous() else three(q)
   T = q3.shape[0]
   if out_q is None:
     out_q = _fresh(q)
@@ -845,8 +847,9 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
     so = _strides2(oq3)
   Hk, k3, ok3, kp, sk, okp, sok = 0, None, None, 0, (0, 0), 0, (0, 0)
   if k is not None:
-    Hk, k3 = ks[-2], three(k)
-    kp, sk = k3.data_ptr(), _strides2(k3)
+    Hk = ks[-2]
+    k3, sk = (k, (Hk * D, D)) if flat and k.is_contiguous() else three(k)
+    kp = k3.data_ptr()
     if out_k is None:
       out_k = _fresh(k)
       ok3, sok = out_k, (Hk * D, D)
@@ -861,7 +864,10 @@ def _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, 
     for a, b, own in meets:
       if not (_disjoint(a, b) or (own and same(a, b))):
         raise ValueError(f"{what}: outputs may be their own input in place, and overlap nothing else")
-  positions, freqs = positions.contiguous(), freqs.contiguous()
+  if not positions.is_contiguous():
+    positions = positions.contiguous()
+  if not freqs.is_contiguous():
+    freqs = freqs.contiguous()
   qw, kw, qb, kb = weights
   a = _lib.rotary_args(T, H, Hk, D, 2 * pairs, bool(interleaved), _ELEMENT_TYPES[dtype], norm, eps, magnitude, q3.data_ptr(), *sq,
                        kp, *sk, oq3.data_ptr(), *so, okp, *sok, positions.data_ptr(), pdtype is torch.int64, freqs.data_ptr(),
@@ -903,15 +909,12 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
     raise ValueError(f"{what}: a key weight or bias without k")
   if not 0.0 <= eps <= 1e30:
     raise ValueError(f"{what}: eps {eps} is not finite and >= 0, or above 1e30")
-  weights = (q_weight, k_weight, q_bias, k_bias)
-  ready = []
+  weights, D = (q_weight, k_weight, q_bias, k_bias), q.shape[-1]
   for w in weights:
     if w is not None:
-      if w.ndim != 1 or w.shape[0] != q.shape[-1]:
-        raise ValueError(f"{what}: weights and biases must be [{q.shape[-1]}], got {tuple(w.shape)}")
-      if w.requires_grad:
-        _no_grad(what, w)
+      if w.shape != (D,):
+        raise ValueError(f"{what}: weights and biases must be [{D}], got {tuple(w.shape)}")
       if w.dtype is not torch.float32 or not w.is_contiguous():
-        w = _f32(w)
-    ready.append(w)
-  return _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, _NORMS[norm], float(eps), ready)
+        _no_grad(what, *weights)
+        weights = tuple(x if x is None else _f32(x) for x in weights)
+  return _rotary(what, q, k, positions, freqs, interleaved, magnitude, out_q, out_k, _NORMS[norm], float(eps), weights)
