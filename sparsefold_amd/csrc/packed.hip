@@ -80,8 +80,8 @@ __device__ __forceinline__ float rescale(float m, float mnew, float c0) {
 
 struct PackedPlan {
   int tiles;         // bound on the row tiles of one key head
-  int slices;        // key slices (workgroups) of every row tile, where there is no share
-  int share;         // packed_stream_kernel: slices of all row tiles of a key head together, dealt out by their keys (0: slices)
+  int slices;        // packed_tile_kernel: key slices (workgroups) of every row tile
+  int share;         // packed_stream_kernel: slices of all row tiles of a key head together, dealt out by their keys (0: one each)
   int whole;         // with a share: no slices where the longest sequence is near the mean
   int pieces;        // blocks of packed_combine_kernel per row tile
   float c0;          // scale log2 e
@@ -839,8 +839,8 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
 // 32 rows a workgroup (a new token's heads, short pieces): its 4 waves each stream a slice of the
 // keys, no barrier until the slices are joined: K straight into the registers of the matrix operand,
 // V through registers to LDS of the wave's own.  With few rows the keys are split over workgroups too, joined by
-// packed_combine_kernel.  Bound by the reads of K and V: 64 tokens over caches of 2048, 32 / 8 heads of 128, 537 MB in 110
-// us, 4.9 TB/s; where there is less, by start, join and the latency of their loads: one token over 65536 keys, 16 / 2 heads, 67
+// packed_combine_kernel.  Bound by the reads of K and V: 64 tokens over caches of 2048, 32 / 8 heads of 128, 537 MB in 114
+// us, 4.7 TB/s; where there is less, by start, join and the latency of their loads: one token over 65536 keys, 16 / 2 heads, 67
 // MB in 21.7 us, of which the join is 5.
 template <class E, int KC>
 __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
@@ -862,12 +862,9 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
     if (!there) return;
   } else {
     int ntiles;
-    slices = pl.slices;
-    const int idx = item / slices;
-    slice = item - idx * slices;
-    const bool there = find_tile<32>(a, pl, idx, s, tile, ntiles);
-    if (slices > 1 && hk + slice + tid == 0) note_tile(pl, idx, there, s, tile, item, slices);
-    if (!there) return;
+    slice = 0;
+    slices = 1;
+    if (!find_tile<32>(a, pl, item, s, tile, ntiles)) return;
   }
   const int rows = s.lq * pl.G, r0 = tile * 32;
   const int row = min(r0 + li, rows - 1);
@@ -1150,7 +1147,7 @@ int route(const sf_packed_attention_args* a, Route& r) {
   // tiles end at sequence ends: sum_b ceil(rows_b / R) <= rows / R + B
   const int64_t tiles = rows / R + (a->B < rows ? a->B : rows);
   const int64_t full = (rows + R - 1) / R, wgs = (full > a->B ? full : a->B) * a->Hkv;
-  int64_t slices, share = 0;
+  int64_t slices = 1, share = 0;
   bool whole = false;
   r.groups = 1;
   if (r.nw) {
@@ -1165,22 +1162,21 @@ int route(const sf_packed_attention_args* a, Route& r) {
     const int64_t most = seen / (triangle ? 256 : 512);
     if (slices > most) slices = most;
     if (slices < 3 && seen < 2048) slices = 1;
+    slices = slices < 1 ? 1 : slices > 64 ? 64 : slices;
   } else {
     const int64_t least = r.dp > 64 ? 128 : 256;
-    slices = 256 / wgs;
-    if (slices > seen / least) slices = seen / least;
     // Slices dealt out by the keys, a workgroup a CU or the next multiple of that (one token for 4 caches of 128 to 8192
     // keys, 32 / 8 heads of 128: 16.8 us, as many slices for each 21.6; 32 of them 85 / 126; 100 of 64 to 4096 93 / 141; 384
     // workgroups in place of 256 25 / 20).  From 256 workgroups on only where sequences are uneven and long: of one length
-    // the join's launch is lost (4 caches of 4096 20.5 / 20.1, 32 of 4096 108 / 104, 32 of 1024 30 / 28).
-    if (a->B <= kShared && seen >= 2 * least && (wgs < 256 || seen >= 512)) {
+    // the join's launch is lost (4 caches of 4096 20.5 / 20.1, 32 of 4096 108 / 104, 32 of 1024 30 / 28, 256 of 512 129 / 115;
+    // 16 of 750 on average, 16 heads of 64, 20.5 / 31.9).
+    if (a->B <= kShared && seen >= 2 * least && (wgs < 256 || seen >= 640)) {
       share = 256 * (wgs / 256 + 1) / a->Hkv;
       whole = wgs >= 256;
       // (many key heads of few rows each: the join's buffer, of 32 rows a slice, would exceed 256 MiB)
       if (whole && (share + tiles) * a->Hkv * 32 * (r.dp + 2) > 64 << 20) share = 0;
     }
   }
-  slices = slices < 1 || share > 0 || a->B > kScanned ? 1 : slices > 64 ? 64 : slices;
   r.counted = a->B > kScanned && share == 0;
   // rows of a tile join in blocks of 32, or -- packed_stream_kernel -- one by one, as many blocks as a
   // sequence has rows on average, but few where there are many tiles, most of which need no join
@@ -1197,7 +1193,7 @@ int route(const sf_packed_attention_args* a, Route& r) {
 
 size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
   const size_t starts = r.counted ? ((size_t)a->B + 1) * sizeof(int) : 0;
-  if (!r.joined()) return starts;                       // (so many sequences fill the GPU)
+  if (!r.joined()) return starts;
   const int R = r.nw ? 32 * r.nw : 32;
   return (size_t)r.wgs * R * (r.dp + 2) * sizeof(float) + (size_t)r.pl.tiles * 2 * sizeof(int4);
 }
