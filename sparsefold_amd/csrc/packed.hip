@@ -33,7 +33,6 @@ typedef __attribute__((address_space(3))) v4i16p lds_v4i16p;
 struct Bf16 {
   // a tile whose weights sum to more moves the reference point (2^60: weights far below bf16's largest)
   static constexpr float kMassLimit = 1.152921504606846976e18f;
-  static constexpr float kHuge = 0x1p28f;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -45,7 +44,6 @@ struct Bf16 {
 struct Fp16 {
   // 2^12: every weight stays finite in fp16
   static constexpr float kMassLimit = 4096.f;
-  static constexpr float kHuge = 0x1p24f;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -60,22 +58,44 @@ struct Fp16 {
   static __device__ __forceinline__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
 
-// A reference point m of a row's products s = q.k: weights are 2^(c s - mc) with c = scale log2 e, one
-// fma and one exp2.  The rounding of mc scales all weights of the row alike; products so large
-// that it could overflow them (E::kHuge and up, in log2 units) take the power of two below |c|
-// instead, with which c m is exact: neighbouring fp32 products of that size weigh everything or
-// nothing against each other in either scale.
-template <class E>
-struct Ref {
-  float c, mc;
-  Ref() = default;
-  __device__ __forceinline__ Ref(float m, float c0) : c(fabsf(m * c0) < E::kHuge ? c0 : __uint_as_float(__float_as_uint(c0) & 0xff800000u)), mc(fminf(fmaxf(m * c, -FLT_MAX), FLT_MAX)) {}            // (finite: a logit of -inf weighs nothing)
-};
-// What sums against m are worth against mnew (the larger logit of the two).
-template <class E>
-__device__ __forceinline__ float rescale(float m, float mnew, float c0) {
-  const Ref<E> a(m, c0), b(mnew, c0);
-  return a.c == b.c ? fast_exp2(a.mc - b.mc) : 0.f;
+// A reference point m of a row's products s = q.k: weights are 2^(c (s - m)) with c = |scale| log2 e, one fma and one
+// exp2 as 2^(c s - mc), mc = c m.  The rounding of mc scales all weights of the row alike, by up to 2^(1/2) while
+// |c m| < 2^24.  Beyond it could be any factor: there mc is NaN, which accepts no tile as it stands, and
+// settle() forms the weights from s - m, whose rounding is relative to what it is.  (m = -FLT_MAX: no key yet.)
+constexpr float kFar = 0x1p24f;
+__device__ __forceinline__ float times(float m, float c) {
+  float x = m * c;
+  asm("" : "+v"(x));                                         // (rounded here, not within a later fma)
+  return x;
+}
+__device__ __forceinline__ float reference(float m, float c) {
+  const float x = times(m, c);
+  return fabsf(x) < kFar ? x : __builtin_nanf("");
+}
+// What sums against each of m are worth against mnew, no smaller than any of them.  A difference of the rounded c m
+// where none is far, or one lies so far below that it is worth nothing (no key yet).  ALWAYS: without the branch that
+// skips the rest, in loops whose loads it would hold up.
+template <bool ALWAYS = false, int N>
+__device__ __forceinline__ void rescale(const float (&m)[N], float mnew, float c, float (&w)[N]) {
+  const float b = times(mnew, c);
+  float far = fabsf(b);
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const float a = times(m[x], c);
+    far = fmaxf(far, a > -2.f * kFar ? fabsf(a) : 0.f);
+    w[x] = a - b;
+  }
+  if (ALWAYS || __any(!(far < kFar))) {
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const float a = times(m[x], c);
+      const float from_far = fabsf(b) < kFar ? __builtin_fmaf(m[x], c, -b) : (m[x] - mnew) * c;
+      const float from_near = fabsf(b) < kFar ? w[x] : -__builtin_fmaf(mnew, c, -a);
+      w[x] = fabsf(a) < kFar ? from_near : from_far;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < N; ++x) w[x] = fast_exp2(w[x]);
 }
 
 struct PackedPlan {
@@ -437,10 +457,8 @@ __device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, con
     float mx = fmaxf(t, m);
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const float w = rescale<E>(m, mx, fabsf(c0));
-    const Ref<E> ref(mx, fabsf(c0));
+    const float w = fast_exp2((m - mx) * fabsf(c0)), p = fast_exp2((t - mx) * fabsf(c0));
     m = mx;
-    const float p = fast_exp2(__builtin_fmaf(t, ref.c, -ref.mc));
     l = l * w + wave_sum(p);
     o[0] *= w;
     o[1] *= w;
@@ -464,8 +482,7 @@ struct RowState {
   using T = Dims<KC>;
   u32x4 q[KC];                                               // Q operand: dims 16 kk + 8 half .. +7
   f32x16 o[T::DB];
-  float m, l, c0;
-  Ref<E> ref;                                                // of m
+  float m, l, c0, mc;                                        // mc: reference(m, c0)
 
   __device__ __forceinline__ void init(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
     const int half = (threadIdx.x >> 5) & 1;
@@ -488,7 +505,8 @@ struct RowState {
     m = -FLT_MAX;
     l = 0.f;
     c0 = fabsf(pl.c0);
-    ref = Ref<E>(m, c0);
+    asm("" : "+v"(c0));                                      // (an fma that takes it from a scalar register issues more slowly)
+    mc = reference(m, c0);
   }
 
   // S^T = K Q^T of a tile of 32 NB keys in LDS: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4.
@@ -528,20 +546,20 @@ struct RowState {
   }
 
   // Weights against a reference point that stays where an earlier tile put it, until a tile's weights
-  // sum to more than the limit (as those of the first do): no running maximum, exp or rescale of O in
-  // the others.  Pair x of the tile's weights: rounded to 16 bits for the matrix product; the sum
-  // takes the rounded weights, so that they still average to one.
+  // sum to more than the limit (or to NaN: the first tile's, and far from zero): no running maximum, exp or
+  // rescale of O in the others.  Pair x of the tile's weights, `less` from their exponents: rounded to 16
+  // bits for the matrix product; the sum takes the rounded weights, so that they still average to one.
   template <int NB>
-  __device__ __forceinline__ void weight_pair(const f32x16 (&s)[NB], int x, uint32_t (&p)[8 * NB], float (&sum)[2]) const {
-    const float w0 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7)], ref.c, -ref.mc));
-    const float w1 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7) + 1], ref.c, -ref.mc));
+  __device__ __forceinline__ void weight_pair(const f32x16 (&s)[NB], int x, uint32_t (&p)[8 * NB], float (&sum)[2], float less) const {
+    const float w0 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7)], c0, -less));
+    const float w1 = fast_exp2(__builtin_fmaf(s[x >> 3][2 * (x & 7) + 1], c0, -less));
     p[x] = E::pack(w0, w1);
     sum[x & 1] = E::sum2(p[x], sum[x & 1]);
   }
 
   // The tile's sum of weights accepted, or the reference point moved and the weights formed again.
   template <int NB>
-  __device__ __forceinline__ void settle(const f32x16 (&s)[NB], uint32_t (&p)[8 * NB], float (&sum)[2]) {
+  __device__ __forceinline__ void settle(f32x16 (&s)[NB], uint32_t (&p)[8 * NB], float (&sum)[2]) {
     if (__any(!(sum[0] + sum[1] <= E::kMassLimit))) {
       float mx = s[0][0];
 #pragma unroll
@@ -549,17 +567,26 @@ struct RowState {
 #pragma unroll
         for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[kb][x]);
       mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-      const float w = rescale<E>(m, mx, c0);
+      float w[1];
+      rescale({m}, mx, c0, w);
       m = mx;
-      l *= w;
+      mc = reference(m, c0);
+      l *= w[0];
 #pragma unroll
       for (int db = 0; db < T::DB; ++db)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[db][x] *= w;
-      ref = Ref<E>(m, c0);
+        for (int x = 0; x < 16; ++x) o[db][x] *= w[0];
+      const bool far = mc != mc;
+      if (__any(far)) {
+        const float from = far ? m : 0.f;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s[kb][x] -= from;
+      }
       sum[0] = sum[1] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum);
+      for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum, far ? 0.f : mc);
     }
     l += sum[0] + sum[1];
   }
@@ -599,10 +626,10 @@ struct RowState {
 
   // A tile's weights in one go.
   template <int NB>
-  __device__ __forceinline__ void weights(const f32x16 (&s)[NB], uint32_t (&p)[8 * NB]) {
+  __device__ __forceinline__ void weights(f32x16 (&s)[NB], uint32_t (&p)[8 * NB]) {
     float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum);
+    for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum, mc);
     settle<NB>(s, p, sum);
   }
 
@@ -774,14 +801,16 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
       lds_only_barrier();
       if (group == 0) {
         const f32x4 ml = so[64 * 4 * T::DB];
-        const float m = fmaxf(st.m, ml[0]), w0 = rescale<E>(st.m, m, st.c0), w1 = rescale<E>(ml[0], m, st.c0);
+        const float m = fmaxf(st.m, ml[0]);
+        float w[2];
+        rescale({st.m, ml[0]}, m, st.c0, w);
         st.m = m;
-        st.l = st.l * w0 + ml[1] * w1;
+        st.l = st.l * w[0] + ml[1] * w[1];
 #pragma unroll
         for (int x = 0; x < 4 * T::DB; ++x) {
           const f32x4 o = so[64 * x];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) st.o[x / 4][4 * (x % 4) + e] = st.o[x / 4][4 * (x % 4) + e] * w0 + o[e] * w1;
+          for (int e = 0; e < 4; ++e) st.o[x / 4][4 * (x % 4) + e] = st.o[x / 4][4 * (x % 4) + e] * w[0] + o[e] * w[1];
         }
       }
     }
@@ -933,11 +962,9 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 #pragma unroll
   for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][jr][0]);
   float l = 0.f, wt[4];
+  rescale({ml[0][jr][0], ml[1][jr][0], ml[2][jr][0], ml[3][jr][0]}, m, fabsf(pl.c0), wt);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    wt[w] = rescale<E>(ml[w][jr][0], m, fabsf(pl.c0));
-    l += wt[w] * ml[w][jr][1];
-  }
+  for (int w = 0; w < 4; ++w) l += wt[w] * ml[w][jr][1];
   f32x4 o[T::DB];
   float probe = 0.f;
 #pragma unroll
@@ -1031,15 +1058,15 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
           float mx = m;
 #pragma unroll
           for (int y = 0; y < 4; ++y) mx = fmaxf(mx, v[y][0]);
-          const float w0 = rescale<E>(m, mx, c0);
+          float w[5];
+          rescale<true>({v[0][0], v[1][0], v[2][0], v[3][0], m}, mx, c0, w);
           m = mx;
-          l *= w0;
-          acc *= w0;
+          l *= w[4];
+          acc *= w[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const float w = rescale<E>(v[y][0], mx, c0);
-            l += w * v[y][1];
-            acc += w * ov[y];
+            l += w[y] * v[y][1];
+            acc += w[y] * ov[y];
           }
         }
       }
@@ -1047,16 +1074,20 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
         so[group][tid % LR] = acc;
         if (d == 0) sml[group] = f32x2{m, l};
         __syncthreads();
+        float mg[GROUPS], w[GROUPS];
         m = -FLT_MAX;
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, sml[g][0]);
+        for (int g = 0; g < GROUPS; ++g) {
+          mg[g] = sml[g][0];
+          m = fmaxf(m, mg[g]);
+        }
+        rescale(mg, m, c0, w);
         l = 0.f;
         acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-          const float w = rescale<E>(sml[g][0], m, c0);
-          l += w * sml[g][1];
-          acc += w * so[g][tid % LR];
+          l += w[g] * sml[g][1];
+          acc += w[g] * so[g][tid % LR];
         }
         __syncthreads();                                     // (the shares may be overwritten)
       }

@@ -1,0 +1,58 @@
+"""Packed attention at the ends of the number range, by every kernel route: logits far from zero whose
+differences are exact.
+
+Logits: products that fp32 holds exactly leave the difference from the row's largest as it is, so a weight is off by
+the rounding of difference times scale (differences up to 100 in log2 units: 3 products and sums, 100 * 3 * 2^-24 < 2^-15)
+and of exp2 (2^-22): d = 2^-15 in the tolerance 2 (u + d + n 2^-24) A + u |o|, with u = finfo.eps / 2 of the element type and
+A = sum p |v|.
+"""
+import math
+
+import pytest
+import torch
+
+from sparsefold_amd.backends.hip import ops
+from tests.test_gpu_packed_attention import DEV, TYPES, offsets
+
+pytestmark = pytest.mark.gpu
+
+# (queries, keys, heads): shared key slices, stream, tiles of one and two groups of waves, sliced tiles
+ROUTES = [(1, 9000, (8, 2)), (9, 300, (8, 2)), (200, 200, (8, 2)), (333, 5000, (8, 2)), (1300, 1300, (32, 32))]
+
+# first two: the second lies at 2^24 log2 units; (digits of q, digits of k, step, scale)
+FAR = [((256, 256, 1), (177 * 256, 114, 24), 1, 1.0), ((4096,), (4096,), 2, 1.0), ((4096,), (4096,), 2, -1.0),
+       ((16384,), (12288,), 16, 1.0), ((256, 256, 1), (20 * 256, 7, 3), 1, 1.0)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("route", ROUTES, ids=lambda r: f"{r[0]}x{r[1]}")
+@pytest.mark.parametrize("far", FAR, ids=lambda f: f"{sum(a * b for a, b in zip(f[0], f[1]))}by{f[2] * f[3]:g}")
+def test_logits_far_from_zero(far, route, causal, dtype):
+  """Keys a few exact steps apart: every other query row; the rows between have small logits."""
+  (n, m, (H, Hk)), (qd, kd, step, scale) = route, far
+  D, g = 32, torch.Generator().manual_seed(n)
+  dt = TYPES[dtype]
+  x = torch.randint(-3, 0, (m,), generator=g).float()
+  x[37] = 0.0                                        # one key above all others
+  sign = 1.0 if scale > 0 else -1.0
+  q, k = torch.zeros(n, H, D), torch.zeros(m, Hk, D)
+  for i, (a, b) in enumerate(zip(qd, kd)):
+    q[::2, :, i], k[:, :, i] = a, sign * b
+  q[::2, :, 8] = 1.0
+  k[:, :, 8] = (sign * step * x)[:, None]
+  q[1::2, :, 16:] = torch.randn(len(range(1, n, 2)), H, 16, generator=g) / 2
+  k[:, :, 16:] = torch.randn(m, Hk, 16, generator=g) / 2
+  q, k = q.to(dt).double(), k.to(dt).double()
+  v = torch.randn(m, Hk, D, generator=g).to(dt)
+  out = ops.packed_attention(q.to(dt).to(DEV), k.to(dt).to(DEV), v.to(DEV), offsets([n]), offsets([m]), causal=causal, scale=scale).cpu().double()
+  u, vd = torch.finfo(dt).eps / 2, v.double()
+  for h in range(0, H, max(H // 4, 1)):
+    s = scale * q[:, h] @ k[:, h // (H // Hk)].T
+    if causal:
+      s = s.masked_fill(torch.arange(m)[None] > torch.arange(n)[:, None] + (m - n), -math.inf)
+    p = torch.softmax(s, -1)
+    want, a = p @ vd[:, h // (H // Hk)], p @ vd[:, h // (H // Hk)].abs()
+    tol = 2 * (u + 2.0 ** -15 + m * 2.0 ** -24) * a + u * want.abs() + (m * 2.0 ** -25 * vd.abs().amax() if dtype == "fp16" else 0.0)
+    worst = ((out[:, h] - want).abs() / tol).amax(-1)
+    assert worst.max() <= 1.0, f"head {h}: rows {torch.nonzero(worst > 1).flatten().tolist()[:5]} at {worst.max().item():.2f} of the tolerance"
