@@ -29,10 +29,15 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef short v4i16p __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16p lds_v4i16p;
 
+// A lane's weights of a tile that sum to more than 2^kMass against the row's reference point move it.
+constexpr int kMass = 12;
+
 // 16-bit element types: the matrix product, rounding of two weights to one word, their sum.
 struct Bf16 {
-  // a tile whose weights sum to more moves the reference point (2^60: weights far below bf16's largest)
-  static constexpr float kMassLimit = 1.152921504606846976e18f;
+  // All weights of a row are 2^-shift of what the reference point makes them, so that those of n keys together, each of at most
+  // n / 32 + 1 tiles in two lanes up to 2^kMass, sum to 1/2 at most: values up to the largest bf16 do not pass
+  // fp32 in any partial sum.  (Values below 2^-126 + shift may lose digits instead.)
+  static __device__ __forceinline__ float shift(int n) { return (float)(kMass - 3 + max(32 - __clz(n), 5)); }
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -42,8 +47,7 @@ struct Bf16 {
   static __device__ __forceinline__ uint16_t from_float(float v) { return f2bf(v); }
 };
 struct Fp16 {
-  // 2^12: every weight stays finite in fp16
-  static constexpr float kMassLimit = 4096.f;
+  static __device__ __forceinline__ float shift(int) { return 0.f; }          // (values are small, and so is fp16's range of weights)
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -58,9 +62,9 @@ struct Fp16 {
   static __device__ __forceinline__ uint16_t from_float(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
 
-// A reference point m of a row's products s = q.k: weights are 2^(c (s - m)) with c = |scale| log2 e, one fma and one
-// exp2 as 2^(c s - mc), mc = c m.  The rounding of mc scales all weights of the row alike, by up to 2^(1/2) while
-// |c m| < 2^24.  Beyond it could be any factor: there mc is NaN, which accepts no tile as it stands, and
+// A reference point m of a row's products s = q.k: weights are 2^(c (s - m) - shift) with c = |scale| log2 e, one fma and
+// one exp2 as 2^(c s - mc), mc = c m + shift.  The rounding of mc scales all weights of the row alike, by up to 2^(1/2)
+// while |mc| < 2^24.  Beyond it could be any factor: there mc is NaN, which accepts no tile as it stands, and
 // settle() forms the weights from s - m, whose rounding is relative to what it is.  (m = -FLT_MAX: no key yet.)
 constexpr float kFar = 0x1p24f;
 __device__ __forceinline__ float times(float m, float c) {
@@ -68,29 +72,28 @@ __device__ __forceinline__ float times(float m, float c) {
   asm("" : "+v"(x));                                         // (rounded here, not within a later fma)
   return x;
 }
-__device__ __forceinline__ float reference(float m, float c) {
-  const float x = times(m, c);
+__device__ __forceinline__ float reference(float m, float c, float shift) {
+  const float x = times(m, c) + shift;
   return fabsf(x) < kFar ? x : __builtin_nanf("");
 }
 // What sums against each of m are worth against mnew, no smaller than any of them.  A difference of the rounded c m
-// where none is far, or one lies so far below that it is worth nothing (no key yet).  ALWAYS: without the branch that
-// skips the rest, in loops whose loads it would hold up.
-template <bool ALWAYS = false, int N>
-__device__ __forceinline__ void rescale(const float (&m)[N], float mnew, float c, float (&w)[N]) {
-  const float b = times(mnew, c);
+// where none is far, or one lies so far below that it is worth nothing (no key yet).
+template <int N>
+__device__ __forceinline__ void rescale(const float (&m)[N], float mnew, float c, float shift, float (&w)[N]) {
+  const float b = times(mnew, c) + shift;
   float far = fabsf(b);
 #pragma unroll
   for (int x = 0; x < N; ++x) {
-    const float a = times(m[x], c);
+    const float a = times(m[x], c) + shift;
     far = fmaxf(far, a > -2.f * kFar ? fabsf(a) : 0.f);
     w[x] = a - b;
   }
-  if (ALWAYS || __any(!(far < kFar))) {
+  if (__any(!(far < kFar))) {
 #pragma unroll
     for (int x = 0; x < N; ++x) {
-      const float a = times(m[x], c);
-      const float from_far = fabsf(b) < kFar ? __builtin_fmaf(m[x], c, -b) : (m[x] - mnew) * c;
-      const float from_near = fabsf(b) < kFar ? w[x] : -__builtin_fmaf(mnew, c, -a);
+      const float a = times(m[x], c) + shift;
+      const float from_far = fabsf(b) < kFar ? __builtin_fmaf(m[x], c, -b) + shift : (m[x] - mnew) * c;
+      const float from_near = fabsf(b) < kFar ? w[x] : -(__builtin_fmaf(mnew, c, -a) + shift);
       w[x] = fabsf(a) < kFar ? from_near : from_far;
     }
   }
@@ -457,7 +460,7 @@ __device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, con
     float mx = fmaxf(t, m);
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const float w = fast_exp2((m - mx) * fabsf(c0)), p = fast_exp2((t - mx) * fabsf(c0));
+    const float w = fast_exp2((m - mx) * fabsf(c0)), p = fast_exp2(__builtin_fmaf(t - mx, fabsf(c0), -E::shift(s.lk)));
     m = mx;
     l = l * w + wave_sum(p);
     o[0] *= w;
@@ -482,7 +485,7 @@ struct RowState {
   using T = Dims<KC>;
   u32x4 q[KC];                                               // Q operand: dims 16 kk + 8 half .. +7
   f32x16 o[T::DB];
-  float m, l, c0, mc;                                        // mc: reference(m, c0)
+  float m, l, c0, mc, shift, limit;                          // mc: reference(m, c0, shift); limit: 2^(kMass - shift)
 
   __device__ __forceinline__ void init(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
     const int half = (threadIdx.x >> 5) & 1;
@@ -506,7 +509,9 @@ struct RowState {
     l = 0.f;
     c0 = fabsf(pl.c0);
     asm("" : "+v"(c0));                                      // (an fma that takes it from a scalar register issues more slowly)
-    mc = reference(m, c0);
+    shift = E::shift(s.lk);
+    limit = __uint_as_float((uint32_t)(127 + kMass - (int)shift) << 23);
+    mc = reference(m, c0, shift);
   }
 
   // S^T = K Q^T of a tile of 32 NB keys in LDS: lane (row li) gets keys 32 kb + 8 (r / 4) + 4 half + r % 4.
@@ -560,7 +565,7 @@ struct RowState {
   // The tile's sum of weights accepted, or the reference point moved and the weights formed again.
   template <int NB>
   __device__ __forceinline__ void settle(f32x16 (&s)[NB], uint32_t (&p)[8 * NB], float (&sum)[2]) {
-    if (__any(!(sum[0] + sum[1] <= E::kMassLimit))) {
+    if (__any(!(sum[0] + sum[1] <= limit))) {
       float mx = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
@@ -568,9 +573,9 @@ struct RowState {
         for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[kb][x]);
       mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
       float w[1];
-      rescale({m}, mx, c0, w);
+      rescale({m}, mx, c0, shift, w);
       m = mx;
-      mc = reference(m, c0);
+      mc = reference(m, c0, shift);
       l *= w[0];
 #pragma unroll
       for (int db = 0; db < T::DB; ++db)
@@ -586,7 +591,7 @@ struct RowState {
       }
       sum[0] = sum[1] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum, far ? 0.f : mc);
+      for (int x = 0; x < 8 * NB; ++x) weight_pair<NB>(s, x, p, sum, far ? shift : mc);
     }
     l += sum[0] + sum[1];
   }
@@ -803,7 +808,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
         const f32x4 ml = so[64 * 4 * T::DB];
         const float m = fmaxf(st.m, ml[0]);
         float w[2];
-        rescale({st.m, ml[0]}, m, st.c0, w);
+        rescale({st.m, ml[0]}, m, st.c0, st.shift, w);
         st.m = m;
         st.l = st.l * w[0] + ml[1] * w[1];
 #pragma unroll
@@ -962,7 +967,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 #pragma unroll
   for (int w = 1; w < 4; ++w) m = fmaxf(m, ml[w][jr][0]);
   float l = 0.f, wt[4];
-  rescale({ml[0][jr][0], ml[1][jr][0], ml[2][jr][0], ml[3][jr][0]}, m, fabsf(pl.c0), wt);
+  rescale({ml[0][jr][0], ml[1][jr][0], ml[2][jr][0], ml[3][jr][0]}, m, fabsf(pl.c0), E::shift(s.lk), wt);
 #pragma unroll
   for (int w = 0; w < 4; ++w) l += wt[w] * ml[w][jr][1];
   f32x4 o[T::DB];
@@ -1019,7 +1024,7 @@ template <class E, int DP, int R>
 __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   constexpr int LR = DP <= 32 ? 8 : DP <= 64 ? 16 : 32, GROUPS = 256 / LR;
   constexpr bool kOneRow = R == 32;
-  constexpr int ROWS = kOneRow ? 1 : 32, PASSES = kOneRow ? 1 : ROWS / GROUPS;
+  constexpr int ROWS = kOneRow ? 1 : 32, PASSES = kOneRow ? 1 : ROWS / GROUPS, kBatch = 4;
   const int64_t kStep = (int64_t)a.Hkv * R * (DP + 2);      // from slice to slice
   __shared__ f32x4 so[kOneRow ? GROUPS : 1][LR];
   __shared__ f32x2 sml[GROUPS];
@@ -1030,7 +1035,7 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
   const int slices = f1.z;
   const int rows = s.lq * pl.G, r0 = f0.w * R;
   const float* part = pl.part + ((int64_t)f1.y * a.Hkv + hk) * R * (DP + 2);
-  const float c0 = fabsf(pl.c0);
+  const float c0 = fabsf(pl.c0), shift = E::shift(s.lk);
   for (int in0 = piece * ROWS; in0 < R && r0 + in0 < rows; in0 += pl.pieces * ROWS) {      // (uniform over the block)
     f32x4 o[PASSES];
     float sum[PASSES];
@@ -1043,28 +1048,35 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
       float m = -FLT_MAX, l = 0.f;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       if (r0 + in < rows && d < DP) {
-        for (int z = z0; z < slices; z += 4 * dz) {
-          f32x2 v[4];
-          f32x4 ov[4];
+        for (int z = z0; z < slices; z += kBatch * dz) {
+          f32x2 v[kBatch];
+          f32x4 ov[kBatch];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const bool in_range = z + y * dz < slices;
-            const int64_t at = (in_range ? z + y * dz : z) * kStep;
+          for (int y = 0; y < kBatch; ++y) {
+            const int64_t at = (z + y * dz < slices ? z + y * dz : z) * kStep;
             v[y] = *reinterpret_cast<const f32x2*>(ml + at);
             ov[y] = *reinterpret_cast<const f32x4*>(po + at);
-            if (!in_range) v[y] = f32x2{-FLT_MAX, 0.f};
-            if (!in_range) ov[y] = f32x4{0.f, 0.f, 0.f, 0.f};   // (whatever it weighs: it may not be finite)
           }
-          float mx = m;
+          // (no use before the last of the loads: left to itself the compiler waited for each in turn, 7.9 us for 4.9)
 #pragma unroll
-          for (int y = 0; y < 4; ++y) mx = fmaxf(mx, v[y][0]);
-          float w[5];
-          rescale<true>({v[0][0], v[1][0], v[2][0], v[3][0], m}, mx, c0, w);
+          for (int y = 0; y < kBatch; ++y) asm volatile("" : "+v"(v[y]), "+v"(ov[y]) : : "memory");
+          float mz[kBatch + 1], w[kBatch + 1], mx = m;
+#pragma unroll
+          for (int y = 0; y < kBatch; ++y) {
+            if (z + y * dz >= slices) {
+              v[y] = f32x2{-FLT_MAX, 0.f};
+              ov[y] = f32x4{0.f, 0.f, 0.f, 0.f};             // (whatever it weighs: it may not be finite)
+            }
+            mz[y] = v[y][0];
+            mx = fmaxf(mx, v[y][0]);
+          }
+          mz[kBatch] = m;
+          rescale(mz, mx, c0, shift, w);
           m = mx;
-          l *= w[4];
-          acc *= w[4];
+          l *= w[kBatch];
+          acc *= w[kBatch];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
+          for (int y = 0; y < kBatch; ++y) {
             l += w[y] * v[y][1];
             acc += w[y] * ov[y];
           }
@@ -1081,7 +1093,7 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
           mg[g] = sml[g][0];
           m = fmaxf(m, mg[g]);
         }
-        rescale(mg, m, c0, w);
+        rescale(mg, m, c0, shift, w);
         l = 0.f;
         acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -1,5 +1,5 @@
 """Packed attention at the ends of the number range, by every kernel route: logits far from zero whose
-differences are exact.
+differences are exact, values near the largest.
 
 Logits: products that fp32 holds exactly leave the difference from the row's largest as it is, so a weight is off by
 the rounding of difference times scale (differences up to 100 in log2 units: 3 products and sums, 100 * 3 * 2^-24 < 2^-15)
@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from sparsefold_amd.backends.hip import ops
-from tests.test_gpu_packed_attention import DEV, TYPES, offsets
+from tests.test_gpu_packed_attention import DEV, TYPES, check, make, offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,35 @@ def test_logits_far_from_zero(far, route, causal, dtype):
     tol = 2 * (u + 2.0 ** -15 + m * 2.0 ** -24) * a + u * want.abs() + (m * 2.0 ** -25 * vd.abs().amax() if dtype == "fp16" else 0.0)
     worst = ((out[:, h] - want).abs() / tol).amax(-1)
     assert worst.max() <= 1.0, f"head {h}: rows {torch.nonzero(worst > 1).flatten().tolist()[:5]} at {worst.max().item():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("kind", ["rising", "largest", "signs", "steep"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("route", ROUTES, ids=lambda r: f"{r[0]}x{r[1]}")
+def test_values_near_the_largest(route, D, causal, kind):
+  """bf16 values whose sum, or whose product with a weight above 1, passes fp32: the mean does not."""
+  n, m, (H, Hk) = route
+  q, k, v = make([n], [m], H, Hk, D, torch.bfloat16, 11)
+  if kind == "rising":                               # logits 34.7 nats above those of the later keys
+    q, k, v = torch.zeros_like(q), torch.zeros_like(k), torch.full_like(v, 2.0 ** 80)
+    q[..., 0] = 1.0
+    k[:m // 2, :, 0] = 34.75 * math.sqrt(D)
+  elif kind == "steep":                              # rising all along, by a nat every 8 keys, over 40 nats
+    q[..., 0] = math.sqrt(D)
+    k[..., 0] = (40.0 - torch.arange(m, device=DEV) / 8).clamp(min=0).to(k.dtype)[:, None]
+    v = v * 2.0 ** 110
+  elif kind == "largest":
+    q, v = torch.zeros_like(q), torch.full_like(v, torch.finfo(torch.bfloat16).max)
+  else:
+    v = v.sign() * 2.0 ** 126
+  check(ops.packed_attention(q, k, v, offsets([n]), offsets([m]), causal=causal), q, k, v, [n], [m], causal)
+
+
+@pytest.mark.parametrize("route", ROUTES, ids=lambda r: f"{r[0]}x{r[1]}")
+def test_small_values_keep_their_digits(route):
+  n, m, (H, Hk) = route
+  q, k, v = make([n], [m], H, Hk, 64, torch.bfloat16, 12)
+  v = v * 2.0 ** -60
+  out = ops.packed_attention(q, k, v, offsets([n]), offsets([m]))
+  check(out * 2.0 ** 60, q, k, v * 2.0 ** 60, [n], [m])
