@@ -29,11 +29,10 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef short v4i16p __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16p lds_v4i16p;
 
-// A lane's weights of a tile that sum to more than 2^kMass against the row's reference point move it.
-constexpr int kMass = 12;
-
 // 16-bit element types: the matrix product, rounding of two weights to one word, their sum.
 struct Bf16 {
+  // A lane's weights of a tile that sum to more than 2^kMass against the row's reference point move it.
+  static constexpr int kMass = 12;
   // All weights of a row are 2^-shift of what the reference point makes them, so that those of n keys together, each of at most
   // n / 32 + 1 tiles in two lanes up to 2^kMass, sum to 1/2 at most: values up to the largest bf16 do not pass
   // fp32 in any partial sum.  (Values below 2^-126 + shift may lose digits instead.)
@@ -47,7 +46,10 @@ struct Bf16 {
   static __device__ __forceinline__ uint16_t from_float(float v) { return f2bf(v); }
 };
 struct Fp16 {
-  static __device__ __forceinline__ float shift(int) { return 0.f; }          // (values are small, and so is fp16's range of weights)
+  // Weights of 2^6 at the reference point, and of 2^15 where a lane's move it: finite, and rounded to a multiple of 2^-24,
+  // so that only those below 2^-31 of the reference point's vanish.  (Values are too small to pass fp32.)
+  static constexpr int kMass = 9;
+  static __device__ __forceinline__ float shift(int) { return -6.f; }
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -485,7 +487,7 @@ struct RowState {
   using T = Dims<KC>;
   u32x4 q[KC];                                               // Q operand: dims 16 kk + 8 half .. +7
   f32x16 o[T::DB];
-  float m, l, c0, mc, shift, limit;                          // mc: reference(m, c0, shift); limit: 2^(kMass - shift)
+  float m, l, c0, mc, shift, limit;                          // mc: reference(m, c0, shift); limit: 2^(E::kMass - shift)
 
   __device__ __forceinline__ void init(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
     const int half = (threadIdx.x >> 5) & 1;
@@ -510,7 +512,7 @@ struct RowState {
     c0 = fabsf(pl.c0);
     asm("" : "+v"(c0));                                      // (an fma that takes it from a scalar register issues more slowly)
     shift = E::shift(s.lk);
-    limit = __uint_as_float((uint32_t)(127 + kMass - (int)shift) << 23);
+    limit = __uint_as_float((uint32_t)(127 + E::kMass - (int)shift) << 23);
     mc = reference(m, c0, shift);
   }
 

@@ -1,5 +1,5 @@
 """Packed attention at the ends of the number range, by every kernel route: logits far from zero whose
-differences are exact, values near the largest.
+differences are exact, values near the largest, weights far below the row's largest.
 
 Logits: products that fp32 holds exactly leave the difference from the row's largest as it is, so a weight is off by
 the rounding of difference times scale (differences up to 100 in log2 units: 3 products and sums, 100 * 3 * 2^-24 < 2^-15)
@@ -88,3 +88,17 @@ def test_small_values_keep_their_digits(route):
   v = v * 2.0 ** -60
   out = ops.packed_attention(q, k, v, offsets([n]), offsets([m]))
   check(out * 2.0 ** 60, q, k, v * 2.0 ** 60, [n], [m])
+
+
+@pytest.mark.parametrize("nats", [17.375, 19.0])
+def test_fp16_weights_far_below_the_largest(nats):
+  """One key above 30000 others whose weights are 2^-25.07 or 2^-27.4 of its: a weight is off by 2^-25 where the largest is
+  2^6 2^-1/2 at least, so n 2^-30 max |v|, and by 2 u of itself where it is normal."""
+  n, m, H, D = 1300, 30000, 32, 32                   # (enough workgroups that all keys share a reference point)
+  q, k = torch.zeros(n, H, D, dtype=torch.float16, device=DEV), torch.zeros(m, H, D, dtype=torch.float16, device=DEV)
+  v = (1 + torch.rand(m, H, D, generator=torch.Generator().manual_seed(1)) / 4).half().to(DEV)
+  q[..., 0], k[-1, :, 0], v[-1] = 1.0, nats, 0.0
+  out = ops.packed_attention(q, k, v, offsets([n]), offsets([m]), scale=1.0).double()
+  p = math.exp(-nats) / (1 + (m - 1) * math.exp(-nats))
+  want = p * v.double().sum(0)
+  assert ((out - want).abs() <= m * 2.0 ** -30 * 1.25 + 3 * 2.0 ** -11 * want).all()
