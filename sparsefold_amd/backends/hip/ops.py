@@ -12,6 +12,7 @@ import itertools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from sparsefold_amd import _lib
 
@@ -595,11 +596,16 @@ _NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 
 
 def _no_grad(what: str, *ts) -> None:
-  """These calls have no backward pass: a tensor that expects a gradient through them is refused."""
+  """These calls have no backward pass and no tangents: a tensor that expects a gradient or carries a tangent through them
+  is refused."""
   if torch.is_grad_enabled():
     for t in ts:
       if t is not None and t.requires_grad:
         raise ValueError(f"{what}: has no backward pass; detach the inputs or call it under torch.no_grad()")
+  if forward_ad._current_level >= 0:                           # (inside a dual level)
+    for t in ts:
+      if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what}: has no forward-mode derivative; pass the primals of dual tensors")
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
