@@ -103,6 +103,10 @@ __device__ __forceinline__ void rescale(const float (&m)[N], float mnew, float c
   for (int x = 0; x < N; ++x) w[x] = fast_exp2(w[x]);
 }
 
+// A launch dimension holds less than 2^32 threads: workgroups past kGridX (of up to 512) continue in the next row of the grid.
+constexpr int kGridX = 1 << 22;
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.y * kGridX + blockIdx.x); }
+
 struct PackedPlan {
   int tiles;         // bound on the row tiles of one key head
   int slices;        // packed_tile_kernel: key slices (workgroups) of every row tile
@@ -719,7 +723,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW));
   uint8_t* const smem = shared + group * 4 * kTile;
   // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
-  const int hk = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+  const int block = workgroup(), hk = block % a.Hkv, rest = block / a.Hkv;
   const int slice = rest % pl.slices, idx = rest / pl.slices;
   Seq s;
   int tile, ntiles;
@@ -825,7 +829,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
   if (r0 >= rows || group > 0) return;                       // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
   if (pl.slices > 1) {
-    float* po = pl.part + (int64_t)blockIdx.x * R * (T::DP + 2);
+    float* po = pl.part + (int64_t)block * R * (T::DP + 2);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
@@ -887,7 +891,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
   __shared__ f32x2 ml[4][32];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hk = blockIdx.x % a.Hkv, item = blockIdx.x / a.Hkv;
+  const int block = workgroup(), hk = block % a.Hkv, item = block / a.Hkv;
   Seq s;
   int tile, slice, slices;
   if (pl.share > 0) {
@@ -987,7 +991,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
     for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[db][e], 0.f, probe);
   }
   if (slices > 1) {
-    float* po = pl.part + (int64_t)blockIdx.x * 32 * (T::DP + 2);
+    float* po = pl.part + (int64_t)block * 32 * (T::DP + 2);
     if (r0 + jr < rows) {
 #pragma unroll
       for (int db = 0; db < T::DB; ++db) *reinterpret_cast<f32x4*>(po + jr * T::DP + 32 * db + jd) = o[db];
@@ -1245,7 +1249,7 @@ size_t part_bytes(const sf_packed_attention_args* a, const Route& r) {
 
 template <class E, int KC>
 int launch(const sf_packed_attention_args* a, const Route& r, hipStream_t st) {
-  const dim3 grid((unsigned)r.wgs);
+  const dim3 grid = r.wgs <= kGridX ? dim3((unsigned)r.wgs) : dim3(kGridX, (unsigned)((r.wgs + kGridX - 1) / kGridX));
   if (r.pl.starts != nullptr) {
     hipLaunchKernelGGL(packed_starts_kernel, dim3(1), dim3(1024), 0, st, *a, r.pl, r.nw ? 32 * r.nw : 32);
     if (sf_check_launch("packed_starts_kernel")) return 1;

@@ -102,3 +102,17 @@ def test_fp16_weights_far_below_the_largest(nats):
   p = math.exp(-nats) / (1 + (m - 1) * math.exp(-nats))
   want = p * v.double().sum(0)
   assert ((out - want).abs() <= m * 2.0 ** -30 * 1.25 + 3 * 2.0 ** -11 * want).all()
+
+
+def test_more_workgroups_than_a_launch_dimension_holds():
+  """2^21 sequences of one token, 8 key heads: 2^24 workgroups of 256 threads and some.  One key each: its value."""
+  B, H, D = (1 << 21) + 5, 8, 8
+  g = torch.Generator(device=DEV).manual_seed(2)
+  q, k, v = (torch.randn(B, H, D, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+  cu = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+  assert torch.equal(ops.packed_attention(q, k, v, cu), v)
+  used = torch.ones(B, dtype=torch.int32, device=DEV)
+  used[::3] = 0
+  out = torch.full_like(q, 7.0)
+  ops.packed_attention(q, k, v, cu, len_q=used, out=out)
+  assert torch.equal(out[used == 1], v[used == 1]) and (out[::3] == 7.0).all()

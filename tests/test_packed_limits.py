@@ -1,8 +1,11 @@
-"""More refusals of the packed-sequence calls: tangents.  Host tensors; nothing here launches a kernel."""
+"""More refusals of the packed-sequence calls: tangents, grids.  Host tensors; nothing here launches a kernel."""
+import ctypes as C
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from sparsefold_amd import _lib
 from sparsefold_amd.backends.hip import ops
 
 BF = torch.bfloat16
@@ -39,3 +42,17 @@ def test_tangents_are_refused(host_tensors, which, no_grad):
         calls[which % 5](q, k)
     with pytest.raises(_Launched):
       calls[which % 5](q, k)
+
+
+def test_c_attention_refuses_more_workgroups_than_a_grid_holds():
+  lib = _lib.load()
+  cu = torch.zeros(2, dtype=torch.int32)
+  a = _lib.PackedAttentionArgs(B=(1 << 26) // 4 + 1, H=8, Hkv=4, D=8, Tq=1 << 28, Tk=1 << 28, scale=1.0, q=4096, k=4096, v=4096, out=4096,
+                               cu_q=cu.data_ptr(), cu_k=cu.data_ptr())
+  for s in (a.q_s, a.k_s, a.v_s, a.o_s):
+    s[0], s[1] = 64, 8
+  assert lib.sf_hip_packed_attention_workspace_bytes(C.byref(a)) == 0
+  assert lib.sf_hip_packed_attention_fwd(C.byref(a), None, 0, None) != 0
+  buf = C.create_string_buffer(1024)
+  lib.sf_hip_last_error(buf, 1024)
+  assert "too large for the grid" in buf.value.decode()
