@@ -22,6 +22,8 @@ namespace {
 
 constexpr int kMaxPairs = 128;                               // head dims up to 256
 constexpr int kWaves = 4;
+// A launch dimension holds less than 2^32 threads: workgroups past kGridX continue in the next row of the grid.
+constexpr int kGridX = 1 << 22;
 
 struct RotBf16 {
   typedef uint16_t raw;
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
   __shared__ f32x2 table[kWaves][kMaxPairs];
   __shared__ __attribute__((aligned(16))) float affine[NORM == 2 ? 4 : NORM == 1 ? 2 : 1][2 * kMaxPairs];   // weights of q, k, biases of q, k
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t task = (int64_t)blockIdx.x * kWaves + wave;
+  const int64_t task = ((int64_t)blockIdx.y * kGridX + blockIdx.x) * kWaves + wave;
   const int64_t token = task / pl.chunks;
   if (NORM != 0) {                                           // read from memory once for all waves
     for (int d = threadIdx.x; d < a.D; d += 64 * kWaves) {
@@ -303,7 +305,7 @@ extern "C" int sf_hip_rotary_fwd(const sf_rotary_args* a, void* stream) {
   pl.pos64 = a->positions_64;
   const int64_t blocks = (a->T * pl.chunks + kWaves - 1) / kWaves;
   if (blocks > INT32_MAX) { sf_set_error("rotary: problem too large for the grid"); return 1; }
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid = blocks <= kGridX ? dim3((unsigned)blocks) : dim3(kGridX, (unsigned)((blocks + kGridX - 1) / kGridX));
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   auto by_width = [&](auto type) {
     using E = decltype(type);
