@@ -13,6 +13,7 @@
 // whichever way the pairs lie, and the loads and stores are 16 bytes wide.  The next heads' loads are on their
 // way while these are worked on.  8192 tokens, 32 + 8 heads of 128 in fp16, half of the dims: 32 us, 5.2 TB/s (a large
 // copy: 5.2); 16384 tokens in bf16 with a norm: 71 us, 4.7 TB/s; up to some hundred tokens 3.4 to 4 us, the launch.
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -196,32 +197,51 @@ __global__ __launch_bounds__(64 * kWaves) void rotary_kernel(const sf_rotary_arg
         }
       if (hb + step < h1) fetch(h + step);
       if (NORM != 0) {
-        auto head_sum = [&](float v) __attribute__((always_inline)) {
-          for (int o = 1; o < pl.lph; o <<= 1) v += __shfl_xor(v, o);
-          return v;
-        };
-        float mean = 0.f;
-        if (NORM == 2) {
-          float t = 0.f;
+        auto each = [&](auto fn) __attribute__((always_inline)) {
 #pragma unroll
           for (int x = 0; x < UPL; ++x)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
-              for (int e = 0; e < V; ++e) t += f[x][p][e];
-          mean = head_sum(t) * inv_d;
+              for (int e = 0; e < V; ++e) fn(f[x][p][e], at[x][p] >= 0);
+        };
+        auto head_sum = [&](float v) __attribute__((always_inline)) {
+          for (int o = 1; o < pl.lph; o <<= 1) v += __shfl_xor(v, o);
+          return v;
+        };
+        // the mean of squares of f, from which a layer norm's mean is taken first
+        auto mean_square = [&]() __attribute__((always_inline)) {
+          float t = 0.f;
+          if (NORM == 2) {
+            each([&](float v, bool) { t += v; });
+            const float mean = head_sum(t) * inv_d;
+            each([&](float& v, bool there) { v -= there ? mean : 0.f; });
+            t = 0.f;
+          }
+          each([&](float v, bool) { t += v * v; });
+          return head_sum(t) * inv_d;
+        };
+        float square = mean_square() + a.eps;
+        const bool outside = !(square >= 0x1p-100f && square <= FLT_MAX);
+        if (__any(outside)) {
+          // sums that pass fp32, or squares that vanish in it: again from the head over a power of two near its largest value (or eps's
+          // root), which the norm takes out.  Infinities stay.
+          const raw* sp = src + (int64_t)min(h, h1 - 1) * src_h;
+          float top = sqrtf(a.eps);
+#pragma unroll
+          for (int x = 0; x < UPL; ++x)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              if (at[x][p] >= 0) Piece<E, V>::widen(Piece<E, V>::load(sp + at[x][p]), f[x][p]);
+          each([&](float v, bool there) { top = there ? fmaxf(top, fabsf(v)) : top; });
+          for (int o = 1; o < pl.lph; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+          const uint32_t exponent = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+          const float scale = outside && top <= FLT_MAX ? __uint_as_float((254u - exponent) << 23) : 1.f;
+          each([&](float& v, bool there) { v = there ? v * scale : 0.f; });
+          square = mean_square() + a.eps * scale * scale;
+          if (a.eps > 0.f) square = fmaxf(square, FLT_MIN);                  // (a head of one value: 0)
         }
-        float t = 0.f;
-#pragma unroll
-        for (int x = 0; x < UPL; ++x)
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              f[x][p][e] -= NORM == 2 && at[x][p] >= 0 ? mean : 0.f;
-              t += f[x][p][e] * f[x][p][e];
-            }
-        const float rs = rsqrtf(head_sum(t) * inv_d + a.eps);
+        const float rs = rsqrtf(square);
 #pragma unroll
         for (int x = 0; x < UPL; ++x)
 #pragma unroll
