@@ -417,74 +417,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, in
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
 
-// A weight of zero does not keep a NaN or an infinity out of a sum, so a tile that some of its rows see in
-// part can leave in a row's result what only keys hidden from it hold.  Such rows are done again by
-// exact_row.  That is slow, so a result that is not finite for a reason of its own is told apart
-// first: every hidden value near is finite, or the row's last key has a NaN in the very dims.
-
-// Whether keys first .. end - 1 of the key head hold a value that is not finite; by a wave, uniform.
-template <class E>
-__device__ __forceinline__ bool hidden_not_finite(const sf_packed_attention_args& a, const Seq& s, int hk, int first, int end) {
-  const int lane = threadIdx.x & 63;
-  float f = 0.f;
-  for (int j = max(first, 0); j < end; ++j) {
-    const uint16_t* v = (const uint16_t*)a.v + (int64_t)(s.k0 + j) * a.v_s[0] + (int64_t)hk * a.v_s[1];
-    if (lane < a.D) f = __builtin_fmaf(E::to_float(v[lane]), 0.f, f);
-    if (lane + 64 < a.D) f = __builtin_fmaf(E::to_float(v[lane + 64]), 0.f, f);
-  }
-  return __any(!(f == 0.f));
-}
-
-// Of a row's dims d .. d + 3: whether one is not finite that is no NaN in the row's last key (-1: it has none).
-template <class E>
-__device__ __forceinline__ bool unexplained(const sf_packed_attention_args& a, const Seq& s, int hk, int last, int d, const float (&o)[4]) {
-  bool doubt = false;
-  for (int e = 0; e < 4; ++e) {
-    if (__builtin_fmaf(o[e], 0.f, 0.f) == 0.f || d + e >= a.D) continue;
-    const uint16_t* v = (const uint16_t*)a.v + (int64_t)(s.k0 + max(last, 0)) * a.v_s[0] + (int64_t)hk * a.v_s[1];
-    const float x = last < 0 ? 0.f : E::to_float(v[d + e]);
-    doubt |= x == x;
-  }
-  return doubt;
-}
-
-// One row exactly, by a wave, straight from its definition: keys 0 .. last in chunks of 64, a lane
-// each for the products, lanes over the dims for the sums.
-template <class E>
-__device__ __forceinline__ void exact_row(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r, int hk) {
-  const int lane = threadIdx.x & 63, D = a.D, last = last_key(s, a.causal, r, pl);
-  const float c0 = pl.c0;
-  const uint16_t* q = (const uint16_t*)a.q + row_at(s, pl, hk, r, a.q_s);
-  const uint16_t* k = (const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1];
-  const uint16_t* v = (const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1];
-  float m = -FLT_MAX, l = 0.f, o[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 <= last; j0 += 64) {
-    const int j = min(j0 + lane, last);
-    float t = 0.f;
-    for (int d = 0; d < D; ++d) t += E::to_float(q[d]) * E::to_float(k[(int64_t)j * a.k_s[0] + d]);
-    t = c0 < 0.f ? -t : t;
-    if (j0 + lane > last) t = -INFINITY;
-    float mx = fmaxf(t, m);
-#pragma unroll
-    for (int x = 32; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const float w = fast_exp2((m - mx) * fabsf(c0)), p = fast_exp2(__builtin_fmaf(t - mx, fabsf(c0), -E::shift(s.lk)));
-    m = mx;
-    l = l * w + wave_sum(p);
-    o[0] *= w;
-    o[1] *= w;
-    const int n = min(64, last + 1 - j0);
-    for (int x = 0; x < n; ++x) {
-      const float px = __shfl(p, x);
-      const uint16_t* vr = v + (int64_t)(j0 + x) * a.v_s[0];
-      if (lane < D) o[0] += px * E::to_float(vr[lane]);
-      if (lane + 64 < D) o[1] += px * E::to_float(vr[lane + 64]);
-    }
-  }
-  uint16_t* out = (uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s);
-  if (lane < D) out[lane] = last < 0 ? 0 : E::from_float(o[0] / l);
-  if (lane + 64 < D) out[lane + 64] = last < 0 ? 0 : E::from_float(o[1] / l);
-}
-
 // What a wave holds of its 32 rows: lane (li, half) has row li; o[db][r] is dim 32 db + 8 (r / 4) +
 // 4 half + r % 4; l is the lane's own part of the sum (its keys).
 template <class E, int KC>
@@ -572,7 +504,7 @@ struct RowState {
   // The tile's sum of weights accepted, or the reference point moved and the weights formed again.
   template <int NB>
   __device__ __forceinline__ void settle(f32x16 (&s)[NB], uint32_t (&p)[8 * NB], float (&sum)[2]) {
-    if (__any(!(sum[0] + sum[1] <= limit))) {
+    if (__builtin_expect(__any(!(sum[0] + sum[1] <= limit)), 0)) {
       float mx = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
@@ -645,14 +577,64 @@ struct RowState {
     settle<NB>(s, p, sum);
   }
 
-  // Zero where every accumulator is finite, NaN otherwise.
-  __device__ __forceinline__ float finite_probe() const {
-    float f = 0.f;
+  // A weight of zero does not keep a NaN or an infinity out of a sum, so the tiles that only some of the rows see leave in a
+  // row's sums what keys hidden from it hold.  They come first; after them, the sums that are not finite are formed again, from
+  // the visible values alone: by the wave, row by row, keys top KT .. +KT - 1, (top - step) KT .., down to `end` KT, a lane each
+  // for the products, lanes over the dims for the sums.
+  template <int KT>
+  __device__ __forceinline__ void without_hidden(const sf_packed_attention_args& a, const PackedPlan& pl, const Seq& s, int r0, int hk,
+                                                 int top, int end, int step) {
+    float probe[4] = {0.f, 0.f, 0.f, 0.f};                   // zero where all are finite, NaN otherwise
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) f = __builtin_fmaf(o[db][x], 0.f, f);
-    return f;
+      for (int x = 0; x < 16; ++x) probe[x & 3] = __builtin_fmaf(o[db][x], 0.f, probe[x & 3]);
+    const float f = (probe[0] + probe[1]) + (probe[2] + probe[3]);
+    const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
+    const uint64_t not_finite = __ballot(!(f == 0.f) && r0 + li < s.lq * pl.G);
+    const uint16_t* k = (const uint16_t*)a.k + (int64_t)s.k0 * a.k_s[0] + (int64_t)hk * a.k_s[1];
+    const uint16_t* v = (const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1];
+#pragma unroll 1
+    for (uint32_t rows = (uint32_t)not_finite | (uint32_t)(not_finite >> 32); rows != 0; rows &= rows - 1) {
+      const int own = __builtin_ctz(rows), last = last_key(s, a.causal, r0 + own, pl);
+      const uint16_t* qr = (const uint16_t*)a.q + row_at(s, pl, hk, r0 + own, a.q_s);
+      const float far = __shfl(mc, own), from = far != far ? __shfl(m, own) : 0.f, less = far != far ? shift : far;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int t = top; t >= end; t -= step) {
+        const int n = min(KT, last + 1 - t * KT);            // visible keys of the tile
+        if (n <= 0) continue;
+        const uint16_t* kr = k + (int64_t)(t * KT + min(lane, n - 1)) * a.k_s[0];
+        float x = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < a.D; d += 8) {
+          const u32x4 qd = ld16(qr + d), kd = ld16(kr + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x += E::to_float((uint16_t)qd[e]) * E::to_float((uint16_t)kd[e]);
+            x += E::to_float((uint16_t)(qd[e] >> 16)) * E::to_float((uint16_t)(kd[e] >> 16));
+          }
+        }
+        x = pl.c0 < 0.f ? -x : x;
+        const float w = E::to_float(E::from_float(fast_exp2(__builtin_fmaf(x - from, c0, -less))));
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+          const float wj = __shfl(w, j);
+          const uint16_t* vr = v + (int64_t)(t * KT + j) * a.v_s[0];
+          if (lane < a.D) sum[0] += wj * E::to_float(vr[lane]);
+          if (lane + 64 < a.D) sum[1] += wj * E::to_float(vr[lane + 64]);
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int d = 32 * db + 8 * (x >> 2) + 4 * half + (x & 3);
+          const float y = __shfl(sum[db >> 1], d & 63);
+          o[db][x] = li == own ? y : o[db][x];
+          if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);                 // (few registers)
+        }
+    }
   }
 };
 
@@ -777,6 +759,8 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
       vs.load(64 * (t - 2 * KG), s.lk, t - 2 * KG >= t_lo);
       lds_only_barrier();
     }
+    const int top = t;
+    int hidden = a.causal ? max(t_lo, (low + 1) >> 6) + KG - 1 : -KG;        // once there, the group's tiles left are seen to their end
     // (the buffers as constants: LDS addresses are formed once)
     auto step = [&](auto constant) __attribute__((always_inline)) {
       constexpr int B = decltype(constant)::value;
@@ -792,6 +776,10 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
       uint32_t p[16];
       st.template weights<2>(sc, p);
       st.template gather<2>(p, vt(B), [](int) {});
+      if (__builtin_expect(t <= hidden, 0)) {
+        st.template without_hidden<64>(a, pl, s, r0, hk, top, max(t, t_lo), KG);
+        hidden = -KG;
+      }
       lds_only_barrier();
       t -= KG;
     };
@@ -841,23 +829,8 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
     return;
   }
   const float inv = mine < 0 ? 0.f : 1.f / l;
-  // rows to be done again (see exact_row): either half's accumulators are not finite
-  uint64_t badl = __ballot(a.causal && !(st.finite_probe() == 0.f) && r0 + li < rows);
-  if (badl != 0) {
-    bool doubt = false;
-#pragma unroll
-    for (int db = 0; db < T::DB; ++db)
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {
-        const float o[4] = {st.o[db][4 * c4], st.o[db][4 * c4 + 1], st.o[db][4 * c4 + 2], st.o[db][4 * c4 + 3]};
-        doubt |= unexplained<E>(a, s, hk, mine, 32 * db + 8 * c4 + 4 * half, o);
-      }
-    badl &= __ballot(doubt);
-    if (badl != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (high | 63) + 1))) badl = 0;
-  }
-  uint32_t bad = (uint32_t)badl | (uint32_t)(badl >> 32);
   uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, row, a.o_s);
-  const bool write = r0 + li < rows && !(bad >> li & 1);
+  const bool write = r0 + li < rows;
 #pragma unroll
   for (int db = 0; db < T::DB; ++db)
 #pragma unroll
@@ -871,10 +844,6 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_p
       const int d0 = 32 * db + 16 * c + 8 * half;
       if (write && d0 < a.D) st16(op + d0, u32x4{x[0], y[0], x[1], y[1]});
     }
-  for (; bad != 0; bad &= bad - 1) {
-    const int r = r0 + __builtin_ctz(bad);
-    exact_row<E>(a, pl, s, r, hk);
-  }
 }
 
 // 32 rows a workgroup (a new token's heads, short pieces): its 4 waves each stream a slice of the
@@ -938,6 +907,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
       vs.init((const uint16_t*)a.v + (int64_t)s.k0 * a.v_s[0] + (int64_t)hk * a.v_s[1], a.v_s[0], lane, a.D);
       load_k(KT * (t_hi - 1), true);
       vs.load(KT * (t_hi - 1), s.lk, true);
+      const int hidden = a.causal ? max(t_lo, (low + 1) / KT) : -1;          // last of the tiles that some rows do not see to their end
       for (int t = t_hi - 1; t >= t_lo; --t) {
         f32x16 sc[NB];
 #pragma unroll
@@ -954,6 +924,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
         uint32_t p[8 * NB];
         st.template weights<NB>(sc, p);
         st.template gather<NB>(p, vt, [](int) {});
+        if (__builtin_expect(t == hidden, 0)) st.template without_hidden<KT>(a, pl, s, r0, hk, t_hi - 1, t, 1);
       }
     }
     // the slice's O over the wave's tiles, for all threads
@@ -978,7 +949,6 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 #pragma unroll
   for (int w = 0; w < 4; ++w) l += wt[w] * ml[w][jr][1];
   f32x4 o[T::DB];
-  float probe = 0.f;
 #pragma unroll
   for (int db = 0; db < T::DB; ++db) {
     o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -988,8 +958,6 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[db][e] += wt[w] * x[e];
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[db][e], 0.f, probe);
   }
   if (slices > 1) {
     float* po = pl.part + (int64_t)block * 32 * (T::DP + 2);
@@ -1001,16 +969,7 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
     return;
   }
   const int r = r0 + jr;
-  uint64_t bad8 = __ballot(a.causal && !(probe == 0.f) && r < rows);         // a byte for each of the wave's 8 rows
-  if (bad8 != 0) {
-    bool doubt = false;
-#pragma unroll
-    for (int db = 0; db < T::DB; ++db)
-      doubt |= unexplained<E>(a, s, hk, last_key(s, a.causal, min(r, rows - 1), pl), 32 * db + jd, {o[db][0], o[db][1], o[db][2], o[db][3]});
-    bad8 &= __ballot(doubt);
-    if (bad8 != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (seen - 1 | 63) + 1))) bad8 = 0;
-  }
-  if (r < rows && !(bad8 >> (lane & 56) & 0xff)) {
+  if (r < rows) {
     const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / l;
     uint16_t* op = (uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s);
 #pragma unroll
@@ -1018,8 +977,6 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const sf_packed_a
       if (32 * db + jd < a.D)
         *reinterpret_cast<u32x2*>(op + 32 * db + jd) = u32x2{E::pack(o[db][0] * inv, o[db][1] * inv), E::pack(o[db][2] * inv, o[db][3] * inv)};
   }
-  for (int x = 0; x < 8; ++x)
-    if (bad8 >> (8 * x) & 0xff) exact_row<E>(a, pl, s, r0 + wave * 8 + x, hk);
 }
 
 // Joins the key slices: o = sum_z w_z O_z / sum_z w_z l_z with w_z the worth of slice z's reference point
@@ -1118,24 +1075,11 @@ __global__ __launch_bounds__(256) void packed_combine_kernel(const sf_packed_att
     for (int x = 0; x < PASSES; ++x) {
       const int in = kOneRow ? in0 : in0 + x * GROUPS + group, r = r0 + in;
       const bool mine = r < rows && d < a.D && (!kOneRow || tid < LR);
-      float probe = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) probe = __builtin_fmaf(o[x][e], 0.f, probe);
-      uint64_t bad = __ballot(a.causal && mine && !(probe == 0.f));
-      if (bad != 0) {
-        const int r32 = r0 + (in0 & ~31), low = last_key(s, a.causal, r32, pl), high = last_key(s, a.causal, min(r32 + 31, rows - 1), pl);
-        bad &= __ballot(unexplained<E>(a, s, hk, last_key(s, a.causal, min(r, rows - 1), pl), d, {o[x][0], o[x][1], o[x][2], o[x][3]}));
-        if (bad != 0 && !hidden_not_finite<E>(a, s, hk, low + 1, min(s.lk, (high | 63) + 1))) bad = 0;
-      }
-      const uint64_t lanes = ((1ull << LR) - 1) << (lane / LR * LR);
-      if (mine && !(bad & lanes)) {
+      if (mine) {
         const float inv = last_key(s, a.causal, r, pl) < 0 ? 0.f : 1.f / sum[x];
         *reinterpret_cast<u32x2*>((uint16_t*)a.out + row_at(s, pl, hk, r, a.o_s) + d) =
             u32x2{E::pack(o[x][0] * inv, o[x][1] * inv), E::pack(o[x][2] * inv, o[x][3] * inv)};
       }
-#pragma unroll
-      for (int g = 0; g < 64 / LR; ++g)
-        if (bad >> (g * LR) & ((1ull << LR) - 1)) exact_row<E>(a, pl, s, kOneRow ? r : r0 + in0 + x * GROUPS + tid / 64 * (64 / LR) + g, hk);
     }
   }
 }

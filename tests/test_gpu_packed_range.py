@@ -116,3 +116,33 @@ def test_more_workgroups_than_a_launch_dimension_holds():
   out = torch.full_like(q, 7.0)
   ops.packed_attention(q, k, v, cu, len_q=used, out=out)
   assert torch.equal(out[used == 1], v[used == 1]) and (out[::3] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,share", [(128, 0.02), (64, 0.0005), (24, 0.3)])
+@pytest.mark.parametrize("route", ROUTES + [(5, 40, (4, 1)), (4200, 4200, (32, 8))], ids=lambda r: f"{r[0]}x{r[1]}")
+def test_values_that_are_not_finite_here_and_there(route, D, share, dtype):
+  """Causal, a share of the values NaN or infinite: a result has what its row sees in its dim, and nothing of what it does not."""
+  n, m, (H, Hk) = route
+  q, k, v = make([n], [m], H, Hk, D, TYPES[dtype], 7)
+  q = q / 4                                          # (every weight is far from vanishing)
+  kind = torch.rand(m, Hk, D, generator=torch.Generator().manual_seed(m)).to(DEV) / share
+  for i, bad in enumerate((math.inf, -math.inf, math.nan)):
+    v[(kind >= i / 3) & (kind < (i + 1) / 3)] = bad
+  out = ops.packed_attention(q, k, v, offsets([n]), offsets([m]), causal=True)
+  some = sorted(set(range(0, n, max(n // 60, 1))) | set(range(max(n - 40, 0), n)))
+  for h in range(0, H, max(H // 3, 1)):
+    vh, oh = v[:, h // (H // Hk)].cpu().double(), out[some, h].cpu().double()
+    s = q[some, h].cpu().double() @ k[:, h // (H // Hk)].cpu().double().T / math.sqrt(D)
+    limit = torch.tensor(some) + (m - n)
+    p = torch.softmax(s.masked_fill(torch.arange(m)[None] > limit[:, None], -math.inf), -1)
+    nan, top, low = (c.double().cumsum(0)[limit] > 0 for c in (torch.isnan(vh), vh == math.inf, vh == -math.inf))
+    nan |= top & low
+    assert torch.equal(torch.isnan(oh), nan)
+    assert torch.equal(oh == math.inf, top & ~nan) and torch.equal(oh == -math.inf, low & ~nan)
+    rest = ~(nan | top | low)
+    vf = vh.nan_to_num(0.0, 0.0, 0.0)
+    want, a, u = p @ vf, p @ vf.abs(), torch.finfo(TYPES[dtype]).eps / 2
+    size = (q[some, h].cpu().double().abs() @ k[:, h // (H // Hk)].cpu().double().abs().T).amax() / math.sqrt(D)
+    tol = 2 * (u + (D + 8) * 2.0 ** -23 * size + m * 2.0 ** -24) * a + u * want.abs() + (m * 2.0 ** -30 * 4 if dtype == "fp16" else 0.0) + 1e-30
+    assert ((oh - want).abs() <= tol)[rest].all()
