@@ -146,3 +146,61 @@ def test_values_that_are_not_finite_here_and_there(route, D, share, dtype):
     size = (q[some, h].cpu().double().abs() @ k[:, h // (H // Hk)].cpu().double().abs().T).amax() / math.sqrt(D)
     tol = 2 * (u + (D + 8) * 2.0 ** -23 * size + m * 2.0 ** -24) * a + u * want.abs() + (m * 2.0 ** -30 * 4 if dtype == "fp16" else 0.0) + 1e-30
     assert ((oh - want).abs() <= tol)[rest].all()
+
+
+def sampled(out, q, k, v, causal):
+  """Rows of one sequence against the definition, two heads: every 61st, the first and the last ones."""
+  (n, H, D), (m, Hk, _), dt = q.shape, k.shape, q.dtype
+  some = torch.tensor(sorted(set(range(0, n, 61)) | set(range(min(n, 20))) | set(range(max(n - 40, 0), n))), device=DEV)
+  u = torch.finfo(dt).eps / 2
+  for h in (0, H - 1):
+    qh, kh, vh = q[some, h].double(), k[:, h // (H // Hk)].double(), v[:, h // (H // Hk)].double()
+    s, size = qh @ kh.T / math.sqrt(D), (qh.abs() @ kh.abs().T).amax(-1, keepdim=True) / math.sqrt(D)
+    if causal:
+      s = s.masked_fill(torch.arange(m, device=DEV)[None] > some[:, None] + (m - n), -math.inf)
+    p = torch.softmax(s, -1).nan_to_num(0.0)
+    want, a = p @ vh, p @ vh.abs()
+    tol = 2 * (u + (D + 8) * 2.0 ** -23 * size + m * 2.0 ** -24) * a + u * want.abs() + 1e-30
+    assert ((out[some, h].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_widest_tiles_over_caches_with_free_rows(causal):
+  """Tiles of 256 rows: lengths in use, fewer keys than queries, NaN in every free row of queries and caches."""
+  room, used, cache, filled = [2500, 1700], [2300, 1650], [2700, 1800], [2650, 900]
+  q, k, v = make(room, cache, 32, 8, 128, torch.bfloat16, 21)
+  # (k and v have as many rows as the caches)
+  for b in range(2):
+    q[sum(room[:b]) + used[b]:sum(room[:b + 1])] = math.nan
+    for t in (k, v):
+      t[sum(cache[:b]) + filled[b]:sum(cache[:b + 1])] = math.nan
+  i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+  out = torch.full_like(q, 7.0)
+  ops.packed_attention(q, k, v, offsets(room), offsets(cache), len_q=i32(used), len_k=i32(filled), causal=causal, out=out)
+  for b in range(2):
+    aq, ak = sum(room[:b]), sum(cache[:b])
+    assert (out[aq + used[b]:sum(room[:b + 1])] == 7.0).all()
+    sampled(out[aq:aq + used[b]], q[aq:aq + used[b]], k[ak:ak + filled[b]], v[ak:ak + filled[b]], causal)
+
+
+def test_one_long_sequence_among_empty_ones():
+  """Shared key slices of 512 row tiles over 5 million keys: more units of keys than 32-bit floats count one by one."""
+  n, m, B = 16384, 5_000_000, 256
+  g = torch.Generator(device=DEV).manual_seed(5)
+  q, k, v = (torch.randn(t, 1, 8, generator=g, device=DEV, dtype=torch.bfloat16) for t in (n, m, m))
+  lens_q, lens_k = [0] * 100 + [n] + [0] * (B - 101), [0] * 100 + [m] + [0] * (B - 101)
+  out = ops.packed_attention(q, k, v, offsets(lens_q), offsets(lens_k))
+  for r in torch.arange(0, n, 2000).tolist() + [n - 1]:
+    s = q[r, 0].double() @ k[:, 0].double().T / math.sqrt(8)
+    p = torch.softmax(s, -1)
+    want, a = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+    # (fp32 sums of m terms, whose roundings are of random sign, are split over 4 x slices waves: 2^-24 m / 64 is far above them)
+    assert ((out[r, 0].double() - want).abs() <= 2 * (2.0 ** -8 + 2.0 ** -18 + m / 64 * 2.0 ** -24) * a + 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_prompt_beside_single_tokens(causal):
+  """A piece of a prompt, tokens over long caches, an empty sequence: one call, each as by itself."""
+  lens_q, lens_k = [512, 1, 1, 0, 1, 300], [700, 9000, 1, 5, 65, 300]
+  q, k, v = make(lens_q, lens_k, 8, 2, 128, torch.bfloat16, 22)
+  check(ops.packed_attention(q, k, v, offsets(lens_q), offsets(lens_k), causal=causal), q, k, v, lens_q, lens_k, causal)
