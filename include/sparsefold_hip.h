@@ -491,7 +491,7 @@ int sf_hip_diffusion_conditioning_fwd(const sf_diffusion_conditioning_args* a, v
  * bf16 or f16, last dimension contiguous, 16-byte aligned rows (strides multiples of 8); D % 8 == 0,
  * D <= 128; k_s[0], v_s[0] in [D, 2^24); Tk and Tq * G up to 2^30, (Tq * G / 32 + B) * Hkv up to 2^26.  fp32
  * softmax and accumulation; the weights are rounded to the element type for the product with v, in f16 those below
- * 2^-31 of the largest of their keys to 0.  A mean of finite values is finite, up to the type's largest; in bf16
+ * 2^-29 of the largest of their keys to 0.  A mean of finite values is finite, up to the type's largest; in bf16
  * values below 2^(bits of the number of keys - 105) may lose digits.  out holds each element once and may not
  * overlap q, k or v. */
 typedef struct sf_packed_attention_args {

@@ -47,10 +47,11 @@ struct Bf16 {
   static __device__ __forceinline__ uint16_t from_float(float v) { return f2bf(v); }
 };
 struct Fp16 {
-  // Weights of 2^6 at the reference point, and of 2^15 where a lane's move it: finite, and rounded to a multiple of 2^-24,
-  // so that only those below 2^-31 of the reference point's vanish.  (Values are too small to pass fp32.)
-  static constexpr int kMass = 9;
-  static __device__ __forceinline__ float shift(int) { return -6.f; }
+  // Weights of 2^4 at the reference point, finite where a lane's sum to no more than 2^16 (an infinite one does not), and
+  // rounded to a multiple of 2^-24: only those below 2^-29 of the reference point's vanish.  (Values are too small to pass
+  // fp32.)
+  static constexpr int kMass = 12;
+  static __device__ __forceinline__ float shift(int) { return -4.f; }
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }

@@ -93,7 +93,7 @@ def test_small_values_keep_their_digits(route):
 @pytest.mark.parametrize("nats", [17.375, 19.0])
 def test_fp16_weights_far_below_the_largest(nats):
   """One key above 30000 others whose weights are 2^-25.07 or 2^-27.4 of its: a weight is off by 2^-25 where the largest is
-  2^6 2^-1/2 at least, so n 2^-30 max |v|, and by 2 u of itself where it is normal."""
+  2^4 2^-1/2 at least, so n 2^-28.5 max |v|, and by 2 u of itself where it is normal."""
   n, m, H, D = 1300, 30000, 32, 32                   # (enough workgroups that all keys share a reference point)
   q, k = torch.zeros(n, H, D, dtype=torch.float16, device=DEV), torch.zeros(m, H, D, dtype=torch.float16, device=DEV)
   v = (1 + torch.rand(m, H, D, generator=torch.Generator().manual_seed(1)) / 4).half().to(DEV)
@@ -101,7 +101,7 @@ def test_fp16_weights_far_below_the_largest(nats):
   out = ops.packed_attention(q, k, v, offsets([n]), offsets([m]), scale=1.0).double()
   p = math.exp(-nats) / (1 + (m - 1) * math.exp(-nats))
   want = p * v.double().sum(0)
-  assert ((out - want).abs() <= m * 2.0 ** -30 * 1.25 + 3 * 2.0 ** -11 * want).all()
+  assert ((out - want).abs() <= m * 2.0 ** -28.5 * 1.25 + 3 * 2.0 ** -11 * want).all()
 
 
 def test_more_workgroups_than_a_launch_dimension_holds():
