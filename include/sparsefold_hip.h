@@ -491,9 +491,9 @@ int sf_hip_diffusion_conditioning_fwd(const sf_diffusion_conditioning_args* a, v
  * bf16 or f16, last dimension contiguous, 16-byte aligned rows (strides multiples of 8); D % 8 == 0,
  * D <= 128; k_s[0], v_s[0] in [D, 2^24); Tk and Tq * G up to 2^30, (Tq * G / 32 + B) * Hkv up to 2^26.  fp32
  * softmax and accumulation; the weights are rounded to the element type for the product with v, in f16 those below
- * 2^-29 of the largest of their keys to 0.  A mean of finite values is finite, up to the type's largest; in bf16
- * values below 2^(bits of the number of keys - 105) may lose digits.  out holds each element once and may not
- * overlap q, k or v. */
+ * 2^-29 of the largest of their keys to 0.  A mean of finite values is finite, up to the type's largest; for that,
+ * bf16 weights below 2^(bits of the number of keys - 105) of the largest are 0 and values below that may lose digits.
+ * out holds each element once and may not overlap q, k or v. */
 typedef struct sf_packed_attention_args {
   int32_t B, H, Hkv, D;
   int64_t Tq, Tk;                               /* rows of q / out and of k / v */
@@ -518,7 +518,8 @@ int sf_hip_packed_attention_fwd(const sf_packed_attention_args* a, void* workspa
  * The angle is formed and reduced in 64 bits, the rest is fp32, rounded once.  q [T, H, D] and
  * k [T, Hk, D] (Hk = 0: none) share token positions; the last dimension is contiguous.  q_out may be q
  * and k_out may be k (same strides); otherwise outputs overlap no input.  H, Hk <= 2^24, D <= 256, R even, 2 <= R <= D.
- * Weights and biases f32 [D] or NULL (1 and 0), read only where norm asks for them. */
+ * Weights and biases f32 [D] or NULL (1 and 0), read only where norm asks for them.  A norm holds for heads of any finite
+ * size, also where their squares leave f32. */
 #define SF_NORM_NONE 0
 #define SF_NORM_RMS 1
 #define SF_NORM_LAYER 2

@@ -905,7 +905,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
   """Norm of each query and key head, then their rotary positions, in one pass; arguments and results
   as ``rotary``.  ``norm`` ``"rms"``: ``x rsqrt(mean x^2 + eps) weight``; ``"layer"``:
   ``(x - mean) rsqrt(var + eps) weight + bias``, over the D dims of a head.  Weights and biases ``[D]``
-  (None: 1 and 0; biases with ``"layer"`` only)."""
+  (None: 1 and 0; biases with ``"layer"`` only), float32; others are cast at every call."""
   what = "qk_norm_rotary"
   if norm not in _NORMS:
     raise ValueError(f"{what}: norm {norm!r} is not 'rms' or 'layer'")

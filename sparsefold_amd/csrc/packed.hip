@@ -695,9 +695,9 @@ struct Stage {
 //
 // Bound by the issue of matrix products and of the weights' vector instructions, which overlap little: 64 keys x 32 rows
 // of 128 dims take 435 and 249 ns, together 577 in a loop of registers alone (64 dims: 218, 237, 406).  A prompt of 16384,
-// 32 / 8 heads of 128, causal, bf16: 1.85 to 1.97 ms from card to card, 1.19 to 1.12 PFLOP/s (bf16 products of 8192^3:
-// 1.2 to 1.4), of 4096 136 to 144 us; 1.52 ms where all inputs are zero, which draw less power.  8192 tokens, 16
-// heads of 64: 168 us, 0.82 PFLOP/s.
+// 32 / 8 heads of 128, causal, bf16: 1.83 to 2.03 ms from card to card, 1.20 to 1.08 PFLOP/s (bf16 products of 8192^3:
+// 1.2 to 1.4), of 4096 134 to 143 us; 1.52 ms where all inputs are zero, which draw less power.  8192 tokens, 16
+// heads of 64: 168 to 177 us, 0.82 to 0.78 PFLOP/s.
 template <class E, int KC, int NW, int KG>
 __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const sf_packed_attention_args a, const PackedPlan pl) {
   using T = Dims<KC>;
