@@ -100,7 +100,7 @@ def draw(rng):
     x, w = rng.choice([("mxfp8", "mxfp4"), ("mxfp8", "mxfp8"), ("mxfp4", "mxfp4")])
     dim, features = BLOCK * _log_int(rng, 4, 256), _log_int(rng, 64, 8192)
     return _linear(None, _log_int(rng, 1, 8192), dim, features - features % rng.choice([1, 8, 64]), x, w, rng.random() < 0.4,
-                   rng.choice(["bf16", "bf16", "fp16", "fp32"]))
+                   rng.choice(["bf16", "bf16", "fp16"]))
   kv_heads, group = rng.choice([1, 2, 4, 8]), rng.choice([1, 2, 4, 4, 8])
   dim, page, dtype = rng.choice([32, 64, 64, 80, 96, 128, 128]), rng.choice([16, 16, 32, 64, 64, 128, 48]), rng.choice(["bf16", "fp16"])
   if op == "write":
