@@ -11,10 +11,11 @@ from pathlib import Path
 from struct import Struct
 
 LIB_PATH = Path(__file__).resolve().parent / "libsparsefold_hip.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 TRI_STAGE_PROJECT, TRI_STAGE_ATTEND, TRI_STAGE_OUTPUT, TRI_STAGE_ALL, TRI_STAGE_FUSE = 1, 2, 4, 7, 8
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2   # SF_DTYPE_*
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2    # SF_NORM_*
+FORMAT_MXFP8, FORMAT_MXFP4 = 0, 1            # SF_FORMAT_*
 NOALLOC_SCRATCH_BYTES = 64 << 20           # SF_HIP_NOALLOC_SCRATCH_BYTES
 
 _i32, _i64, _f32, _vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
@@ -179,6 +180,51 @@ class RotaryArgs(C.Structure):
   ]
 
 
+class PagedAttentionArgs(C.Structure):
+  _fields_ = [
+      ("B", _i32), ("H", _i32), ("Hkv", _i32), ("D", _i32), ("Tq", _i64), ("pages", _i64),
+      ("page_rows", _i32), ("table_cols", _i32), ("max_keys", _i64),
+      ("scale", _f32), ("causal", _i32), ("dtype", _i32),
+      ("q", _vp), ("q_s", _i64 * 2), ("k", _vp), ("k_s", _i64 * 3), ("v", _vp), ("v_s", _i64 * 3),
+      ("out", _vp), ("o_s", _i64 * 2),
+      ("cu_q", _vp), ("len_q", _vp), ("len_k", _vp), ("table", _vp), ("table_s", _i64),
+  ]
+
+
+class PagedWriteArgs(C.Structure):
+  _fields_ = [
+      ("B", _i32), ("Hkv", _i32), ("D", _i32), ("T", _i64), ("pages", _i64), ("page_rows", _i32), ("table_cols", _i32),
+      ("k", _vp), ("k_s", _i64 * 2), ("v", _vp), ("v_s", _i64 * 2),
+      ("k_pages", _vp), ("kp_s", _i64 * 3), ("v_pages", _vp), ("vp_s", _i64 * 3),
+      ("cu", _vp), ("len_new", _vp), ("len_k", _vp), ("table", _vp), ("table_s", _i64),
+  ]
+
+
+class MxConvertArgs(C.Structure):
+  _fields_ = [
+      ("R", _i64), ("K", _i32), ("dtype", _i32), ("format", _i32),
+      ("x", _vp), ("x_rs", _i64), ("codes", _vp), ("c_rs", _i64), ("scales", _vp), ("s_rs", _i64),
+  ]
+
+
+class AddRmsNormArgs(C.Structure):
+  _fields_ = [
+      ("R", _i64), ("C", _i32), ("dtype", _i32), ("format", _i32), ("eps", _f32),
+      ("x", _vp), ("x_rs", _i64), ("residual", _vp), ("r_rs", _i64), ("weight", _vp),
+      ("sum", _vp), ("h_rs", _i64), ("y", _vp), ("y_rs", _i64),
+      ("codes", _vp), ("c_rs", _i64), ("scales", _vp), ("s_rs", _i64),
+  ]
+
+
+class MxLinearArgs(C.Structure):
+  _fields_ = [
+      ("M", _i64), ("N", _i32), ("K", _i32), ("x_format", _i32), ("w_format", _i32), ("dtype", _i32),
+      ("x", _vp), ("x_rs", _i64), ("x_scales", _vp), ("xs_rs", _i64),
+      ("w", _vp), ("w_rs", _i64), ("w_scales", _vp), ("ws_rs", _i64),
+      ("bias", _vp), ("y", _vp), ("y_rs", _i64),
+  ]
+
+
 STRUCTS = {
     "sf_attention_args": AttentionArgs,
     "sf_layer_norm_args": LayerNormArgs,
@@ -194,6 +240,11 @@ STRUCTS = {
     "sf_transition_args": TransitionArgs,
     "sf_packed_attention_args": PackedAttentionArgs,
     "sf_rotary_args": RotaryArgs,
+    "sf_paged_attention_args": PagedAttentionArgs,
+    "sf_paged_write_args": PagedWriteArgs,
+    "sf_mx_convert_args": MxConvertArgs,
+    "sf_add_rms_norm_args": AddRmsNormArgs,
+    "sf_mx_linear_args": MxLinearArgs,
 }
 
 
@@ -214,6 +265,11 @@ def filler(struct: type[C.Structure]):
 
 packed_attention_args = filler(PackedAttentionArgs)
 rotary_args = filler(RotaryArgs)
+paged_attention_args = filler(PagedAttentionArgs)
+paged_write_args = filler(PagedWriteArgs)
+mx_convert_args = filler(MxConvertArgs)
+add_rms_norm_args = filler(AddRmsNormArgs)
+mx_linear_args = filler(MxLinearArgs)
 
 # (name, restype, argtypes) of every exported entry point.
 SIGNATURES = [
@@ -244,6 +300,14 @@ SIGNATURES = [
     ("sf_hip_packed_attention_workspace_bytes", C.c_size_t, [C.POINTER(PackedAttentionArgs)]),
     ("sf_hip_packed_attention_fwd", C.c_int, [C.POINTER(PackedAttentionArgs), _vp, C.c_size_t, _vp]),
     ("sf_hip_rotary_fwd", C.c_int, [C.POINTER(RotaryArgs), _vp]),
+    ("sf_hip_paged_attention_workspace_bytes", C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
+    ("sf_hip_paged_attention_fwd", C.c_int, [C.POINTER(PagedAttentionArgs), _vp, C.c_size_t, _vp]),
+    ("sf_hip_paged_write_fwd", C.c_int, [C.POINTER(PagedWriteArgs), _vp]),
+    ("sf_hip_mx_encode_fwd", C.c_int, [C.POINTER(MxConvertArgs), _vp]),
+    ("sf_hip_mx_decode_fwd", C.c_int, [C.POINTER(MxConvertArgs), _vp]),
+    ("sf_hip_add_rms_norm_fwd", C.c_int, [C.POINTER(AddRmsNormArgs), _vp]),
+    ("sf_hip_mx_linear_workspace_bytes", C.c_size_t, [C.POINTER(MxLinearArgs)]),
+    ("sf_hip_mx_linear_fwd", C.c_int, [C.POINTER(MxLinearArgs), _vp, C.c_size_t, _vp]),
 ]
 
 _lib: C.CDLL | None = None
