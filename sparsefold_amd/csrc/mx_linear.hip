@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "mx.h"
+#include "mx_linear.h"
 
 namespace {
 
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const sf_mx_linear_args a,
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Route {
-  bool stream;
+  bool stream, large;
   Extra ex;
 };
 
@@ -378,10 +379,11 @@ void route(const sf_mx_linear_args* a, Route& r) {
   r.ex.vector = al16(a->y) && a->y_rs % 8 == 0;
   r.ex.part = nullptr;
   r.stream = a->M <= 64;
+  r.large = !r.stream && sf_mx_linear_pp_ok(a);
   const int64_t tiles = ((a->M + 127) / 128) * ((a->N + 127) / 128);
   const int steps = (a->K / 32 + 3) / 4;
   int64_t slices = 1;
-  if (!r.stream) slices = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, steps / 8));
+  if (!r.stream && !r.large) slices = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, steps / 8));
   r.ex.steps = (int)((steps + slices - 1) / slices);
   r.ex.slices = (steps + r.ex.steps - 1) / r.ex.steps;
 }
@@ -454,5 +456,6 @@ extern "C" int sf_hip_mx_linear_fwd(const sf_mx_linear_args* a, void* workspace,
   }
   r.ex.part = static_cast<float*>(workspace);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (r.large) return sf_mx_linear_pp_launch(a, st);
   return a->dtype == SF_DTYPE_BF16 ? launch_formats<RowBf16>(a, r, st) : launch_formats<RowFp16>(a, r, st);
 }

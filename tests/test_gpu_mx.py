@@ -191,10 +191,20 @@ def test_product(M, N, K, formats):
 
 
 @pytest.mark.parametrize("formats", FORMATS, ids="-".join)
-@pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (1500, 4104, 1088), (2049, 1999, 640)])
+@pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (1500, 4104, 1088), (2049, 1999, 640), (4096, 2048, 512), (3900, 2312, 640), (2049, 4104, 1152),
+                                   (4099, 4104, 512), (9000, 1032, 512)])
 def test_large_product(M, N, K, formats):
+  """Scales of many binades too; the last ones more than one tile a workgroup."""
   x, w = operands(M, N, K, formats, 3)
+  bias = torch.randn(N, device=DEV)
   check(ops.mx_linear(x, w), x, w)
+  g = torch.Generator().manual_seed(M)
+  xs, ws = (torch.randint(120, 135, t.scales.shape, generator=g).to(torch.uint8).to(DEV) for t in (x, w))
+  x, w = ops.Microscaled(x.codes, xs), ops.Microscaled(w.codes, ws)
+  out = torch.full((M + 1, N + 16), 5.0, dtype=torch.bfloat16, device=DEV)
+  ops.mx_linear(x, w, bias, out=out[:M, 8:8 + N])
+  check(out[:M, 8:8 + N], x, w, bias)
+  assert (out[M] == 5).all() and (out[:, :8] == 5).all() and (out[:, 8 + N:] == 5).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
@@ -225,7 +235,7 @@ def test_each_scale_reaches_its_block(M):
       check(ops.mx_linear(x, w), x, w)
 
 
-@pytest.mark.parametrize("M", [4, 40, 200, 2048])
+@pytest.mark.parametrize("M", [4, 40, 200, 4096])
 def test_nan_and_extreme_scales(M):
   x, w = operands(M, 2048, 256, FORMATS[1], M)
   xs, ws = x.scales.view(torch.uint8).clone(), w.scales.view(torch.uint8).clone()
