@@ -954,10 +954,10 @@ def _apart(dims) -> bool:
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
   """First byte and the byte past the last of a view with non-negative strides."""
-  p = t.data_ptr()
-  if t.numel() == 0:
-    return p, p
-  return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+  p, n = t.data_ptr(), t.numel()
+  if n > 0 and not t.is_contiguous():
+    n = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+  return p, p + n * t.element_size()
 
 
 def _spans_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -976,28 +976,40 @@ def _cache(what, k_pages, v_pages, page_table, len_k, B, dtype):
     raise ValueError(f"{what}: a cache needs pages of a multiple of 16 rows, got {tuple(shape)}")
   if D % 8 != 0 or not 0 < D <= 128:
     raise ValueError(f"{what}: head dim {D} is not a multiple of 8 up to 128")
-  ks, vs = _page_strides(k_pages), _page_strides(v_pages)
+  row = Hkv * D
+  packed = (R * row, row, D)
+  ks = packed if k_pages.is_contiguous() else _page_strides(k_pages)
+  vs = packed if v_pages.is_contiguous() else _page_strides(v_pages)
   for t, s in ((k_pages, ks), (v_pages, vs)):
-    if t.stride(3) != 1 or (s[0] | s[1] | s[2] | t.data_ptr() >> 1) % 8 or not D <= s[1] < 1 << 24:
+    if (s[0] | s[1] | s[2] | t.data_ptr() >> 1) % 8 or not D <= s[1] < 1 << 24 or t.stride(3) != 1:
       raise ValueError(f"{what}: pages must lie in 16-byte aligned rows of 1 dim after another, strides {t.stride()}")
-  if page_table.dtype is not torch.int32 or page_table.ndim != 2 or page_table.shape[0] != B or page_table.shape[1] < 1:
-    raise ValueError(f"{what}: page_table must be int32 [{B}, pages of a sequence], got {page_table.dtype} {tuple(page_table.shape)}")
-  cols = page_table.shape[1]
+  tshape = page_table.shape
+  if page_table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != B or tshape[1] < 1:
+    raise ValueError(f"{what}: page_table must be int32 [{B}, pages of a sequence], got {page_table.dtype} {tuple(tshape)}")
+  cols = tshape[1]
   if cols * R > 1 << 30:
     raise ValueError(f"{what}: {cols} pages of {R} rows a sequence exceed 2^30")
-  if cols > 1 and page_table.stride(1) != 1:
-    page_table = page_table.contiguous()
-  ts = page_table.stride(0) if B > 1 else cols
+  ts = cols
+  if not page_table.is_contiguous():
+    if cols > 1 and page_table.stride(1) != 1:
+      page_table = page_table.contiguous()
+    elif B > 1:
+      ts = page_table.stride(0)
   return ks, vs, page_table, ts, cols, _offsets32(len_k, "len_k", B, what)
 
 
-def _token_rows(t: torch.Tensor, D: int):
+def _token_rows(t: torch.Tensor, T: int, H: int, D: int):
   """``[T, H, D]`` in 16-byte aligned rows (copied where it is not): the tensor, its pointer and strides."""
-  st, sh = _strides2(t)
   ptr = t.data_ptr()
+  if ptr % 16 == 0 and t.is_contiguous():
+    return t, ptr, (H * D, D)
+  st, sh, sd = t.stride()
+  if sd == 1 and T > 1 and H > 1 and not (st | sh | ptr >> 1) % 8:
+    return t, ptr, (st, sh)
+  st, sh = _strides2(t)
   if t.stride(2) != 1 or (st | sh | ptr >> 1) % 8:
     t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
-    (st, sh), ptr = (t.shape[1] * D, D), t.data_ptr()
+    (st, sh), ptr = (H * D, D), t.data_ptr()
   return t, ptr, (st, sh)
 
 
@@ -1029,17 +1041,18 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
   ks, vs, table, ts, cols, len_k = _cache(what, k_pages, v_pages, page_table, len_k, B, dtype)
   if k_pages.shape[2:] != k.shape[1:] or Hkv * D > 1 << 24:
     raise ValueError(f"{what}: {tuple(k.shape[1:])} of k and v against {tuple(k_pages.shape[2:])} of the pages (2^24 elements at most)")
-  dims = list(zip(k_pages.shape, (*ks, 1)))
-  if not (_apart(dims) and _apart(list(zip(v_pages.shape, (*vs, 1))))):
-    raise ValueError(f"{what}: pages must hold every element once")
-  if not (_spans_apart(k_pages, v_pages) or
-          (ks == vs and _apart([*dims, (2, abs(v_pages.data_ptr() - k_pages.data_ptr()) // 2)]))):
+  for pages, strides in ((k_pages, ks), (v_pages, vs)):
+    if not (pages.is_contiguous() or _apart(zip(pages.shape, (*strides, 1)))):
+      raise ValueError(f"{what}: pages must hold every element once")
+  (k0, k1), (v0, v1) = _span(k_pages), _span(v_pages)
+  if not (k1 <= v0 or v1 <= k0 or (ks == vs and _apart([*zip(k_pages.shape, (*ks, 1)), (2, abs(v0 - k0) // 2)]))):
     raise ValueError(f"{what}: k_pages and v_pages overlap")
-  for pages in (k_pages, v_pages):
-    if not (_spans_apart(pages, k) and _spans_apart(pages, v)):
+  k, kp, sk = _token_rows(k, T, Hkv, D)                        # (copies overlap nothing)
+  v, vp, sv = _token_rows(v, T, Hkv, D)
+  for p, (st, sh) in ((kp, sk), (vp, sv)):
+    end = p + 2 * ((T - 1) * st + (Hkv - 1) * sh + D)
+    if T > 0 and not ((end <= k0 or k1 <= p) and (end <= v0 or v1 <= p)):
       raise ValueError(f"{what}: pages overlap k or v")
-  k, kp, sk = _token_rows(k, D)
-  v, vp, sv = _token_rows(v, D)
   a = _lib.paged_write_args(B, Hkv, D, T, k_pages.shape[0], k_pages.shape[1], cols, kp, *sk, vp, *sv, k_pages.data_ptr(), *ks,
                             v_pages.data_ptr(), *vs, cu.data_ptr(), _vp(len_new) or 0, len_k.data_ptr(), table.data_ptr(), ts)
   _launch(_lib.load().sf_hip_paged_write_fwd, k, "sf_hip_paged_write_fwd", C.byref(a))
@@ -1091,7 +1104,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
       raise ValueError(f"{what}: out must be {dtype} {(Tq, H, D)} in 16-byte aligned rows, apart from each other")
     if not (_disjoint(out, q) and _spans_apart(out, k_pages) and _spans_apart(out, v_pages)):
       raise ValueError(f"{what}: out overlaps an input")
-  q, qp, sq = _token_rows(q, D)
+  q, qp, sq = _token_rows(q, Tq, H, D)
   a = _lib.paged_attention_args(B, H, Hkv, D, Tq, P, R, cols, max(max_len, 1) if max_len is not None else 0, scale, bool(causal),
                                 _ELEMENT_TYPES[dtype], qp, *sq, k_pages.data_ptr(), *ks, v_pages.data_ptr(), *vs, out.data_ptr(), *so,
                                 cu_q.data_ptr(), _vp(len_q) or 0, len_k.data_ptr(), table.data_ptr(), ts)
@@ -1134,32 +1147,44 @@ def _microscaled(x, name: str, what: str):
   """Checks codes and scales and returns them as rows: format, rows, K, codes, their stride, scales, their stride."""
   codes, scales = x
   dtype = codes.dtype
-  if (dtype is not _FP8 and dtype is not torch.uint8) or (scales.dtype is not _E8M0 and scales.dtype is not torch.uint8):
+  eight = dtype is _FP8
+  if not (eight or dtype is torch.uint8) or (scales.dtype is not _E8M0 and scales.dtype is not torch.uint8):
     raise ValueError(f"{what}: {name} must have float8_e4m3fn or packed uint8 codes and float8_e8m0fnu or uint8 scales, got "
                      f"{dtype} and {scales.dtype}")
   cs, ss = codes.shape, scales.shape
-  K = cs[-1] if dtype is _FP8 else 2 * cs[-1]
-  if len(cs) < 1 or K < 32 or K % 32 != 0 or ss[:-1] != cs[:-1] or ss[-1] * 32 != K:
+  K = (cs[-1] if eight else 2 * cs[-1]) if cs else 0
+  if K < 32 or K % 32 != 0 or ss[:-1] != cs[:-1] or ss[-1] * 32 != K:
     raise ValueError(f"{what}: {name} needs a scale for each block of 32, got codes {tuple(cs)} and scales {tuple(ss)}")
+  format = _lib.FORMAT_MXFP8 if eight else _lib.FORMAT_MXFP4
+  if codes.is_contiguous() and scales.is_contiguous() and codes.data_ptr() % 16 == 0:
+    return format, scales.numel() // ss[-1], K, codes, cs[-1], scales, ss[-1]
   c2, s2 = codes.reshape(-1, cs[-1]), scales.reshape(-1, ss[-1])
   if c2.stride(1) != 1 or c2.data_ptr() % 16 or (c2.shape[0] > 1 and (c2.stride(0) % 16 or not cs[-1] <= c2.stride(0) < 1 << 23)):
     c2 = torch.empty(c2.shape, dtype=dtype, device=c2.device).copy_(c2)
   if (ss[-1] > 1 and s2.stride(1) != 1) or (s2.shape[0] > 1 and not ss[-1] <= s2.stride(0) < 1 << 23):
     s2 = torch.empty(s2.shape, dtype=scales.dtype, device=s2.device).copy_(s2)
   R = c2.shape[0]
-  return (_lib.FORMAT_MXFP8 if dtype is _FP8 else _lib.FORMAT_MXFP4), R, K, c2, (c2.stride(0) if R > 1 else cs[-1]), s2, \
-      (s2.stride(0) if R > 1 else ss[-1])
+  return format, R, K, c2, (c2.stride(0) if R > 1 else cs[-1]), s2, (s2.stride(0) if R > 1 else ss[-1])
+
+
+def _empty_rows(lead, n: int, dtype: torch.dtype, dev) -> torch.Tensor:
+  """``torch.empty((*lead, n))``, for a matrix in 3/5 of its host time."""
+  if len(lead) == 1:
+    return torch.empty_strided((lead[0], n), (n, 1), dtype=dtype, device=dev)
+  return torch.empty((*lead, n), dtype=dtype, device=dev)
 
 
 def _empty_microscaled(lead, K: int, format: str, dev) -> Microscaled:
-  codes = torch.empty((*lead, K), dtype=_FP8, device=dev) if format == "mxfp8" else torch.empty((*lead, K // 2), dtype=torch.uint8, device=dev)
-  return Microscaled(codes, torch.empty((*lead, K // 32), dtype=_E8M0, device=dev))
+  codes = _empty_rows(lead, K, _FP8, dev) if format == "mxfp8" else _empty_rows(lead, K // 2, torch.uint8, dev)
+  return Microscaled(codes, _empty_rows(lead, K // 32, _E8M0, dev))
 
 
 def _rows2(t: torch.Tensor, aligned: bool):
   """``[R, C]`` rows of ``[..., C]`` with a unit last stride (copied where there is none, or where 16-byte rows are asked for),
   and their stride."""
   Cn = t.shape[-1]
+  if t.ndim == 2 and t.is_contiguous() and not (aligned and t.data_ptr() % 16):
+    return t, Cn
   t2 = t if t.ndim == 2 else t.reshape(-1, Cn)
   if (Cn > 1 and t2.stride(1) != 1) or (aligned and (t2.data_ptr() % 16 or (t2.shape[0] > 1 and t2.stride(0) * t2.element_size() % 16))):
     t2 = torch.empty(t2.shape, dtype=t2.dtype, device=t2.device).copy_(t2)
@@ -1198,7 +1223,7 @@ def mx_dequantize(x: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.
   if dtype not in _ELEMENT_TYPES:
     raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
   format, R, K, codes, c_rs, scales, s_rs = _microscaled(x, "x", what)
-  out = torch.empty((*x.codes.shape[:-1], K), dtype=dtype, device=codes.device)
+  out = _empty_rows(x.codes.shape[:-1], K, dtype, codes.device)
   if R == 0:
     return out
   a = _lib.mx_convert_args(R, K, _ELEMENT_TYPES[dtype], format, out.data_ptr(), K, codes.data_ptr(), c_rs, scales.data_ptr(), s_rs)
@@ -1232,7 +1257,7 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
   if out is None:
     if dtype not in (torch.bfloat16, torch.float16):
       raise ValueError(f"{what}: dtype must be bfloat16 or float16, got {dtype}")
-    y = result = torch.empty(shape, dtype=dtype, device=dev)
+    y = result = _empty_rows(shape[:-1], N, dtype, dev)
     y_rs = N
   else:
     dtype = out.dtype
@@ -1259,6 +1284,35 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
   _launch(lib.sf_hip_mx_linear_fwd, xc, "sf_hip_mx_linear_fwd", ref, _vp(work), need)
   _written(out)
   return result
+
+
+def _norm_outputs(what, x, x2, r2, weight, aligned, out, out_sum):
+  """Checks given outputs of the norm; returns the rows and row strides of both."""
+  shape, dtype, Cn, R = x.shape, x.dtype, x.shape[-1], x2.shape[0]
+  rows = []
+  for o, name in ((out, "out"), (out_sum, "out_sum")):
+    if o is None:
+      rows.append((None, 0))
+      continue
+    if o.shape != shape or o.dtype is not dtype or (Cn > 1 and o.stride(-1) != 1):
+      raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)} with a unit last stride")
+    try:
+      o2 = o if o.ndim == 2 else o.view(-1, Cn)
+    except RuntimeError:
+      raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
+    if R > 1 and o2.stride(0) < Cn:
+      raise ValueError(f"{what}: {name} must hold every element once")
+    if aligned and (o2.data_ptr() % 16 or (R > 1 and o2.stride(0) * o2.element_size() % 16)):
+      raise ValueError(f"{what}: {name} must lie in 16-byte aligned rows with a microscaled output")
+    same = lambda i: o2.data_ptr() == i.data_ptr() and (R <= 1 or o2.stride(0) == i.stride(0))
+    if not all(same(i) or _disjoint(o2.unsqueeze(1), i.unsqueeze(1)) for i in (x2, r2) if i is not None):
+      raise ValueError(f"{what}: outputs may be x or residual itself, and overlap nothing else")
+    if weight is not None and not _spans_apart(o2, weight):
+      raise ValueError(f"{what}: an output overlaps the weight")
+    rows.append((o2, o2.stride(0) if R > 1 else Cn))
+  if out is not None and out_sum is not None and not _disjoint(rows[0][0].unsqueeze(1), rows[1][0].unsqueeze(1)):
+    raise ValueError(f"{what}: out and out_sum overlap")
+  return rows
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, *, eps: float = 1e-6,
@@ -1299,45 +1353,19 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
   x2, x_rs = _rows2(x, aligned)
   R = x2.shape[0]
   r2, r_rs = (None, 0) if residual is None else _rows2(residual, aligned)
-
-  def given(o, name):
-    if o.shape != shape or o.dtype is not dtype or (Cn > 1 and o.stride(-1) != 1):
-      raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)} with a unit last stride")
-    try:
-      o2 = o if o.ndim == 2 else o.view(-1, Cn)
-    except RuntimeError:
-      raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
-    if R > 1 and o2.stride(0) < Cn:
-      raise ValueError(f"{what}: {name} must hold every element once")
-    if aligned and (o2.data_ptr() % 16 or (R > 1 and o2.stride(0) * o2.element_size() % 16)):
-      raise ValueError(f"{what}: {name} must lie in 16-byte aligned rows with a microscaled output")
-    return o2, (o2.stride(0) if R > 1 else Cn)
-
-  y2, y_rs, h2, h_rs, result, total = None, 0, None, 0, None, None
-  if out is not None:
-    result = out
-    y2, y_rs = given(out, "out")
-  if out_sum is not None:
-    total = out_sum
-    h2, h_rs = given(out_sum, "out_sum")
+  y2, y_rs, h2, h_rs, total, codes = out, 0, None, 0, None, None
   if out is not None or out_sum is not None:
-    same = lambda a, b: a.data_ptr() == b.data_ptr() and (R <= 1 or a.stride(0) == b.stride(0))
-    three = lambda t: t.view(R, 1, Cn) if t.is_contiguous() else t.unsqueeze(1)
-    for o in (y2, h2):
-      if o is not None and not all(same(o, i) or _disjoint(three(o), three(i)) for i in (x2, r2) if i is not None):
-        raise ValueError(f"{what}: outputs may be x or residual itself, and overlap nothing else")
-      if o is not None and weight is not None and not _spans_apart(o, weight):
-        raise ValueError(f"{what}: an output overlaps the weight")
-    if y2 is not None and h2 is not None and not _disjoint(three(y2), three(h2)):
-      raise ValueError(f"{what}: out and out_sum overlap")
-  codes = None
+    (y2, y_rs), (h2, h_rs) = _norm_outputs(what, x, x2, r2, weight, aligned, out, out_sum)
+    total = out_sum
   if output is not None:
     result = codes = _empty_microscaled(shape[:-1], Cn, output, dev)
   elif out is None:
-    result = y2 = torch.empty(shape, dtype=dtype, device=dev)
+    result = y2 = _fresh(x)
     y_rs = Cn
+  else:
+    result = out
   if residual is not None and out_sum is None:
-    total = h2 = torch.empty(shape, dtype=dtype, device=dev)
+    total = h2 = _fresh(x)
     h_rs = Cn
   if R == 0:
     return result, total
