@@ -382,11 +382,15 @@ __device__ __forceinline__ void note_tile(const PackedPlan& pl, int slot, bool t
   pl.found[2 * slot + 1] = there ? int4{s.k0, first, slices, 0} : int4{0, 0, 0, 0};
 }
 
+// Whether packed_tile_kernel's slices may be dealt out by the keys too (its rule is in route()).
+template <class A>
+constexpr bool kShareTiles = std::is_same<A, PagedArgs>::value;
+
 // Slice `item` of all, where the tiles of up to 64 N sequences (N a lane) share pl.share slices by their keys, in
 // slices of c units of `unit` keys: the smallest c that needs no more than the share, one slice a tile aside.  c is at
 // least all units / share, which needs share + tiles at most (the launch's bound), and at most all units / (share - tiles).
 // False past the last; `slot` is the tile's number among all, past the last slice one that no tile has.
-template <int N, class A>
+template <int R, int N, class A>
 __device__ __forceinline__ bool find_slice(const A& a, const PackedPlan& pl, int unit, int item, Seq& s, int& tile,
                                            int& slot, int& slice, int& slices) {
   const int lane = threadIdx.x & 63;
@@ -400,7 +404,7 @@ __device__ __forceinline__ bool find_slice(const A& a, const PackedPlan& pl, int
       seq_range(a.cu_q, a.len_q, b, a.Tq, start[j], n[j]);
       key_range(a, b, k0[j], lk[j]);
     }
-    nt[j] = (int)(((uint32_t)n[j] * (uint32_t)pl.G + 31) / 32);
+    nt[j] = (int)(((uint32_t)n[j] * (uint32_t)pl.G + R - 1) / R);
     units[j] = (lk[j] + unit - 1) / unit;
     own_tiles += nt[j];
     own_units += (float)nt[j] * (float)units[j];
@@ -858,8 +862,8 @@ struct KeyOperand<sf_packed_attention_args, KC, NB> {
     D = a.D;
     lk = s.lk;
   }
-  __device__ __forceinline__ void fetch(int) {}
-  __device__ __forceinline__ void load(int j0, bool there) {
+  template <class P>
+  __device__ __forceinline__ void load(const P&, int j0, bool there) {
     const int half = (threadIdx.x >> 5) & 1;
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(base + j0 * row, there ? (min(32 * NB, lk - j0) - 1) * row + D * 2 : 0);
     uint32_t o = off, oh = half ? kOutside : off;            // steps that both halves have, that the first has
@@ -872,42 +876,39 @@ struct KeyOperand<sf_packed_attention_args, KC, NB> {
             r, (int)((16 * kk + 8 < D ? o : 16 * kk < D ? oh : kOutside) + kb * 32 * (uint32_t)row + 32 * kk), 0, 0));
   }
 };
-// Of a paged cache: a lane's row has its own page, found a tile ahead.  Rows past the sequence read its last key's (they are
-// hidden), rows of a page that does not exist zeros.
+// Of a paged cache: 16 rows have one page, 32 lanes two of them, found a tile ahead with those of V.  Rows past the sequence read
+// what their page holds (they are hidden), rows of a page that does not exist zeros.
 template <int KC, int NB>
 struct KeyOperand<PagedArgs, KC, NB> {
-  const PagedArgs& a;
-  const int32_t* table;
   const char* base;
-  PageDiv div;
-  int lk, id[NB], row[NB];                                   // of the next tile
+  int64_t page;
+  uint32_t line, off;
+  int D, pages;
   u32x4 f[NB][KC];
   // chunks that are whole for every D of this KC
   static constexpr int kWhole = (KC == 2 ? 8 : KC == 3 ? 40 : KC == 4 ? 56 : KC == 6 ? 72 : 104) / 16;
-  __device__ __forceinline__ KeyOperand(const PagedArgs& args, const Seq& s, int hk)
-      : a(args), table(args.table + s.k0 * args.table_s), base((const char*)((const uint16_t*)args.k + hk * args.k_s[2])),
-        div(args.div), lk(s.lk) {}
-  __device__ __forceinline__ void fetch(int j0) {
-    const int li = threadIdx.x & 31;
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
-      const int j = min(max(j0, 0) + 32 * kb + li, lk - 1), page = page_of(div, j >> 4);
-      id[kb] = table[page];
-      row[kb] = j - page * a.page_rows;
-    }
-  }
-  __device__ __forceinline__ void load(int, bool there) {
+  __device__ __forceinline__ KeyOperand(const PagedArgs& a, const Seq&, int hk)
+      : base((const char*)((const uint16_t*)a.k + hk * a.k_s[2])), page(a.k_s[0] * 2), line((uint32_t)a.k_s[1] * 2),
+        off((threadIdx.x & 15) * ((uint32_t)a.k_s[1] * 2)), D(a.D), pages((int)a.pages) {}
+  __device__ __forceinline__ void load(const Pages<PagedArgs, 32 * NB, 64>& p, int, bool there) {
     const int half = (threadIdx.x >> 5) & 1;
+    const bool second = threadIdx.x & 16;
     if (!there) return;                                      // (uniform; what the registers hold is not used)
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
-      const bool exists = (uint32_t)id[kb] < (uint32_t)a.pages;
-      const char* p = exists ? base + ((int64_t)id[kb] * a.k_s[0] + (int64_t)row[kb] * a.k_s[1]) * 2 : reinterpret_cast<const char*>(kZeros);
+      uint64_t at[2];
+      uint32_t rows[2];
 #pragma unroll
-      for (int kk = 0; kk < KC; ++kk) {
-        const int d0 = 16 * kk + 8 * half;
-        f[kb][kk] = ld16(kk < kWhole || d0 < a.D ? p + 2 * d0 : reinterpret_cast<const char*>(kZeros));
+      for (int x = 0; x < 2; ++x) {
+        const int id = p.id[2 * kb + x];
+        const bool exists = (uint32_t)id < (uint32_t)pages;
+        at[x] = (uint64_t)(uintptr_t)(exists ? base + id * page + (uint64_t)(uint32_t)p.row[2 * kb + x] * line : reinterpret_cast<const char*>(kZeros));
+        rows[x] = exists ? 0xffffffffu : 0u;
       }
+      const char* const q = reinterpret_cast<const char*>((uintptr_t)(second ? at[1] : at[0])) + ((off & (second ? rows[1] : rows[0])) + 16 * half);
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk)
+        f[kb][kk] = ld16(kk < kWhole || 16 * kk + 8 * half < D ? q + 32 * kk : reinterpret_cast<const char*>(kZeros));
     }
   }
 };
@@ -923,7 +924,7 @@ struct KeyOperand<PagedArgs, KC, NB> {
 // 32 / 8 heads of 128, causal, bf16: 1.83 to 2.03 ms from card to card, 1.20 to 1.08 PFLOP/s (bf16 products of 8192^3:
 // 1.2 to 1.4), of 4096 134 to 143 us; 1.52 ms where all inputs are zero, which draw less power.  8192 tokens, 16
 // heads of 64: 168 to 177 us, 0.82 to 0.78 PFLOP/s.
-template <class A, class E, int KC, int NW, int KG>
+template <class A, class E, int KC, int NW, int KG, bool SHARE = false>
 __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const A a, const PackedPlan pl) {
   using T = Dims<KC>;
   constexpr int kTile = 64 * T::kRow, R = 32 * NW;
@@ -933,26 +934,32 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const A a,
   uint8_t* const smem = shared + group * 4 * kTile;
   // the key heads of one tile are neighbours, so that with 8 of them each XCD keeps to its own K and V
   const int block = workgroup(), hk = block % a.Hkv, rest = block / a.Hkv;
-  const int slice = rest % pl.slices, idx = rest / pl.slices;
+  int slice = rest % pl.slices, slices = pl.slices;
+  const int idx = rest / pl.slices;
   Seq s;
   int tile, ntiles;
   bool there;
   // The rows with the most keys first, so that the last workgroups to start are short (8 prompts of 1 to 2048, 16 heads
   // of 64: 42 us, sequence by sequence 47; 10 proteins of 20 to 1024, 16 heads of 48: 24.8 / 26.9).  Of more than
   // 64 sequences there are enough workgroups after any of them.
-  if (a.B > 1 && a.B <= 64) {
+  if constexpr (SHARE) {
+    int slot;
+    there = a.B <= 64 ? find_slice<R, 1>(a, pl, 64 * KG, idx, s, tile, slot, slice, slices)
+                      : find_slice<R, 4>(a, pl, 64 * KG, idx, s, tile, slot, slice, slices);
+    if (hk + (int)threadIdx.x == 0 && slot < pl.tiles && (!there || slice == 0)) note_tile(pl, slot, there && slices > 1, s, tile, idx, slices);
+  } else if (a.B > 1 && a.B <= 64) {                           // (SHARE is a kernel of its own: its code here slowed the other by 5%)
     there = find_longest<R>(a, pl, idx, s, tile);
   } else {
     there = find_tile<R>(a, pl, idx, s, tile, ntiles);
     tile = ntiles - 1 - tile;
   }
-  if (pl.slices > 1 && hk + slice + (int)threadIdx.x == 0) note_tile(pl, idx, there, s, tile, idx * pl.slices, pl.slices);
+  if (!SHARE && pl.slices > 1 && hk + slice + (int)threadIdx.x == 0) note_tile(pl, idx, there, s, tile, idx * pl.slices, pl.slices);
   if (!there) return;
   const int rows = s.lq * pl.G, r0 = tile * R + wave * 32;
   const int row = min(r0 + li, rows - 1);                    // rows past the end repeat the last
   const int seen = last_key(s, a.causal, min(tile * R + R, rows) - 1, pl) + 1;   // keys the workgroup's last row sees
   const int n_all = (seen + 63) / 64;
-  const int per = (n_all + pl.slices - 1) / pl.slices, t_lo = min(slice * per, n_all), t_hi = min(t_lo + per, n_all);
+  const int per = (n_all + slices - 1) / slices, t_lo = min(slice * per, n_all), t_hi = min(t_lo + per, n_all);
 
   RowState<E, KC> st;
   st.init(a, pl, s, row, hk);
@@ -1049,7 +1056,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void packed_tile_kernel(const A a,
   }
   if (r0 >= rows || group > 0) return;                       // (no barrier from here on)
   const float l = st.l + __shfl_xor(st.l, 32);
-  if (pl.slices > 1) {
+  if (slices > 1) {
     float* po = pl.part + (int64_t)block * R * (T::DP + 2);
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
@@ -1098,8 +1105,8 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const A a, const 
   int tile, slice, slices;
   if (pl.share > 0) {
     int slot;
-    const bool there = a.B <= 64 ? find_slice<1>(a, pl, 4 * KT, item, s, tile, slot, slice, slices)
-                                 : find_slice<4>(a, pl, 4 * KT, item, s, tile, slot, slice, slices);
+    const bool there = a.B <= 64 ? find_slice<32, 1>(a, pl, 4 * KT, item, s, tile, slot, slice, slices)
+                                 : find_slice<32, 4>(a, pl, 4 * KT, item, s, tile, slot, slice, slices);
     if (hk + tid == 0 && slot < pl.tiles && (!there || slice == 0)) note_tile(pl, slot, there && slices > 1, s, tile, item, slices);
     if (!there) return;
   } else {
@@ -1124,11 +1131,9 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const A a, const 
       Stage<A, KC, KT, 64> vs;
       Pages<A, KT, 64> pages(a, s, 0);
       vs.init(a, a.v, a.v_s, s, hk, lane);
-      kf.fetch(KT * (t_hi - 1));
       pages.fetch(KT * (t_hi - 1));
-      kf.load(KT * (t_hi - 1), true);
+      kf.load(pages, KT * (t_hi - 1), true);
       vs.load(pages, KT * (t_hi - 1), s.lk, true);
-      kf.fetch(KT * (t_hi - 2));
       pages.fetch(KT * (t_hi - 2));
       const int hidden = a.causal ? max(t_lo, (low + 1) / KT) : -1;          // last of the tiles that some rows do not see to their end
       for (int t = t_hi - 1; t >= t_lo; --t) {
@@ -1141,9 +1146,8 @@ __global__ __launch_bounds__(256, 2) void packed_stream_kernel(const A a, const 
           for (int kk = 0; kk < KC; ++kk) sc[kb] = E::mfma(kf.f[kb][kk], st.q[kk], sc[kb]);
         }
         vs.template store<true>(vt, lane);
-        kf.load(KT * (t - 1), t > t_lo);
+        kf.load(pages, KT * (t - 1), t > t_lo);
         vs.load(pages, KT * (t - 1), s.lk, t > t_lo);
-        kf.fetch(KT * (t - 2));
         pages.fetch(KT * (t - 2));
         if (KT * t + KT - 1 > low) st.template hide<NB>(sc, mine - KT * t);
         uint32_t p[8 * NB];
@@ -1369,6 +1373,14 @@ int route(const A* a, int64_t keys, Route& r, const char* what) {
     if (slices > most) slices = most;
     if (slices < 3 && seen < 2048) slices = 1;
     slices = slices < 1 ? 1 : slices > 64 ? 64 : slices;
+    // A step that takes tokens of some sequences along with a piece of another: as many slices for each would leave most
+    // workgroups with little to do, so they are dealt out by the keys, a workgroup a CU.
+    if (kShareTiles<A> && r.nw == 4 && a->B > 1 && a->B <= kShared && !triangle && wgs < 256 && seen >= 1024) {
+      r.groups = 2;
+      slices = 1;
+      share = 256 / a->Hkv;
+      if (share < 1) share = 0;
+    }
   } else {
     const int64_t least = r.dp > 64 ? 128 : 256;
     // Slices dealt out by the keys, a workgroup a CU or the next multiple of that (one token for 4 caches of 128 to 8192
@@ -1414,6 +1426,8 @@ int launch(const A* a, const Route& r, hipStream_t st) {
   }
   if (r.nw == 0) {
     hipLaunchKernelGGL((packed_stream_kernel<A, E, KC>), grid, dim3(256), 0, st, *a, r.pl);
+  } else if (r.nw == 4 && r.pl.share > 0) {
+    if constexpr (kShareTiles<A>) hipLaunchKernelGGL((packed_tile_kernel<A, E, KC, 4, 2, true>), grid, dim3(512), 0, st, *a, r.pl);
   } else if (r.nw == 4) {
     if (r.groups == 2) hipLaunchKernelGGL((packed_tile_kernel<A, E, KC, 4, 2>), grid, dim3(512), 0, st, *a, r.pl);
     else hipLaunchKernelGGL((packed_tile_kernel<A, E, KC, 4, 1>), grid, dim3(256), 0, st, *a, r.pl);
