@@ -87,7 +87,7 @@ __device__ __forceinline__ void put(const sf_mx_linear_args& a, bool vector, int
   if (vector && n + C <= a.N) {
     if constexpr (C == 8) {
       st16(y, E::pack(v));
-    } else {
+    } else if constexpr (C == 4) {
       const float w[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
       const u32x4 p = E::pack(w);
       *reinterpret_cast<u32x2*>(y) = u32x2{p[0], p[1]};
@@ -100,77 +100,92 @@ __device__ __forceinline__ void put(const sf_mx_linear_args& a, bool vector, int
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows of x.  A wave's step is 512 k, four instructions: instruction s takes the blocks 4 g + s as its blocks g, so that a
-// lane's scales of all four are one word and a row's 4-bit codes of a lane 64 consecutive bytes.
+// Few rows of x.  A wave's step is 512 k, four instructions.  An instruction's loads take 64 consecutive bytes of each of 16 rows
+// (lanes that each read on along their own 64 bytes would touch four times the lines).
 // ---------------------------------------------------------------------------------------
-template <class F>
-struct Step512 {
+template <class F, int SI>
+struct StepOperand {
   using O = Op<F>;
-  u32x4 c[4][O::kParts];
-  uint32_t scale;
+  u32x4 c[SI][O::kParts];
+  uint32_t scale[SI];                                        // of instruction s: byte 0
   // row: byte offset of the lane's row of codes, srow of scales; blocks: of the row
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rc, __amdgpu_buffer_rsrc_t rs, uint32_t row, uint32_t srow, int b0, int blocks,
                                        bool wide) {
     const int g = (threadIdx.x >> 4) & 3;
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < SI; ++s)
 #pragma unroll
       for (int p = 0; p < O::kParts; ++p) {
-        const int b = b0 + (O::k8 ? 4 * (g / 2 + 2 * p) : 4 * g) + s;
-        c[s][p] = load16(rc, b < blocks ? row + b * O::kBlock + (O::k8 ? 16 * (g & 1) : 0) : kOutside);
+        const int at = 4 * O::kBlock * s + 64 * p + 16 * g;  // bytes from the step's first
+        c[s][p] = load16(rc, b0 + at / O::kBlock < blocks ? row + b0 * O::kBlock + at : kOutside);
       }
-    scale = scales4(rs, srow, b0 + 4 * g, blocks - b0 - 4 * g, wide);
+    if (SI == 4 && wide && b0 + 16 <= blocks) {              // (uniform)
+      const u32x4 w = load16(rs, srow + b0);
+#pragma unroll
+      for (int s = 0; s < SI; ++s) scale[s] = w[s];
+    } else {
+#pragma unroll
+      for (int s = 0; s < SI; ++s) scale[s] = scales4(rs, srow, b0 + 4 * s, blocks - b0 - 4 * s, wide);
+    }
+#pragma unroll
+    for (int s = 0; s < SI; ++s) scale[s] >>= 8 * g;
   }
 };
 
-template <class E, class FX, class FW, int MT, int KW>
+// NT times 16 rows of w and MT times 16 of x a workgroup, whose KW waves take steps of SI instructions in turns.
+template <class E, class FX, class FW, int MT, int NT, int SI, int KW>
 __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_args a, const Extra ex) {
-  __shared__ f32x4 sums[KW][MT][64];
+  static_assert(MT * NT <= KW, "a wave for each 16 x 16 results");
+  __shared__ f32x4 sums[KW][MT * NT][64];
   const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16;
-  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-  const int blocks = a.K / 32, wrows = min(16, a.N - n0);
-  const int64_t mrows = a.M - m0 < 16 * MT ? a.M - m0 : 16 * MT;
+  const int n0 = blockIdx.x * (16 * NT);
+  const int blocks = a.K / 32, wrows = min(16 * NT, a.N - n0), mrows = (int)a.M;
   const __amdgpu_buffer_rsrc_t wc = rsrc((const uint8_t*)a.w + n0 * a.w_rs, (wrows - 1) * a.w_rs + (int64_t)blocks * Op<FW>::kBlock),
                                ws = rsrc((const uint8_t*)a.w_scales + n0 * a.ws_rs, (wrows - 1) * a.ws_rs + blocks),
-                               xc = rsrc((const uint8_t*)a.x + m0 * a.x_rs, (mrows - 1) * a.x_rs + (int64_t)blocks * Op<FX>::kBlock),
-                               xs = rsrc((const uint8_t*)a.x_scales + m0 * a.xs_rs, (mrows - 1) * a.xs_rs + blocks);
+                               xc = rsrc(a.x, (mrows - 1) * a.x_rs + (int64_t)blocks * Op<FX>::kBlock),
+                               xs = rsrc(a.x_scales, (mrows - 1) * a.xs_rs + blocks);
   // (rows past the end repeat the last: their results are not stored)
-  const uint32_t wrow = (uint32_t)(min(li, wrows - 1) * a.w_rs), wsrow = (uint32_t)(min(li, wrows - 1) * a.ws_rs);
-  f32x4v acc[MT];
+  f32x4v acc[NT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
-  for (int b0 = 16 * wave; b0 < blocks; b0 += 16 * KW) {
-    Step512<FW> w;
-    Step512<FX> x[MT];
-    w.load(wc, ws, wrow, wsrow, b0, blocks, ex.wide);
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[i][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  for (int b0 = 4 * SI * wave; b0 < blocks; b0 += 4 * SI * KW) {
+    StepOperand<FW, SI> w[NT];
+    StepOperand<FX, SI> x[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int row = min(16 * i + li, wrows - 1);
+      w[i].load(wc, ws, (uint32_t)(row * a.w_rs), (uint32_t)(row * a.ws_rs), b0, blocks, ex.wide);
+    }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int row = (int)min((int64_t)(16 * t + li), mrows - 1);
+      const int row = min(16 * t + li, mrows - 1);
       x[t].load(xc, xs, (uint32_t)(row * a.x_rs), (uint32_t)(row * a.xs_rs), b0, blocks, ex.wide);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      acc[t] = mfma16s<FW, FX, 0, 0>(operand<FW>(w.c[0]), operand<FX>(x[t].c[0]), acc[t], w.scale, x[t].scale);
-      acc[t] = mfma16s<FW, FX, 1, 1>(operand<FW>(w.c[1]), operand<FX>(x[t].c[1]), acc[t], w.scale, x[t].scale);
-      acc[t] = mfma16s<FW, FX, 2, 2>(operand<FW>(w.c[2]), operand<FX>(x[t].c[2]), acc[t], w.scale, x[t].scale);
-      acc[t] = mfma16s<FW, FX, 3, 3>(operand<FW>(w.c[3]), operand<FX>(x[t].c[3]), acc[t], w.scale, x[t].scale);
-    }
+    for (int s = 0; s < SI; ++s)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          acc[i][t] = mfma16s<FW, FX, 0, 0>(operand<FW>(w[i].c[s]), operand<FX>(x[t].c[s]), acc[i][t], w[i].scale[s], x[t].scale[s]);
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) sums[wave][t][lane] = f32x4{acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sums[wave][i * MT + t][lane] = f32x4{acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
   __syncthreads();
-  // waves 0 .. MT - 1 (KW >= MT) finish 16 rows of x each: lane (row li, columns 4 g ..)
-  if (wave >= MT) return;
+  // waves 0 .. MT NT - 1 finish 16 x 16 results each: lane (row li, columns 4 g ..)
+  if (wave >= MT * NT) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < KW; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += sums[k][wave][lane][e];
-  const int64_t m = m0 + 16 * wave + li;
-  const int n = n0 + 4 * g;
-  if (m >= a.M) return;
+  const int m = 16 * (wave % MT) + li, n = n0 + 16 * (wave / MT) + 4 * g;
+  if (m >= mrows) return;
   if (a.bias != nullptr) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += n + e < a.N ? a.bias[n + e] : 0.f;
@@ -181,13 +196,16 @@ __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_a
 // ---------------------------------------------------------------------------------------
 // Tiles of 128 x 128, waves of 64 x 64, steps of 128 k through two LDS buffers.
 // ---------------------------------------------------------------------------------------
-template <class F>
+// WIDE: scales load as words, and two steps are in flight; else byte by byte and one step ahead (registers).
+template <class F, bool WIDE>
 struct TileOperand {
   using O = Op<F>;
   static constexpr int kRow = 4 * O::kBlock, kPieces = kRow / 16, kBytes = 128 * kRow, kN = kBytes / 16 / 256;
   // the 16 rows that are read together fall on 16 different 16-byte slots of the banks' 256 bytes
   static __device__ __forceinline__ int slot(int row, int piece) { return O::k8 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
-  u32x4 data[kN];
+  static constexpr int kAhead = WIDE ? 2 : 1;                // steps in flight
+  u32x4 data[kAhead][kN];
+  uint32_t sdata[kAhead][2];
   __amdgpu_buffer_rsrc_t r, rs;
   uint32_t off[kN], srow[2];
   __device__ __forceinline__ void init(const void* codes, int64_t c_rs, const void* scales, int64_t s_rs, int64_t row0, int64_t rows, int blocks,
@@ -203,19 +221,24 @@ struct TileOperand {
 #pragma unroll
     for (int t = 0; t < 2; ++t) srow[t] = (uint32_t)(min((int64_t)(wave_row + 32 * t + (threadIdx.x & 31)), n - 1) * s_rs);
   }
+  // step `step` into slot D, zeros past the last
+  template <int D>
   __device__ __forceinline__ void load(int step, int blocks) {
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
       const int piece = (u * 256 + threadIdx.x) % kPieces;
       const bool in = 4 * step + piece * 16 / O::kBlock < blocks;
-      data[u] = load16(r, in ? off[u] + step * kRow : kOutside);
+      data[D][u] = load16(r, in ? off[u] + step * kRow : kOutside);
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sdata[D][t] = scales4(rs, srow[t], 4 * step, blocks - 4 * step, WIDE);
   }
+  template <int D>
   __device__ __forceinline__ void store(uint8_t* lds) const {
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
       const int idx = u * 256 + threadIdx.x, row = idx / kPieces;
-      st16(lds + row * kRow + (slot(row, idx % kPieces) << 4), data[u]);
+      st16(lds + row * kRow + (slot(row, idx % kPieces) << 4), data[D][u]);
     }
   }
   // codes of chunk ch (64 k) of rows wave_row + li
@@ -227,22 +250,19 @@ struct TileOperand {
       p[q] = ld16(lds + row * kRow + (slot(row, (O::k8 ? 4 * ch + 2 * q : 2 * ch) + half) << 4));
     return operand<F>(p);
   }
-  __device__ __forceinline__ void scales(int step, int blocks, bool wide, uint32_t (&s)[2]) const {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) s[t] = scales4(rs, srow[t], 4 * step, blocks - 4 * step, wide);
-  }
 };
 
-template <class E, class FX, class FW>
+template <class E, class FX, class FW, bool WIDE>
 __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args a, const Extra ex) {
-  using X = TileOperand<FX>;
-  using W = TileOperand<FW>;
+  using X = TileOperand<FX, WIDE>;
+  using W = TileOperand<FW, WIDE>;
+  constexpr int kAhead = X::kAhead;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * (X::kBytes + W::kBytes)];
   const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
   const int n0 = blockIdx.x * 128;
   const int64_t m0 = (int64_t)blockIdx.y * 128;
-  const int blocks = a.K / 32, s0 = blockIdx.z * ex.steps, s1 = min(s0 + ex.steps, (blocks + 3) / 4);
+  const int blocks = a.K / 32, s0 = blockIdx.z * ex.steps, s1 = min(s0 + ex.steps, (blocks + 3) / 4), last = min(blocks, 4 * s1);
   X x;
   W w;
   x.init(a.x, a.x_rs, a.x_scales, a.xs_rs, m0, a.M, blocks, 64 * wm);
@@ -254,31 +274,24 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  uint32_t sx[2], sw[2];
-  if (s0 < s1) {
-    x.load(s0, blocks);
-    w.load(s0, blocks);
-    x.scales(s0, blocks, ex.wide, sx);
-    w.scales(s0, blocks, ex.wide, sw);
-  }
-  for (int s = s0, buf = 0; s < s1; ++s, buf ^= 1) {
-    uint8_t* const xt = smem + buf * (X::kBytes + W::kBytes);
+  // Step s is stored to one of two LDS buffers while the next kAhead steps are in flight to registers: one barrier a step (the
+  // buffer's readers, two steps before, passed the last one).
+  const auto step = [&](auto constant, int s) __attribute__((always_inline)) {
+    constexpr int D = decltype(constant)::value;
+    uint8_t* const xt = smem + (s & 1) * (X::kBytes + W::kBytes);
     uint8_t* const wt = xt + X::kBytes;
-    x.store(xt);
-    w.store(wt);
+    x.template store<D>(xt);
+    w.template store<D>(wt);
     uint32_t cx[2], cw[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      cx[t] = sx[t] >> (8 * half);                           // chunk 0: byte 0, chunk 1: byte 2
-      cw[t] = sw[t] >> (8 * half);
+      cx[t] = x.sdata[D][t] >> (8 * half);                   // chunk 0: byte 0, chunk 1: byte 2
+      cw[t] = w.sdata[D][t] >> (8 * half);
     }
-    lds_only_barrier();                                      // (the other buffer's readers passed the last one)
-    if (s + 1 < s1) {
-      x.load(s + 1, blocks);
-      w.load(s + 1, blocks);
-      x.scales(s + 1, blocks, ex.wide, sx);
-      w.scales(s + 1, blocks, ex.wide, sw);
-    }
+    lds_only_barrier();
+    x.template load<D>(s + kAhead, last);                    // (zeros past the slice's end)
+    w.template load<D>(s + kAhead, last);
+    __builtin_amdgcn_sched_barrier(0);                       // (moved behind the products, the loads were waited for at once)
     i32x8 wo[2][2], xo[2][2];
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch)
@@ -295,57 +308,135 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc[i][j] = mfma32s<FW, FX, 2, 2>(wo[1][i], xo[1][j], acc[i][j], cw[i], cx[j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  x.template load<0>(s0, last);
+  w.template load<0>(s0, last);
+  if constexpr (WIDE) {
+    x.template load<1>(s0 + 1, last);
+    w.template load<1>(s0 + 1, last);
+    for (int s = s0; s < s1; s += 2) {                       // (a step too many adds zeros)
+      step(std::integral_constant<int, 0>{}, s);
+      step(std::integral_constant<int, 1>{}, s + 1);
+    }
+  } else {
+    for (int s = s0; s < s1; ++s) step(std::integral_constant<int, 0>{}, s);
   }
   // (the products' lanes all take part: no part of them is moved into the branches below)
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) asm volatile("" : "+v"(acc[i][j]));
-  // lane (row li of x, half): columns 8 (e / 4) + 4 half + e % 4
+  // Results go through LDS so that whole lines are stored (straight from the registers, 32 bytes of each of 32 rows an
+  // instruction, 33 MB of parts took 15 us).  A lane (row li of x, half) has columns 8 c + 4 half .. + 3.
+  if (ex.slices > 1) {
+    constexpr int kLine = 512;                               // 128 columns of a row; pieces of 16 bytes XORed by the row
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {                   // rows 64 pass .. + 63
+      lds_only_barrier();
+      if (wm == pass) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t m = m0 + 64 * wm + 32 * j + li;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = n0 + 64 * wn + 32 * i + 8 * c + 4 * half;
-        float v[4];
+            for (int c = 0; c < 4; ++c) {
+              const int row = 32 * j + li, piece = 16 * wn + 8 * i + 2 * c + half;
+              const f32x16v& v = acc[i][j];
+              *reinterpret_cast<f32x4*>(smem + row * kLine + ((piece ^ (row & 31)) << 4)) = f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+            }
+      }
+      lds_only_barrier();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * c + e];
+      for (int u = 0; u < 8; ++u) {
+        const int idx = u * 256 + threadIdx.x, row = idx >> 5, piece = idx & 31, n = n0 + 4 * piece;
+        const int64_t m = m0 + 64 * pass + row;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(smem + row * kLine + ((piece ^ (row & 31)) << 4));
         if (m >= a.M) continue;
-        if (ex.slices > 1) {
-          float* const p = ex.part + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
+        float* const p = ex.part + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
+        if (a.N % 4 == 0) {
+          if (n < a.N) *reinterpret_cast<f32x4*>(p) = v;
+        } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (n + e < a.N) p[e] = v[e];
-          continue;
         }
-        if (a.bias != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += n + e < a.N ? a.bias[n + e] : 0.f;
-        }
-        put<E, 4>(a, ex.vector, m, n, v);
       }
+    }
+    return;
+  }
+  constexpr int kLine = 256;
+  lds_only_barrier();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = 64 * wn + 32 * i + 8 * c + 4 * half;
+      float b[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = a.bias[min(n0 + col + e, a.N - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 64 * wm + 32 * j + li;
+        const f32x16v& v = acc[i][j];
+        const float w8[8] = {v[4 * c] + b[0], v[4 * c + 1] + b[1], v[4 * c + 2] + b[2], v[4 * c + 3] + b[3], 0.f, 0.f, 0.f, 0.f};
+        const u32x4 q = E::pack(w8);
+        *reinterpret_cast<u32x2*>(smem + row * kLine + (((col >> 3) ^ (row & 15)) << 4) + 8 * half) = u32x2{q[0], q[1]};
+      }
+    }
+  lds_only_barrier();
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int idx = u * 256 + threadIdx.x, row = idx >> 4, piece = idx & 15, n = n0 + 8 * piece;
+    const int64_t m = m0 + row;
+    const u32x4 q = ld16(smem + row * kLine + ((piece ^ (row & 15)) << 4));
+    if (m >= a.M) continue;
+    uint16_t* const y = (uint16_t*)a.y + m * a.y_rs + n;
+    if (ex.vector && n + 8 <= a.N) {
+      st16(y, q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t w2 = q[e / 2];
+        if (n + e < a.N) y[e] = (uint16_t)(e & 1 ? w2 >> 16 : w2);
+      }
+    }
   }
 }
 
-// Sums the slices of a split k: one element a thread.
-template <class E>
+// Sums the slices of a split k: 4 neighbours a thread where rows are whole fours (V), else one.
+template <class E, int V>
 __global__ __launch_bounds__(256) void mx_join_kernel(const sf_mx_linear_args a, const Extra ex) {
-  const int64_t all = a.M * a.N;
+  typedef __attribute__((__vector_size__(V * sizeof(float)))) float fv;
+  const uint32_t per = (uint32_t)a.N / V;
+  const int64_t all = a.M * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / a.N;
-    const int n = (int)(i - m * a.N);
-    float v = 0.f;
-    for (int s = 0; s < ex.slices; ++s) v += ex.part[s * all + i];
-    if (a.bias != nullptr) v += a.bias[n];
-    E::store((typename E::T*)a.y + m * a.y_rs + n, v);
+    const int64_t m = i / per;
+    const int n = V * (int)(i - m * per);
+    const fv* p = reinterpret_cast<const fv*>(ex.part) + i;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = a.bias != nullptr ? a.bias[n + e] : 0.f;
+    for (int s = 0; s < ex.slices; s += 4) {                 // (four loads in flight)
+      fv q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q[u] = p[(int64_t)min(s + u, ex.slices - 1) * all];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += s + u < ex.slices ? q[u][e] : 0.f;
+    }
+    put<E, V>(a, V == 4 && ex.vector, m, n, v);
   }
 }
 
 // ---------------------------------------------------------------------------------------
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// From more rows of w on a workgroup takes 32 of them.
+constexpr int kWideRows = 6144;
 
 struct Route {
   bool stream, large;
@@ -383,7 +474,7 @@ void route(const sf_mx_linear_args* a, Route& r) {
   const int64_t tiles = ((a->M + 127) / 128) * ((a->N + 127) / 128);
   const int steps = (a->K / 32 + 3) / 4;
   int64_t slices = 1;
-  if (!r.stream && !r.large) slices = std::max<int64_t>(1, std::min<int64_t>(256 / tiles, steps / 8));
+  if (!r.stream && !r.large) slices = std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / 4));
   r.ex.steps = (int)((steps + slices - 1) / slices);
   r.ex.slices = (steps + r.ex.steps - 1) / r.ex.steps;
 }
@@ -391,11 +482,14 @@ void route(const sf_mx_linear_args* a, Route& r) {
 template <class E, class FX, class FW>
 int launch(const sf_mx_linear_args* a, const Route& r, hipStream_t st) {
   if (r.stream) {
-    const unsigned gn = (unsigned)((a->N + 15) / 16);
-    if (a->M <= 16) hipLaunchKernelGGL((mx_stream_kernel<E, FX, FW, 1, 8>), dim3(gn, 1), dim3(512), 0, st, *a, r.ex);
-    else if (a->M <= 32) hipLaunchKernelGGL((mx_stream_kernel<E, FX, FW, 2, 8>), dim3(gn, 1), dim3(512), 0, st, *a, r.ex);
-    else hipLaunchKernelGGL((mx_stream_kernel<E, FX, FW, 4, 8>), dim3(gn, 1), dim3(512), 0, st, *a, r.ex);
-    return sf_check_launch("mx_stream_kernel");
+    const auto go = [&](auto kernel, int rows) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((a->N + rows - 1) / rows)), dim3(512), 0, st, *a, r.ex);
+      return sf_check_launch("mx_stream_kernel");
+    };
+    const bool wide = a->N > kWideRows;
+    if (a->M <= 16) return wide ? go(mx_stream_kernel<E, FX, FW, 1, 2, 4, 8>, 32) : go(mx_stream_kernel<E, FX, FW, 1, 1, 4, 8>, 16);
+    if (a->M <= 32) return wide ? go(mx_stream_kernel<E, FX, FW, 2, 2, 4, 8>, 32) : go(mx_stream_kernel<E, FX, FW, 2, 1, 4, 8>, 16);
+    return wide ? go(mx_stream_kernel<E, FX, FW, 4, 2, 2, 8>, 32) : go(mx_stream_kernel<E, FX, FW, 4, 1, 2, 8>, 16);
   }
   const int64_t gm = (a->M + 127) / 128;
   // (a launch dimension past the second holds 65535 workgroups)
@@ -415,12 +509,14 @@ int launch(const sf_mx_linear_args* a, const Route& r, hipStream_t st) {
     rest.ex.steps = (a->K / 32 + 3) / 4;
     return launch<E, FX, FW>(&b, rest, st);
   }
-  hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW>), dim3((unsigned)((a->N + 127) / 128), (unsigned)gm, (unsigned)r.ex.slices), dim3(256), 0, st, *a,
-                     r.ex);
+  const dim3 grid((unsigned)((a->N + 127) / 128), (unsigned)gm, (unsigned)r.ex.slices);
+  if (r.ex.wide) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true>), grid, dim3(256), 0, st, *a, r.ex);
+  else hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, false>), grid, dim3(256), 0, st, *a, r.ex);
   const int rc = sf_check_launch("mx_tile_kernel");
   if (rc || r.ex.slices == 1) return rc;
   const int64_t all = a->M * a->N;
-  hipLaunchKernelGGL(mx_join_kernel<E>, dim3((unsigned)std::min<int64_t>((all + 255) / 256, 4096)), dim3(256), 0, st, *a, r.ex);
+  if (a->N % 4 == 0) hipLaunchKernelGGL((mx_join_kernel<E, 4>), dim3((unsigned)std::min<int64_t>((all / 4 + 255) / 256, 4096)), dim3(256), 0, st, *a, r.ex);
+  else hipLaunchKernelGGL((mx_join_kernel<E, 1>), dim3((unsigned)std::min<int64_t>((all + 255) / 256, 4096)), dim3(256), 0, st, *a, r.ex);
   return sf_check_launch("mx_join_kernel");
 }
 

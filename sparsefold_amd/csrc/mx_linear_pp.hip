@@ -8,10 +8,11 @@
 // A step is 64 bytes of a row of x: 64 k of 8 bits, 128 k of 4 bits; w as many k, so 4-bit w beside 8-bit x takes rows of 32
 // bytes.  Rows of 64 bytes keep their 16-byte pieces XORed by (row / 4) % 4; of 32 bytes two share a line, slots 2 (row % 2) +
 // piece, XORed by (row / 8) % 2: so 16 lanes that read together cover all banks.
-// Scales travel with the codes: each wave copies those of 64 rows (a step's 2 or 4 bytes a row, a word each in LDS), and a lane
-// reads the word of its row with the operands.
-// Results are rounded in registers, neighbouring columns brought together by a swap of the wave's halves, and stored by
-// buffer stores that drop what lies outside, so that their number, which the waits count, does not depend on the tile.
+// Scales come 16 at a time, 512 k: each wave copies those of 64 rows, into one of four LDS buffers, with the first step that needs
+// them, and a lane reads its rows' words with the operands.  (Copied with every step, 2 or 4 bytes a row, they touched 64
+// lines an instruction for 256 bytes: 8192^3 took 330 us of 4 bits and 582 of 8.)
+// Results are rounded in registers, brought together to whole lines by exchanges between lanes, and stored by buffer stores
+// that drop what lies outside, so that their number, which the waits count, does not depend on the tile.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,45 +50,40 @@ struct Copies {
                    "ds_read_b128 %6, %[x1] offset:4096\n\tds_read_b128 %7, %[x1] offset:6144\n\t"
 #define MX_READS_W2 "ds_read_b128 %8, %[w0]\n\tds_read_b128 %9, %[w0] offset:2048\n\tds_read_b128 %10, %[w1]\n\tds_read_b128 %11, %[w1] offset:2048\n\t"
 #define MX_READS_W1 "ds_read_b128 %8, %[w0]\n\tds_read_b128 %9, %[w0] offset:1024\n\t"
-#define MX_READS_S "ds_read_b32 %[s0], %[sx]\n\tds_read_b32 %[s1], %[sx] offset:128\n\tds_read_b32 %[s2], %[sx] offset:256\n\t" \
-                   "ds_read_b32 %[s3], %[sx] offset:384\n\tds_read_b32 %[s4], %[sw]\n\tds_read_b32 %[s5], %[sw] offset:128\n\t"
+#define MX_READS_S "ds_read_b32 %[s0], %[sx]\n\tds_read_b32 %[s1], %[sx] offset:512\n\tds_read_b32 %[s2], %[sx] offset:1024\n\t" \
+                   "ds_read_b32 %[s3], %[sx] offset:1536\n\tds_read_b32 %[s4], %[sw]\n\tds_read_b32 %[s5], %[sw] offset:512\n\t"
 #define MX_COPY_X "s_mov_b32 m0, %[mx]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[xo0], %[xa]\n\ts_add_u32 m0, m0, 0x400\n\ts_nop 0\n\t" \
                   "global_load_lds_dwordx4 %[xo1], %[xa]\n\t"
 #define MX_COPY_W1 "s_mov_b32 m0, %[mw]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[wo0], %[wa]\n\t"
 #define MX_COPY_W2 MX_COPY_W1 "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[wo1], %[wa]\n\t"
-#define MX_COPY_S4 "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dword %[so], %[sa]\n\t"
-#define MX_COPY_S2 "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_ushort %[so], %[sa]\n\t"
+#define MX_COPY_S "s_mov_b32 m0, %[ms]\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %[so], %[sa]\n\t"
 #define MX_WAIT "s_waitcnt lgkmcnt(0)"
 #define MX_OUT_X "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]), "=&v"(x[1][0]), "=&v"(x[1][1]), "=&v"(x[1][2]), "=&v"(x[1][3])
 #define MX_OUT_S [s0] "=&v"(s[0]), [s1] "=&v"(s[1]), [s2] "=&v"(s[2]), [s3] "=&v"(s[3]), [s4] "=&v"(s[4]), [s5] "=&v"(s[5])
 #define MX_IN [x0] "v"(x0), [x1] "v"(x0 ^ 32u), [w0] "v"(w0), [w1] "v"(w0 ^ 32u), [sx] "v"(sx), [sw] "v"(sw)
 #define MX_IN_COPY [mx] "s"(mx), [mw] "s"(mw), [ms] "s"(ms), [xa] "s"(xa), [wa] "s"(wa), [sa] "s"(sa), [xo0] "v"(c.xo[0]), [xo1] "v"(c.xo[1]), \
                    [wo0] "v"(c.wo[0]), [wo1] "v"(c.wo[1]), [so] "v"(c.so)
-template <int WC, int SB, bool COPY>
+enum Copy { kNone, kCodes, kCodesAndScales };
+template <int WC, Copy COPY>
 __device__ __forceinline__ void read_step(uint32_t x0, uint32_t w0, uint32_t sx, uint32_t sw, u32x4 (&x)[2][4], u32x4 (&w)[2][2], uint32_t (&s)[6],
                                           uint32_t mx, uint32_t mw, uint32_t ms, const char* xa, const char* wa, const char* sa, const Copies& c) {
-  if constexpr (WC == 2 && SB == 4) {
-    if constexpr (COPY)
-      asm volatile(MX_READS_X MX_READS_W2 MX_READS_S MX_COPY_X MX_COPY_W2 MX_COPY_S4 MX_WAIT
-                   : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), MX_OUT_S : MX_IN, MX_IN_COPY : "memory", "m0", "scc");
-    else
-      asm volatile(MX_READS_X MX_READS_W2 MX_READS_S MX_WAIT
-                   : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), MX_OUT_S : MX_IN : "memory");
-  } else if constexpr (WC == 2) {
-    if constexpr (COPY)
-      asm volatile(MX_READS_X MX_READS_W2 MX_READS_S MX_COPY_X MX_COPY_W2 MX_COPY_S2 MX_WAIT
-                   : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), MX_OUT_S : MX_IN, MX_IN_COPY : "memory", "m0", "scc");
-    else
-      asm volatile(MX_READS_X MX_READS_W2 MX_READS_S MX_WAIT
-                   : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), MX_OUT_S : MX_IN : "memory");
+#define MX_STEP(READS, COPIES, OUT_W) asm volatile(READS COPIES MX_WAIT : MX_OUT_X, OUT_W, MX_OUT_S : MX_IN, MX_IN_COPY : "memory", "m0", "scc")
+#define MX_OUT_W1 "=&v"(w[0][0]), "=&v"(w[0][1])
+#define MX_OUT_W2 "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1])
+#define MX_ARGS(...) __VA_ARGS__
+  if constexpr (WC == 2) {
+    if constexpr (COPY == kCodesAndScales) MX_STEP(MX_READS_X MX_READS_W2 MX_READS_S, MX_COPY_S MX_COPY_X MX_COPY_W2, MX_ARGS(MX_OUT_W2));
+    else if constexpr (COPY == kCodes) MX_STEP(MX_READS_X MX_READS_W2 MX_READS_S, MX_COPY_X MX_COPY_W2, MX_ARGS(MX_OUT_W2));
+    else MX_STEP(MX_READS_X MX_READS_W2 MX_READS_S, "", MX_ARGS(MX_OUT_W2));
   } else {
-    static_assert(SB == 2, "rows of 32 bytes of w are 64 k");
-    if constexpr (COPY)
-      asm volatile(MX_READS_X MX_READS_W1 MX_READS_S MX_COPY_X MX_COPY_W1 MX_COPY_S2 MX_WAIT
-                   : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), MX_OUT_S : MX_IN, MX_IN_COPY : "memory", "m0", "scc");
-    else
-      asm volatile(MX_READS_X MX_READS_W1 MX_READS_S MX_WAIT : MX_OUT_X, "=&v"(w[0][0]), "=&v"(w[0][1]), MX_OUT_S : MX_IN : "memory");
+    if constexpr (COPY == kCodesAndScales) MX_STEP(MX_READS_X MX_READS_W1 MX_READS_S, MX_COPY_S MX_COPY_X MX_COPY_W1, MX_ARGS(MX_OUT_W1));
+    else if constexpr (COPY == kCodes) MX_STEP(MX_READS_X MX_READS_W1 MX_READS_S, MX_COPY_X MX_COPY_W1, MX_ARGS(MX_OUT_W1));
+    else MX_STEP(MX_READS_X MX_READS_W1 MX_READS_S, "", MX_ARGS(MX_OUT_W1));
   }
+#undef MX_STEP
+#undef MX_OUT_W1
+#undef MX_OUT_W2
+#undef MX_ARGS
 }
 
 __device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
@@ -95,16 +91,30 @@ __device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
 }
 __device__ __forceinline__ i32x8 join4(u32x4 a) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}; }
 
+// Exchanges lo of the lanes with `bit` for hi of their partners without it (DPP: the partner in the quad).
+template <int DPP>
+__device__ __forceinline__ void turn(u32x4& lo, u32x4& hi, bool bit) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t l = lo[e], h = hi[e];
+    const uint32_t from_l = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)l, DPP, 0xF, 0xF, true);
+    const uint32_t from_h = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)h, DPP, 0xF, 0xF, true);
+    lo[e] = bit ? from_h : l;
+    hi[e] = bit ? h : from_l;
+  }
+}
+
 template <class E, class FX, class FW>
 __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_args a, const int gx, const int gy, const int total) {
   constexpr bool x8 = FX::kFormat == SF_FORMAT_MXFP8, w8 = FW::kFormat == SF_FORMAT_MXFP8;
   constexpr int S = 4, A = S - 1;
   constexpr int WROW = x8 && !w8 ? 32 : 64, WC = WROW / 32;   // bytes of a row of w in a step, copies of w a wave
   constexpr int SB = x8 ? 2 : 4;                              // blocks of 32 in a step
-  constexpr int XBYTES = kTile * 64, WBYTES = kTile * WROW, STAGE = XBYTES + WBYTES + 2 * kTile * 4;
-  constexpr int CPW = 2 + WC + 1;
+  constexpr int GS = 16 / SB;                                 // steps of a group of scales
+  constexpr int XBYTES = kTile * 64, WBYTES = kTile * WROW, STAGE = XBYTES + WBYTES, SCALES = 2 * kTile * 16;
+  constexpr int CPW = 2 + WC;                                 // (and a copy of scales before those of a group's first step)
   constexpr int MB = 4, NB = 2;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * STAGE + 4 * SCALES];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
@@ -155,7 +165,7 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
   const uint32_t wbase = lds0 + XBYTES +
                          (WROW == 64 ? (uint32_t)((wn * 64 + li) * 64 + ((half ^ ((li >> 2) & 3)) << 4))
                                      : (uint32_t)((wn * 32 + (li >> 1)) * 64 + (((2 * (li & 1) + half) ^ ((li >> 3) & 1)) << 4)));
-  const uint32_t sxbase = lds0 + XBYTES + WBYTES + (wm * 128 + li) * 4, swbase = lds0 + XBYTES + WBYTES + (kTile + wn * 64 + li) * 4;
+  const uint32_t sxbase = lds0 + S * STAGE + (wm * 128 + li) * 16, swbase = lds0 + S * STAGE + (kTile + wn * 64 + li) * 16;
   const auto barrier = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
@@ -164,8 +174,12 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
   };
 
   const int n = a.K / (32 * SB);                              // >= A (host rule)
+  const int blocks = a.K / 32, groups = (n + GS - 1) / GS;
+  // first block of a group's 16: the last group ends with the row
+  const auto group_at = [&](int g) __attribute__((always_inline)) { return min(16 * g, blocks - 16); };
   Copies c;
   sources(tile, c);
+  __builtin_amdgcn_global_load_lds(c.s + c.so, (lds_u32*)(smem + S * STAGE + wave * 1024), 16, 0, 0);
 #pragma unroll
   for (int t = 0; t < A; ++t) {
     uint8_t* const st = smem + t * STAGE;
@@ -174,8 +188,6 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
 #pragma unroll
     for (int u = 0; u < WC; ++u)
       __builtin_amdgcn_global_load_lds(c.w + (c.wo[u] + t * WROW), (lds_u32*)(st + XBYTES + (WC * wave + u) * 1024), 16, 0, 0);
-    if constexpr (SB == 4) __builtin_amdgcn_global_load_lds(c.s + (c.so + t * SB), (lds_u32*)(st + XBYTES + WBYTES + wave * 256), 4, 0, 0);
-    else __builtin_amdgcn_global_load_lds(c.s + (c.so + t * SB), (lds_u32*)(st + XBYTES + WBYTES + wave * 256), 2, 0, 0);
   }
   wait<(A - 1) * CPW>();
   barrier();
@@ -185,6 +197,7 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
   constexpr int kStores = MB * NB * 2;
   bool stored = false;
   int T = 0;                                                  // steps done: the stage of step t is (T + t) % S
+  int G = 0;                                                  // groups done: the buffer of group g is (G + g) % 4
   for (;;) {
     const int next = tile + G8;
     const bool has_next = next < tend;                        // uniform
@@ -202,16 +215,25 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
     for (int t = 0; t < n; ++t) {
       const uint32_t so = (uint32_t)((T + t) & A) * STAGE;
       const uint32_t to = lds0 + (uint32_t)((T + t + A) & A) * STAGE;
-      const uint32_t mx = to + wave * 2048, mw = to + XBYTES + wave * WC * 1024, ms = to + XBYTES + WBYTES + wave * 256;
+      const uint32_t mx = to + wave * 2048, mw = to + XBYTES + wave * WC * 1024;
+      const int g = t / GS, at = SB * t - group_at(g);        // the step's first scale among its group's
+      const uint32_t sc0 = (uint32_t)((G + g) & 3) * SCALES + (at & ~3);
       // read step t; copy step t + A of this tile, or step t + A - n of the next one
-      if (t + A < n)
-        read_step<WC, SB, true>(xbase + so, wbase + so, sxbase + so, swbase + so, xa, wa, s, mx, mw, ms, c.x + (int64_t)(t + A) * 64,
-                                c.w + (int64_t)(t + A) * WROW, c.s + (int64_t)(t + A) * SB, c);
-      else if (has_next)
-        read_step<WC, SB, true>(xbase + so, wbase + so, sxbase + so, swbase + so, xa, wa, s, mx, mw, ms, nc.x + (int64_t)(t + A - n) * 64,
-                                nc.w + (int64_t)(t + A - n) * WROW, nc.s + (int64_t)(t + A - n) * SB, nc);
-      else
-        read_step<WC, SB, false>(xbase + so, wbase + so, sxbase + so, swbase + so, xa, wa, s, mx, mw, ms, c.x, c.w, c.s, c);
+      const bool own = t + A < n;                             // (uniform, as all that follows from it)
+      const int ct = own ? t + A : t + A - n, cg = ct / GS;
+      const bool with_scales = ct % GS == 0;
+      const uint32_t ms = lds0 + S * STAGE + (uint32_t)((G + cg + (own ? 0 : groups)) & 3) * SCALES + wave * 1024;
+      const Copies& from = own ? c : nc;
+      const char *const xf = from.x + (int64_t)ct * 64, *const wf = from.w + (int64_t)ct * WROW, *const sf = from.s + group_at(cg);
+      if (own) {
+        if (with_scales) read_step<WC, kCodesAndScales>(xbase + so, wbase + so, sxbase + sc0, swbase + sc0, xa, wa, s, mx, mw, ms, xf, wf, sf, c);
+        else read_step<WC, kCodes>(xbase + so, wbase + so, sxbase + sc0, swbase + sc0, xa, wa, s, mx, mw, ms, xf, wf, sf, c);
+      } else if (has_next) {
+        if (with_scales) read_step<WC, kCodesAndScales>(xbase + so, wbase + so, sxbase + sc0, swbase + sc0, xa, wa, s, mx, mw, ms, xf, wf, sf, nc);
+        else read_step<WC, kCodes>(xbase + so, wbase + so, sxbase + sc0, swbase + sc0, xa, wa, s, mx, mw, ms, xf, wf, sf, nc);
+      } else {
+        read_step<WC, kNone>(xbase + so, wbase + so, sxbase + sc0, swbase + sc0, xa, wa, s, mx, mw, ms, xf, wf, sf, c);
+      }
       // the copies of step t + 1 have landed (in issue order); those of steps t + 2 .. t + A may stay in flight (left: how many
       // of them exist), and the stores issued between A - 1 and A
       const int left = has_next ? A : n - 2 - t;
@@ -224,7 +246,7 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
       barrier();
       uint32_t sc[6];
 #pragma unroll
-      for (int i = 0; i < 6; ++i) sc[i] = s[i] >> (8 * half);
+      for (int i = 0; i < 6; ++i) sc[i] = s[i] >> (8 * half + (x8 ? 8 * (at & 2) : 0));
       if constexpr (x8) {
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
@@ -250,6 +272,7 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
       barrier();
     }
     T += n;
+    G += groups;
 
     // ---- epilogue of this wave's 128 x 64 part: lane (row li, half) has columns 8 (r / 4) + 4 half + r % 4 ----
     {
@@ -273,23 +296,35 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
       const __amdgpu_buffer_rsrc_t r =
           __builtin_amdgcn_make_buffer_rsrc((uint16_t*)a.y + (rows > 0 ? m0 : 0) * a.y_rs, (short)0, rows > 0 ? 0x7fffff00 : 0, 0x00020000);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+      for (int mb = 0; mb < MB; ++mb) {
+        u32x4 p[4];                                           // 8 columns 16 c + 8 half .. of row li: c = 2 nb + q
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int c4 = 0; c4 < 4; ++c4) {
+          const f32x16v& v = acc[mb][c4 >> 1];
+          const int q = 8 * (c4 & 1);
+          const float lo[8] = {v[q], v[q + 1], v[q + 2], v[q + 3], v[q + 4], v[q + 5], v[q + 6], v[q + 7]};
+          const u32x4 k = E::pack(lo);                        // columns 16 c + 4 half .. + 3 and 8 further
+          const uint32_t k0 = k[0], k1 = k[1], k2 = k[2], k3 = k[3];
+          const auto y0 = __builtin_amdgcn_permlane32_swap(k0, k2, false, false);
+          const auto y1 = __builtin_amdgcn_permlane32_swap(k1, k3, false, false);
+          p[c4] = u32x4{y0[0], y1[0], y0[1], y1[1]};
+        }
+        // Four lanes that hold four pieces of a row each turn them over, so that a store takes whole lines: lane 4 i + b's
+        // piece c goes to lane 4 i + c's place b.  (32 bytes of each of 32 rows a store: 8192 x 8192 x 1024 of 4 bits 66 us.)
+        turn<0xB1>(p[0], p[1], lane & 1);
+        turn<0xB1>(p[2], p[3], lane & 1);
+        turn<0x4E>(p[0], p[2], lane & 2);
+        turn<0x4E>(p[1], p[3], lane & 2);
+        const int col = n0 + 16 * (lane & 3) + 8 * half;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const f32x16v& v = acc[mb][nb];
-            const float lo[8] = {v[8 * q], v[8 * q + 1], v[8 * q + 2], v[8 * q + 3], v[8 * q + 4], v[8 * q + 5], v[8 * q + 6], v[8 * q + 7]};
-            const u32x4 p = E::pack(lo);                      // columns 16 q + 4 half .. + 3 and 8 further
-            const uint32_t p0 = p[0], p1 = p[1], p2 = p[2], p3 = p[3];
-            // half 0 takes the 8 columns 16 q .., half 1 the 8 columns 16 q + 8 ..
-            const auto y0 = __builtin_amdgcn_permlane32_swap(p0, p2, false, false);
-            const auto y1 = __builtin_amdgcn_permlane32_swap(p1, p3, false, false);
-            const int row = 32 * mb + li, col = n0 + 32 * nb + 16 * q + 8 * half;
-            const uint32_t off = row < rows && col < a.N ? (uint32_t)row * (uint32_t)(2 * a.y_rs) + 2u * (uint32_t)col : 0x80000000u;
-            typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
-            __builtin_amdgcn_raw_buffer_store_b128(i32x4{(int)y0[0], (int)y1[0], (int)y0[1], (int)y1[1]}, r, (int)off, 0, 0);
-          }
+        for (int c4 = 0; c4 < 4; ++c4) {
+          const int row = 32 * mb + (li & ~3) + c4;
+          const uint32_t off = row < rows && col < a.N ? (uint32_t)row * (uint32_t)(2 * a.y_rs) + 2u * (uint32_t)col : 0x80000000u;
+          typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, p[c4]), r, (int)off, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);                    // (registers)
+      }
       stored = true;
     }
     if (!has_next) break;
@@ -319,13 +354,12 @@ int launch_formats(const sf_mx_linear_args* a, hipStream_t st) {
 
 }  // namespace
 
-// What the kernel assumes: whole steps, at least four of them, aligned rows, offsets inside a tile that fit 32 bits; and sizes
+// What the kernel assumes: whole steps, at least four of them, 16 scales a row and words of them aligned, aligned rows, offsets inside a tile that fit 32 bits; and sizes
 // for which its tiles pay.
 bool sf_mx_linear_pp_ok(const sf_mx_linear_args* a) {
-  const int step = a->x_format == SF_FORMAT_MXFP8 ? 64 : 128, sb = step / 32;
-  if (a->K % step != 0 || a->K < 4 * step || a->N % 8 != 0 || a->M < kTile || a->N < kTile) return false;
+  if (a->K % 128 != 0 || a->K < 512 || a->N % 8 != 0 || a->M < kTile || a->N < kTile) return false;
   if (!al16(a->y) || a->y_rs % 8 != 0 || a->y_rs >= 1 << 22 || (a->bias && !al16(a->bias))) return false;
-  if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales | (uintptr_t)a->xs_rs | (uintptr_t)a->ws_rs) % sb != 0) return false;
+  if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales | (uintptr_t)a->xs_rs | (uintptr_t)a->ws_rs) % 4 != 0) return false;
   const int64_t total = ((a->M + kTile - 1) / kTile) * (((int64_t)a->N + kTile - 1) / kTile);
   return total >= 128 && total < 1ll << 30;
 }

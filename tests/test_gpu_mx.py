@@ -183,7 +183,7 @@ def operands(M, N, K, formats, seed=0):
 
 @pytest.mark.parametrize("formats", FORMATS, ids="-".join)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 16, 512), (8, 4096, 4096), (3, 100, 96), (16, 130, 160), (17, 64, 544), (31, 7, 1056), (33, 48, 2080),
-                                   (64, 257, 1024), (65, 1, 32), (65, 128, 128), (100, 130, 224), (128, 128, 4096), (129, 255, 288),
+                                   (64, 257, 1024), (9, 40, 640), (40, 17, 1664), (65, 1, 32), (65, 128, 128), (100, 130, 224), (128, 128, 4096), (129, 255, 288),
                                    (200, 1000, 1600), (300, 520, 768), (1000, 264, 2048), (70, 4096, 4096)])
 def test_product(M, N, K, formats):
   x, w = operands(M, N, K, formats, M + N)
@@ -228,7 +228,7 @@ def test_each_scale_reaches_its_block(M):
   """Scales that differ from block to block by up to 2^20: a byte in the wrong place would be seen."""
   g = torch.Generator().manual_seed(M)
   for formats in FORMATS:
-    for K in (128, 512, 672, 1536):
+    for K in (128, 512, 640, 672, 1536):
       x, w = operands(M, 140, K, formats, K)
       xs, ws = (torch.randint(117, 138, t.scales.shape, generator=g).to(torch.uint8).to(DEV) for t in (x, w))
       x, w = ops.Microscaled(x.codes, xs), ops.Microscaled(w.codes, ws)
