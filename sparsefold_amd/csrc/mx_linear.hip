@@ -196,7 +196,8 @@ __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_a
 // ---------------------------------------------------------------------------------------
 // Tiles of 128 x 128, waves of 64 x 64, steps of 128 k through two LDS buffers.
 // ---------------------------------------------------------------------------------------
-// WIDE: scales load as words, and two steps are in flight; else byte by byte and one step ahead (registers).
+// WIDE: scales load 16 at a time, 512 k, a row a thread, and go through LDS too (a word of 32 rows a load and step touched as many
+// lines as the codes); and two steps are in flight.  Else byte by byte and one step ahead (registers).
 template <class F, bool WIDE>
 struct TileOperand {
   using O = Op<F>;
@@ -205,7 +206,7 @@ struct TileOperand {
   static __device__ __forceinline__ int slot(int row, int piece) { return O::k8 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
   static constexpr int kAhead = WIDE ? 2 : 1;                // steps in flight
   u32x4 data[kAhead][kN];
-  uint32_t sdata[kAhead][2];
+  uint32_t sdata[2];                                         // (not WIDE)
   __amdgpu_buffer_rsrc_t r, rs;
   uint32_t off[kN], srow[2];
   __device__ __forceinline__ void init(const void* codes, int64_t c_rs, const void* scales, int64_t s_rs, int64_t row0, int64_t rows, int blocks,
@@ -215,7 +216,7 @@ struct TileOperand {
     rs = rsrc((const uint8_t*)scales + row0 * s_rs, (n - 1) * s_rs + blocks);
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
-      const int idx = u * 256 + threadIdx.x, row = idx / kPieces;
+      const int idx = u * 256 + (threadIdx.x & 255), row = idx / kPieces;
       off[u] = row < n ? (uint32_t)(row * c_rs) + idx % kPieces * 16 : kOutside;
     }
 #pragma unroll
@@ -226,18 +227,20 @@ struct TileOperand {
   __device__ __forceinline__ void load(int step, int blocks) {
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
-      const int piece = (u * 256 + threadIdx.x) % kPieces;
+      const int piece = (u * 256 + (threadIdx.x & 255)) % kPieces;
       const bool in = 4 * step + piece * 16 / O::kBlock < blocks;
       data[D][u] = load16(r, in ? off[u] + step * kRow : kOutside);
     }
+    if constexpr (!WIDE) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) sdata[D][t] = scales4(rs, srow[t], 4 * step, blocks - 4 * step, WIDE);
+      for (int t = 0; t < 2; ++t) sdata[t] = scales4(rs, srow[t], 4 * step, blocks - 4 * step, false);
+    }
   }
   template <int D>
   __device__ __forceinline__ void store(uint8_t* lds) const {
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
-      const int idx = u * 256 + threadIdx.x, row = idx / kPieces;
+      const int idx = u * 256 + (threadIdx.x & 255), row = idx / kPieces;
       st16(lds + row * kRow + (slot(row, idx % kPieces) << 4), data[D][u]);
     }
   }
@@ -252,17 +255,24 @@ struct TileOperand {
   }
 };
 
-template <class E, class FX, class FW, bool WIDE>
-__global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args a, const Extra ex) {
+// KG groups of 4 waves take a part of the steps each, through LDS of their own, and are summed through LDS.
+template <class E, class FX, class FW, bool WIDE, int KG>
+__global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear_args a, const Extra ex) {
   using X = TileOperand<FX, WIDE>;
   using W = TileOperand<FW, WIDE>;
   constexpr int kAhead = X::kAhead;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * (X::kBytes + W::kBytes)];
-  const int lane = threadIdx.x & 63, half = lane >> 5, li = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  constexpr int kScales = WIDE ? 256 * 16 : 0;               // of the 128 rows of x, then of w
+  constexpr int kGroup = 2 * (X::kBytes + W::kBytes) + 2 * kScales;
+  __shared__ __attribute__((aligned(1024))) uint8_t shared[KG * kGroup];
+  const int tid = threadIdx.x & 255, lane = tid & 63, half = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  uint8_t* const smem = shared + kg * kGroup;
   const int n0 = blockIdx.x * 128;
   const int64_t m0 = (int64_t)blockIdx.y * 128;
-  const int blocks = a.K / 32, s0 = blockIdx.z * ex.steps, s1 = min(s0 + ex.steps, (blocks + 3) / 4), last = min(blocks, 4 * s1);
+  const int blocks = a.K / 32, per = ex.steps / KG, first = blockIdx.z * ex.steps, end = min(first + ex.steps, (blocks + 3) / 4);
+  const int count = min(per, end - first);                   // steps of every group (the last one's may add zeros)
+  const int s0 = first + kg * per, s1 = s0 + count, last = min(blocks, 4 * min(s0 + per, end));
   X x;
   W w;
   x.init(a.x, a.x_rs, a.x_scales, a.xs_rs, m0, a.M, blocks, 64 * wm);
@@ -274,6 +284,21 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  // scales 16 g .. + 15 of the thread's row, zeros past the row's end
+  u32x4 group = {0, 0, 0, 0};
+  const auto load_group = [&](int g) __attribute__((always_inline)) {
+    const bool of_x = wave < 2;
+    const int row = tid & 127;
+    const __amdgpu_buffer_rsrc_t r = of_x ? x.rs : w.rs;
+    const uint32_t at = (uint32_t)((of_x ? min((int64_t)row, a.M - m0 - 1) * a.xs_rs : (int64_t)min(row, a.N - n0 - 1) * a.ws_rs)) + 16 * g;
+    if (16 * g + 16 <= blocks) {
+      group = load16(r, at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        group[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(16 * g + 4 * e < blocks ? at + 4 * e : kOutside), 0, 0);
+    }
+  };
   // Step s is stored to one of two LDS buffers while the next kAhead steps are in flight to registers: one barrier a step (the
   // buffer's readers, two steps before, passed the last one).
   const auto step = [&](auto constant, int s) __attribute__((always_inline)) {
@@ -283,15 +308,31 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
     x.template store<D>(xt);
     w.template store<D>(wt);
     uint32_t cx[2], cw[2];
+    uint8_t* const sc = smem + 2 * (X::kBytes + W::kBytes) + ((s >> 2) & 1) * kScales;
+    if constexpr (WIDE) {
+      if (D == 0 && (s & 3) == 0) {                          // (uniform; the buffer's readers are four steps behind)
+        st16(sc + tid * 16, group);
+        load_group((s >> 2) + 1);
+      }
+    } else {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      cx[t] = x.sdata[D][t] >> (8 * half);                   // chunk 0: byte 0, chunk 1: byte 2
-      cw[t] = w.sdata[D][t] >> (8 * half);
+      for (int t = 0; t < 2; ++t) {
+        cx[t] = x.sdata[t] >> (8 * half);                    // chunk 0: byte 0, chunk 1: byte 2
+        cw[t] = w.sdata[t] >> (8 * half);
+      }
     }
     lds_only_barrier();
     x.template load<D>(s + kAhead, last);                    // (zeros past the slice's end)
     w.template load<D>(s + kAhead, last);
     __builtin_amdgcn_sched_barrier(0);                       // (moved behind the products, the loads were waited for at once)
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint8_t* const at = sc + 4 * (s & 3) + (32 * t + li) * 16;
+        cx[t] = *reinterpret_cast<const uint32_t*>(at + 64 * wm * 16) >> (8 * half);
+        cw[t] = *reinterpret_cast<const uint32_t*>(at + (128 + 64 * wn) * 16) >> (8 * half);
+      }
+    }
     i32x8 wo[2][2], xo[2][2];
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch)
@@ -310,6 +351,7 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
       for (int j = 0; j < 2; ++j) acc[i][j] = mfma32s<FW, FX, 2, 2>(wo[1][i], xo[1][j], acc[i][j], cw[i], cx[j]);
     __builtin_amdgcn_sched_barrier(0);
   };
+  if constexpr (WIDE) load_group(s0 >> 2);
   x.template load<0>(s0, last);
   w.template load<0>(s0, last);
   if constexpr (WIDE) {
@@ -327,6 +369,32 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) asm volatile("" : "+v"(acc[i][j]));
+  if constexpr (KG == 2) {
+    f32x4* const so = reinterpret_cast<f32x4*>(shared) + tid;
+    lds_only_barrier();
+    if (kg == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            so[256 * (8 * i + 4 * j + c)] = f32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
+    }
+    lds_only_barrier();
+    if (kg == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const f32x4 o = so[256 * (8 * i + 4 * j + c)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * c + e] += o[e];
+          }
+    }
+  }
   // Results go through LDS so that whole lines are stored (straight from the registers, 32 bytes of each of 32 rows an
   // instruction, 33 MB of parts took 15 us).  A lane (row li of x, half) has columns 8 c + 4 half .. + 3.
   if (ex.slices > 1) {
@@ -334,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {                   // rows 64 pass .. + 63
       lds_only_barrier();
-      if (wm == pass) {
+      if (kg == 0 && wm == pass) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -343,15 +411,15 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
             for (int c = 0; c < 4; ++c) {
               const int row = 32 * j + li, piece = 16 * wn + 8 * i + 2 * c + half;
               const f32x16v& v = acc[i][j];
-              *reinterpret_cast<f32x4*>(smem + row * kLine + ((piece ^ (row & 31)) << 4)) = f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+              *reinterpret_cast<f32x4*>(shared + row * kLine + ((piece ^ (row & 31)) << 4)) = f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
             }
       }
       lds_only_barrier();
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int idx = u * 256 + threadIdx.x, row = idx >> 5, piece = idx & 31, n = n0 + 4 * piece;
+      for (int u = 0; u < 8 / KG; ++u) {
+        const int idx = u * 256 * KG + threadIdx.x, row = idx >> 5, piece = idx & 31, n = n0 + 4 * piece;
         const int64_t m = m0 + 64 * pass + row;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(smem + row * kLine + ((piece ^ (row & 31)) << 4));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(shared + row * kLine + ((piece ^ (row & 31)) << 4));
         if (m >= a.M) continue;
         float* const p = ex.part + ((int64_t)blockIdx.z * a.M + m) * a.N + n;
         if (a.N % 4 == 0) {
@@ -367,31 +435,33 @@ __global__ __launch_bounds__(256, 2) void mx_tile_kernel(const sf_mx_linear_args
   }
   constexpr int kLine = 256;
   lds_only_barrier();
+  if (kg == 0) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int col = 64 * wn + 32 * i + 8 * c + 4 * half;
-      float b[4] = {0.f, 0.f, 0.f, 0.f};
-      if (a.bias != nullptr) {
+      for (int c = 0; c < 4; ++c) {
+        const int col = 64 * wn + 32 * i + 8 * c + 4 * half;
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias != nullptr) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = a.bias[min(n0 + col + e, a.N - 1)];
+          for (int e = 0; e < 4; ++e) b[e] = a.bias[min(n0 + col + e, a.N - 1)];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 64 * wm + 32 * j + li;
+          const f32x16v& v = acc[i][j];
+          const float w8[8] = {v[4 * c] + b[0], v[4 * c + 1] + b[1], v[4 * c + 2] + b[2], v[4 * c + 3] + b[3], 0.f, 0.f, 0.f, 0.f};
+          const u32x4 q = E::pack(w8);
+          *reinterpret_cast<u32x2*>(shared + row * kLine + (((col >> 3) ^ (row & 15)) << 4) + 8 * half) = u32x2{q[0], q[1]};
+        }
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = 64 * wm + 32 * j + li;
-        const f32x16v& v = acc[i][j];
-        const float w8[8] = {v[4 * c] + b[0], v[4 * c + 1] + b[1], v[4 * c + 2] + b[2], v[4 * c + 3] + b[3], 0.f, 0.f, 0.f, 0.f};
-        const u32x4 q = E::pack(w8);
-        *reinterpret_cast<u32x2*>(smem + row * kLine + (((col >> 3) ^ (row & 15)) << 4) + 8 * half) = u32x2{q[0], q[1]};
-      }
-    }
+  }
   lds_only_barrier();
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int idx = u * 256 + threadIdx.x, row = idx >> 4, piece = idx & 15, n = n0 + 8 * piece;
+  for (int u = 0; u < 8 / KG; ++u) {
+    const int idx = u * 256 * KG + threadIdx.x, row = idx >> 4, piece = idx & 15, n = n0 + 8 * piece;
     const int64_t m = m0 + row;
-    const u32x4 q = ld16(smem + row * kLine + ((piece ^ (row & 15)) << 4));
+    const u32x4 q = ld16(shared + row * kLine + ((piece ^ (row & 15)) << 4));
     if (m >= a.M) continue;
     uint16_t* const y = (uint16_t*)a.y + m * a.y_rs + n;
     if (ex.vector && n + 8 <= a.N) {
@@ -440,6 +510,7 @@ constexpr int kWideRows = 6144;
 
 struct Route {
   bool stream, large;
+  int groups;          // mx_tile_kernel: of 4 waves a workgroup
   Extra ex;
 };
 
@@ -464,18 +535,38 @@ int check(const sf_mx_linear_args* a) {
   return 0;
 }
 
+// us of mx_tile_kernel with k in `slices` parts, and the join: a step of 128 k 0.70 (8 and 8 bits), 0.60 (8 and 4) or 0.44 (4 and 4), start
+// and results 4, the join's launch 4, the parts written and read again at 4.5 TB/s.  (4096 x 4096 weights, 8 and 8 bits, rows / parts:
+// 100 / 1, 2, 4, 8: 24.0, 19.0, 16.3, 17.8; 256 / 1, 2, 4: 24.5, 22.1, 19.7; 777 / 1, 2: 26.2, 32.5.)
+double tile_cost(const sf_mx_linear_args* a, int steps, int slices) {
+  const double step = a->x_format == SF_FORMAT_MXFP4 ? 0.44 : a->w_format == SF_FORMAT_MXFP4 ? 0.60 : 0.70;
+  const double join = slices > 1 ? 4.0 + slices * (double)a->M * a->N * 8 / 4.5e6 : 0.0;
+  return 4.0 + step * ((steps + slices - 1) / slices) + join;
+}
+
+// us of mx_stream_kernel with more than 32 rows: bound by the workgroups' loads of x (64 rows, 4096 x 4096 weights, 8 and 4 bits of x: 16.9
+// and 11.9; 12288 x 4096 38 and 25).
+double stream_cost(const sf_mx_linear_args* a) {
+  return 3.0 + (a->x_format == SF_FORMAT_MXFP4 ? 9.0 : 13.5) * (a->K / 4096.0) * std::max(1.0, a->N / 4096.0);
+}
+
 void route(const sf_mx_linear_args* a, Route& r) {
   const auto words = [](const void* p, int64_t rs) { return ((uintptr_t)p | (uintptr_t)rs) % 4 == 0; };
   r.ex.wide = a->K % 128 == 0 && words(a->x_scales, a->xs_rs) && words(a->w_scales, a->ws_rs);
   r.ex.vector = al16(a->y) && a->y_rs % 8 == 0;
   r.ex.part = nullptr;
-  r.stream = a->M <= 64;
-  r.large = !r.stream && sf_mx_linear_pp_ok(a);
+  r.large = a->M > 64 && sf_mx_linear_pp_ok(a);
   const int64_t tiles = ((a->M + 127) / 128) * ((a->N + 127) / 128);
   const int steps = (a->K / 32 + 3) / 4;
-  int64_t slices = 1;
-  if (!r.stream && !r.large) slices = std::max<int64_t>(1, std::min<int64_t>(512 / tiles, steps / 4));
-  r.ex.steps = (int)((steps + slices - 1) / slices);
+  int slices = 1;
+  for (int s = 2; s <= 16 && tiles * s <= 256 && 4 * s <= steps; ++s)
+    if (tile_cost(a, steps, s) < tile_cost(a, steps, slices)) slices = s;
+  r.stream = a->M <= 32 || (a->M <= 64 && stream_cost(a) <= tile_cost(a, steps, slices));
+  if (r.stream || r.large) slices = 1;
+  // two groups of waves where a workgroup has a CU to itself (777 rows above: 29.2 us with one)
+  r.groups = r.ex.wide && tiles * slices <= 256 && steps / slices >= 8 ? 2 : 1;
+  const int whole = 4 * r.groups;                            // (whole groups of scales for each group of waves)
+  r.ex.steps = ((steps + slices - 1) / slices + whole - 1) / whole * whole;
   r.ex.slices = (steps + r.ex.steps - 1) / r.ex.steps;
 }
 
@@ -506,12 +597,14 @@ int launch(const sf_mx_linear_args* a, const Route& r, hipStream_t st) {
     Route rest;
     route(&b, rest);
     rest.ex.slices = 1;                                      // (the workspace is the whole call's)
-    rest.ex.steps = (a->K / 32 + 3) / 4;
+    rest.groups = 1;
+    rest.ex.steps = ((a->K / 32 + 3) / 4 + 3) / 4 * 4;
     return launch<E, FX, FW>(&b, rest, st);
   }
   const dim3 grid((unsigned)((a->N + 127) / 128), (unsigned)gm, (unsigned)r.ex.slices);
-  if (r.ex.wide) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true>), grid, dim3(256), 0, st, *a, r.ex);
-  else hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, false>), grid, dim3(256), 0, st, *a, r.ex);
+  if (!r.ex.wide) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, false, 1>), grid, dim3(256), 0, st, *a, r.ex);
+  else if (r.groups == 1) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true, 1>), grid, dim3(256), 0, st, *a, r.ex);
+  else hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true, 2>), grid, dim3(512), 0, st, *a, r.ex);
   const int rc = sf_check_launch("mx_tile_kernel");
   if (rc || r.ex.slices == 1) return rc;
   const int64_t all = a->M * a->N;

@@ -361,7 +361,8 @@ bool sf_mx_linear_pp_ok(const sf_mx_linear_args* a) {
   if (!al16(a->y) || a->y_rs % 8 != 0 || a->y_rs >= 1 << 22 || (a->bias && !al16(a->bias))) return false;
   if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales | (uintptr_t)a->xs_rs | (uintptr_t)a->ws_rs) % 4 != 0) return false;
   const int64_t total = ((a->M + kTile - 1) / kTile) * (((int64_t)a->N + kTile - 1) / kTile);
-  return total >= 128 && total < 1ll << 30;
+  // (4096 x 4096 weights, 8 and 8 bits: 2048 rows, 128 tiles, 64 us here and 50 in tiles of 128; 2304 63 and 64; 3000 64 and 66; 4096 70 and 87)
+  return total >= 160 && total < 1ll << 30;
 }
 
 int sf_mx_linear_pp_launch(const sf_mx_linear_args* a, hipStream_t stream) {

@@ -191,7 +191,7 @@ def test_product(M, N, K, formats):
 
 
 @pytest.mark.parametrize("formats", FORMATS, ids="-".join)
-@pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (1500, 4104, 1088), (2049, 1999, 640), (4096, 2048, 512), (3900, 2312, 640), (2049, 4104, 1152),
+@pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (1500, 4104, 1088), (2049, 1999, 640), (4096, 2560, 512), (4096, 2048, 512), (3900, 2824, 640), (2305, 4104, 1152),
                                    (4099, 4104, 512), (9000, 1032, 512)])
 def test_large_product(M, N, K, formats):
   """Scales of many binades too; the last ones more than one tile a workgroup."""
@@ -235,9 +235,9 @@ def test_each_scale_reaches_its_block(M):
       check(ops.mx_linear(x, w), x, w)
 
 
-@pytest.mark.parametrize("M", [4, 40, 200, 4096])
+@pytest.mark.parametrize("M", [4, 40, 200, 5200])
 def test_nan_and_extreme_scales(M):
-  x, w = operands(M, 2048, 256, FORMATS[1], M)
+  x, w = operands(M, 2048, 512, FORMATS[1], M)
   xs, ws = x.scales.view(torch.uint8).clone(), w.scales.view(torch.uint8).clone()
   xs[1, 3], ws[5, 0] = 255, 255
   y = ops.mx_linear(ops.Microscaled(x.codes, xs), ops.Microscaled(w.codes, ws))
