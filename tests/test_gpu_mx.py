@@ -192,7 +192,7 @@ def test_product(M, N, K, formats):
 
 @pytest.mark.parametrize("formats", FORMATS, ids="-".join)
 @pytest.mark.parametrize("M,N,K", [(2048, 2048, 2048), (1500, 4104, 1088), (2049, 1999, 640), (4096, 2560, 512), (4096, 2048, 512), (3900, 2824, 640), (2305, 4104, 1152),
-                                   (4099, 4104, 512), (9000, 1032, 512)])
+                                   (4099, 4104, 512), (9000, 1032, 512), (4099, 4104, 1536), (2570, 4352, 768)])
 def test_large_product(M, N, K, formats):
   """Scales of many binades too; the last ones more than one tile a workgroup."""
   x, w = operands(M, N, K, formats, 3)
