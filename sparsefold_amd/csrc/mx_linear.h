@@ -6,6 +6,3 @@
 
 bool sf_mx_linear_pp_ok(const sf_mx_linear_args* a);
 int sf_mx_linear_pp_launch(const sf_mx_linear_args* a, hipStream_t stream);
-// The same of 4-bit operands with waves of 128 x 128: whether it serves what the former serves, and its launch.
-bool sf_mx_linear_w4_ok(const sf_mx_linear_args* a);
-int sf_mx_linear_w4_launch(const sf_mx_linear_args* a, hipStream_t stream);

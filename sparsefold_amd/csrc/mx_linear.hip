@@ -645,6 +645,6 @@ extern "C" int sf_hip_mx_linear_fwd(const sf_mx_linear_args* a, void* workspace,
   }
   r.ex.part = static_cast<float*>(workspace);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (r.large) return sf_mx_linear_w4_ok(a) ? sf_mx_linear_w4_launch(a, st) : sf_mx_linear_pp_launch(a, st);
+  if (r.large) return sf_mx_linear_pp_launch(a, st);
   return a->dtype == SF_DTYPE_BF16 ? launch_formats<RowBf16>(a, r, st) : launch_formats<RowFp16>(a, r, st);
 }
