@@ -1024,7 +1024,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
   ``j % rows`` of page ``page_table[b, j // rows]`` (int32 ``[B, pages of a sequence]``).
 
   Offsets, lengths and table are read on the device only: the call can be captured.  Keys whose place lies outside the
-  table or the cache are dropped.  Pages that sequences share may not be written by more than one of them."""
+  table or the cache are dropped.  Each new key has a place of its own: pages that sequences share are written by one of
+  them at most, and a sequence's table names a page once (of two keys written to one place either is left)."""
   what = "paged_cache_write"
   _no_grad(what, k, v, k_pages, v_pages)
   _require_cuda(k, v, k_pages, v_pages, page_table, cu, len_k, len_new)
@@ -1153,7 +1154,7 @@ def _microscaled(x, name: str, what: str):
                      f"{dtype} and {scales.dtype}")
   cs, ss = codes.shape, scales.shape
   K = (cs[-1] if eight else 2 * cs[-1]) if cs else 0
-  if K < 32 or K % 32 != 0 or ss[:-1] != cs[:-1] or ss[-1] * 32 != K:
+  if K < 32 or K % 32 != 0 or not ss or ss[:-1] != cs[:-1] or ss[-1] * 32 != K:
     raise ValueError(f"{what}: {name} needs a scale for each block of 32, got codes {tuple(cs)} and scales {tuple(ss)}")
   format = _lib.FORMAT_MXFP8 if eight else _lib.FORMAT_MXFP4
   if codes.is_contiguous() and scales.is_contiguous() and codes.data_ptr() % 16 == 0:
@@ -1219,6 +1220,7 @@ def mx_quantize(x: torch.Tensor, format: str = "mxfp4") -> Microscaled:
 def mx_dequantize(x: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
   """The numbers ``[..., K]`` that codes and scales stand for, rounded once to ``dtype`` (bf16, fp16 or float32)."""
   what = "mx_dequantize"
+  _no_grad(what, *x)
   _require_cuda(*x)
   if dtype not in _ELEMENT_TYPES:
     raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
@@ -1238,7 +1240,7 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
   ``out`` ``[..., N]`` with a unit last stride overlaps no input.  Sums are fp32; of 8-bit codes the matrix unit adds 8
   products (8 consecutive k) at a time and cuts off what lies below 2^-13 of the largest of them."""
   what = "mx_linear"
-  _no_grad(what, bias, out)
+  _no_grad(what, *x, *w, bias, out)
   dev = _require_cuda(*x, *w, bias, out)
   if w.codes.ndim != 2:
     raise ValueError(f"{what}: w must be [features, K], got codes {tuple(w.codes.shape)}")

@@ -15,7 +15,7 @@
 // that drop what lies outside, so that their number, which the waits count, does not depend on the tile.
 //
 // 8192^3: 287 us of 4 bits, 3.8 PFLOP/s, and 493 of 8 bits, 2.2 (products of 8192^3 in bf16: 1.3; matrix instructions alone, on random codes in
-// registers: 6.8 and 3.8, clocks held by power).  With all codes zero 239 us of 4 bits, without the copies 240.  4 waves of 128 x 128, one a
+// registers: 6.8 and 3.8, clocks held by power).  With all codes zero 236 us of 4 bits and 425 of 8; of 4 bits without the copies 240.  4 waves of 128 x 128, one a
 // SIMD, with the next step's reads between the products took as long (283 us, 285 with copies of whole 128-byte lines), so the two
 // groups' alternation is not what bounds it; L2 hits 90% of the lines asked for.
 #include <algorithm>
@@ -298,6 +298,9 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
           }
       }
       const int64_t rows = a.M - m0;
+      uint32_t line = 2 * (uint32_t)a.y_rs;                   // (taken up here: kept over the loop, the rows' offsets cost registers)
+      int own_row = li & ~3, own_col = 16 * (lane & 3) + 8 * half;
+      asm volatile("" : "+s"(line), "+v"(own_row), "+v"(own_col));
       const __amdgpu_buffer_rsrc_t r =
           __builtin_amdgcn_make_buffer_rsrc((uint16_t*)a.y + (rows > 0 ? m0 : 0) * a.y_rs, (short)0, rows > 0 ? 0x7fffff00 : 0, 0x00020000);
 #pragma unroll
@@ -320,11 +323,11 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
         turn<0xB1>(p[2], p[3], lane & 1);
         turn<0x4E>(p[0], p[2], lane & 2);
         turn<0x4E>(p[1], p[3], lane & 2);
-        const int col = n0 + 16 * (lane & 3) + 8 * half;
+        const int col = n0 + own_col;
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
-          const int row = 32 * mb + (li & ~3) + c4;
-          const uint32_t off = row < rows && col < a.N ? (uint32_t)row * (uint32_t)(2 * a.y_rs) + 2u * (uint32_t)col : 0x80000000u;
+          const int row = 32 * mb + own_row + c4;
+          const uint32_t off = row < rows && col < a.N ? (uint32_t)row * line + 2u * (uint32_t)col : 0x80000000u;
           typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, p[c4]), r, (int)off, 0, 0);
         }
