@@ -207,12 +207,15 @@ struct TileOperand {
   static constexpr int kAhead = WIDE ? 2 : 1;                // steps in flight
   u32x4 data[kAhead][kN];
   uint32_t sdata[2];                                         // (not WIDE)
-  __amdgpu_buffer_rsrc_t r, rs;
+  __amdgpu_buffer_rsrc_t rs;
+  const uint8_t* base;
+  int bytes;
   uint32_t off[kN], srow[2];
   __device__ __forceinline__ void init(const void* codes, int64_t c_rs, const void* scales, int64_t s_rs, int64_t row0, int64_t rows, int blocks,
                                        int wave_row) {
     const int64_t n = rows - row0 < 128 ? rows - row0 : 128;
-    r = rsrc((const uint8_t*)codes + row0 * c_rs, (n - 1) * c_rs + (int64_t)blocks * O::kBlock);
+    base = (const uint8_t*)codes + row0 * c_rs;
+    bytes = (int)((n - 1) * c_rs + (int64_t)blocks * O::kBlock);
     rs = rsrc((const uint8_t*)scales + row0 * s_rs, (n - 1) * s_rs + blocks);
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
@@ -225,11 +228,17 @@ struct TileOperand {
   // step `step` into slot D, zeros past the last
   template <int D>
   __device__ __forceinline__ void load(int step, int blocks) {
+    // (WIDE: whole steps, so a step lies in the row or it does not, and its offset is scalar: 777 rows x 4096 x 4096 26.7 -> 25.1 us)
+    const __amdgpu_buffer_rsrc_t r = rsrc(base, !WIDE || 4 * step < blocks ? bytes : 0);
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
-      const int piece = (u * 256 + (threadIdx.x & 255)) % kPieces;
-      const bool in = 4 * step + piece * 16 / O::kBlock < blocks;
-      data[D][u] = load16(r, in ? off[u] + step * kRow : kOutside);
+      if constexpr (WIDE) {
+        data[D][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[u], 4 * step < blocks ? step * kRow : 0, 0));
+      } else {
+        const int piece = (u * 256 + (threadIdx.x & 255)) % kPieces;
+        const bool in = 4 * step + piece * 16 / O::kBlock < blocks;
+        data[D][u] = load16(r, in ? off[u] + step * kRow : kOutside);
+      }
     }
     if constexpr (!WIDE) {
 #pragma unroll
