@@ -661,11 +661,14 @@ def _separate(t: torch.Tensor) -> bool:
   return t.numel() == 0 or (sh >= D and st >= (H - 1) * sh + D) or (st >= D and sh >= (T - 1) * st + D)
 
 
+_increment_version = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
+
 def _written(*ts) -> None:
   """Tells autograd that the caller's tensors were written: a graph that saved their old values refuses to use them."""
   for t in ts:
     if t is not None and not t.is_inference():
-      torch.autograd.graph.increment_version(t)
+      _increment_version((t,))
 
 
 def _offsets32(t: torch.Tensor, name: str, n: int | None, what: str) -> torch.Tensor:
@@ -978,15 +981,17 @@ def _cache(what, k_pages, v_pages, page_table, len_k, B, dtype):
     raise ValueError(f"{what}: head dim {D} is not a multiple of 8 up to 128")
   row = Hkv * D
   packed = (R * row, row, D)
-  ks = packed if k_pages.is_contiguous() else _page_strides(k_pages)
-  vs = packed if v_pages.is_contiguous() else _page_strides(v_pages)
-  for t, s in ((k_pages, ks), (v_pages, vs)):
-    if (s[0] | s[1] | s[2] | t.data_ptr() >> 1) % 8 or not D <= s[1] < 1 << 24 or t.stride(3) != 1:
+  strides = []
+  for t in (k_pages, v_pages):
+    whole = t.is_contiguous()
+    s = packed if whole else _page_strides(t)
+    if t.data_ptr() % 16 or not (row < 1 << 24 if whole else not (s[0] | s[1] | s[2]) % 8 and D <= s[1] < 1 << 24 and t.stride(3) == 1):
       raise ValueError(f"{what}: pages must lie in 16-byte aligned rows of 1 dim after another, strides {t.stride()}")
+    strides.append(s)
   tshape = page_table.shape
-  if page_table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != B or tshape[1] < 1:
+  cols = tshape[1] if len(tshape) == 2 else 0
+  if page_table.dtype is not torch.int32 or cols < 1 or tshape[0] != B:
     raise ValueError(f"{what}: page_table must be int32 [{B}, pages of a sequence], got {page_table.dtype} {tuple(tshape)}")
-  cols = tshape[1]
   if cols * R > 1 << 30:
     raise ValueError(f"{what}: {cols} pages of {R} rows a sequence exceed 2^30")
   ts = cols
@@ -995,7 +1000,7 @@ def _cache(what, k_pages, v_pages, page_table, len_k, B, dtype):
       page_table = page_table.contiguous()
     elif B > 1:
       ts = page_table.stride(0)
-  return ks, vs, page_table, ts, cols, _offsets32(len_k, "len_k", B, what)
+  return *strides, page_table, ts, cols, _offsets32(len_k, "len_k", B, what)
 
 
 def _token_rows(t: torch.Tensor, T: int, H: int, D: int):
@@ -1040,12 +1045,15 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
   if len_new is not None:
     len_new = _offsets32(len_new, "len_new", B, what)
   ks, vs, table, ts, cols, len_k = _cache(what, k_pages, v_pages, page_table, len_k, B, dtype)
-  if k_pages.shape[2:] != k.shape[1:] or Hkv * D > 1 << 24:
+  P, R, Hp, Dp = k_pages.shape
+  if Hp != Hkv or Dp != D or Hkv * D > 1 << 24:
     raise ValueError(f"{what}: {tuple(k.shape[1:])} of k and v against {tuple(k_pages.shape[2:])} of the pages (2^24 elements at most)")
+  packed = (R * Hkv * D, Hkv * D, D)
   for pages, strides in ((k_pages, ks), (v_pages, vs)):
-    if not (pages.is_contiguous() or _apart(zip(pages.shape, (*strides, 1)))):
+    if strides != packed and not _apart(zip(pages.shape, (*strides, 1))):
       raise ValueError(f"{what}: pages must hold every element once")
-  (k0, k1), (v0, v1) = _span(k_pages), _span(v_pages)
+  k0, v0 = k_pages.data_ptr(), v_pages.data_ptr()
+  k1, v1 = (p + 2 * ((P - 1) * s[0] + (R - 1) * s[1] + (Hkv - 1) * s[2] + D) for p, s in ((k0, ks), (v0, vs)))
   if not (k1 <= v0 or v1 <= k0 or (ks == vs and _apart([*zip(k_pages.shape, (*ks, 1)), (2, abs(v0 - k0) // 2)]))):
     raise ValueError(f"{what}: k_pages and v_pages overlap")
   k, kp, sk = _token_rows(k, T, Hkv, D)                        # (copies overlap nothing)
@@ -1054,8 +1062,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     end = p + 2 * ((T - 1) * st + (Hkv - 1) * sh + D)
     if T > 0 and not ((end <= k0 or k1 <= p) and (end <= v0 or v1 <= p)):
       raise ValueError(f"{what}: pages overlap k or v")
-  a = _lib.paged_write_args(B, Hkv, D, T, k_pages.shape[0], k_pages.shape[1], cols, kp, *sk, vp, *sv, k_pages.data_ptr(), *ks,
-                            v_pages.data_ptr(), *vs, cu.data_ptr(), _vp(len_new) or 0, len_k.data_ptr(), table.data_ptr(), ts)
+  a = _lib.paged_write_args(B, Hkv, D, T, P, R, cols, kp, *sk, vp, *sv, k0, *ks, v0, *vs, cu.data_ptr(), _vp(len_new) or 0,
+                            len_k.data_ptr(), table.data_ptr(), ts)
   _launch(_lib.load().sf_hip_paged_write_fwd, k, "sf_hip_paged_write_fwd", C.byref(a))
   _written(k_pages, v_pages)
 
@@ -1273,8 +1281,13 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
     y_rs = y.stride(0) if M > 1 else N
     if y_rs < N:
       raise ValueError(f"{what}: out must hold every element once")
-    if not all(_spans_apart(y, t) for t in (xc, xs, wc, ws, bias) if t is not None):
-      raise ValueError(f"{what}: out overlaps an input")
+    y0 = y.data_ptr()
+    y1 = y0 + (2 * ((M - 1) * y_rs + N) if M > 0 else 0)
+    for t in (xc, xs, wc, ws, bias):
+      if t is not None:
+        t0, t1 = _span(t)
+        if t0 < y1 and y0 < t1:
+          raise ValueError(f"{what}: out overlaps an input")
   if M == 0:
     return result
   a = _lib.mx_linear_args(M, N, K, xf, wf, _ELEMENT_TYPES[dtype], xc.data_ptr(), x_rs, xs.data_ptr(), xs_rs, wc.data_ptr(), w_rs,
@@ -1288,13 +1301,22 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
   return result
 
 
-def _norm_outputs(what, x, x2, r2, weight, aligned, out, out_sum):
-  """Checks given outputs of the norm; returns the rows and row strides of both."""
-  shape, dtype, Cn, R = x.shape, x.dtype, x.shape[-1], x2.shape[0]
-  rows = []
-  for o, name in ((out, "out"), (out_sum, "out_sum")):
+def _norm_outputs(what, shape, dtype, R, inputs, weight, aligned, outs):
+  """Checks given outputs of the norm (None: not given) against the inputs' rows, (pointer, row stride); returns the pointer and
+  row stride of each."""
+  Cn = shape[-1]
+  size = 4 if dtype is torch.float32 else 2
+  width, rows = Cn * size, []
+
+  def apart(p, sp, q, sq):
+    """Whether rows lie apart: separate ranges, or separate columns of rows of one width."""
+    sp, sq = sp * size, sq * size
+    if p + (R - 1) * sp + width <= q or q + (R - 1) * sq + width <= p:
+      return True
+    return sp == sq and width <= sp and width <= (p - q) % sp <= sp - width
+
+  for o, name in zip(outs, ("out", "out_sum")):
     if o is None:
-      rows.append((None, 0))
       continue
     if o.shape != shape or o.dtype is not dtype or (Cn > 1 and o.stride(-1) != 1):
       raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)} with a unit last stride")
@@ -1302,17 +1324,18 @@ def _norm_outputs(what, x, x2, r2, weight, aligned, out, out_sum):
       o2 = o if o.ndim == 2 else o.view(-1, Cn)
     except RuntimeError:
       raise ValueError(f"{what}: the leading dims of {name} must be one stride apart") from None
-    if R > 1 and o2.stride(0) < Cn:
+    p, st = o2.data_ptr(), o2.stride(0) if R > 1 else Cn
+    if st < Cn:
       raise ValueError(f"{what}: {name} must hold every element once")
-    if aligned and (o2.data_ptr() % 16 or (R > 1 and o2.stride(0) * o2.element_size() % 16)):
+    if aligned and (p % 16 or st * size % 16):
       raise ValueError(f"{what}: {name} must lie in 16-byte aligned rows with a microscaled output")
-    same = lambda i: o2.data_ptr() == i.data_ptr() and (R <= 1 or o2.stride(0) == i.stride(0))
-    if not all(same(i) or _disjoint(o2.unsqueeze(1), i.unsqueeze(1)) for i in (x2, r2) if i is not None):
-      raise ValueError(f"{what}: outputs may be x or residual itself, and overlap nothing else")
-    if weight is not None and not _spans_apart(o2, weight):
-      raise ValueError(f"{what}: an output overlaps the weight")
-    rows.append((o2, o2.stride(0) if R > 1 else Cn))
-  if out is not None and out_sum is not None and not _disjoint(rows[0][0].unsqueeze(1), rows[1][0].unsqueeze(1)):
+    if R > 0:
+      if not all((p == q and (st == sq or R == 1)) or apart(p, st, q, sq) for q, sq in inputs):
+        raise ValueError(f"{what}: outputs may be x or residual itself, and overlap nothing else")
+      if weight is not None and not (p + (R - 1) * st * size + width <= weight.data_ptr() or weight.data_ptr() + 4 * Cn <= p):
+        raise ValueError(f"{what}: an output overlaps the weight")
+    rows.append((p, st))
+  if R > 0 and len(rows) == 2 and not apart(*rows[0], *rows[1]):
     raise ValueError(f"{what}: out and out_sum overlap")
   return rows
 
@@ -1353,26 +1376,32 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
       weight = _f32(weight)
   aligned = output is not None
   x2, x_rs = _rows2(x, aligned)
-  R = x2.shape[0]
-  r2, r_rs = (None, 0) if residual is None else _rows2(residual, aligned)
-  y2, y_rs, h2, h_rs, total, codes = out, 0, None, 0, None, None
+  R, x_p = x2.shape[0], x2.data_ptr()
+  r2, r_p, r_rs = None, 0, 0
+  if residual is not None:
+    r2, r_rs = _rows2(residual, aligned)
+    r_p = r2.data_ptr()
+  y_p, y_rs, h_p, h_rs, total, codes = 0, 0, 0, 0, out_sum, None
   if out is not None or out_sum is not None:
-    (y2, y_rs), (h2, h_rs) = _norm_outputs(what, x, x2, r2, weight, aligned, out, out_sum)
-    total = out_sum
+    rows = _norm_outputs(what, shape, dtype, R, ((x_p, x_rs),) if r2 is None else ((x_p, x_rs), (r_p, r_rs)), weight, aligned, (out, out_sum))
+    if out is not None:
+      y_p, y_rs = rows[0]
+    if out_sum is not None:
+      h_p, h_rs = rows[-1]
   if output is not None:
     result = codes = _empty_microscaled(shape[:-1], Cn, output, dev)
   elif out is None:
-    result = y2 = _fresh(x)
-    y_rs = Cn
+    result = _fresh(x)
+    y_p, y_rs = result.data_ptr(), Cn
   else:
     result = out
   if residual is not None and out_sum is None:
-    total = h2 = _fresh(x)
-    h_rs = Cn
+    total = _fresh(x)
+    h_p, h_rs = total.data_ptr(), Cn
   if R == 0:
     return result, total
-  a = _lib.add_rms_norm_args(R, Cn, _ELEMENT_TYPES[dtype], 0 if output is None else _FORMATS[output], eps, x2.data_ptr(), x_rs,
-                             _vp(r2) or 0, r_rs, _vp(weight) or 0, _vp(h2) or 0, h_rs, _vp(y2) or 0, y_rs,
+  a = _lib.add_rms_norm_args(R, Cn, _ELEMENT_TYPES[dtype], 0 if output is None else _FORMATS[output], eps, x_p, x_rs, r_p, r_rs,
+                             _vp(weight) or 0, h_p, h_rs, y_p, y_rs,
                              *((0, 0, 0, 0) if codes is None else
                                (codes.codes.data_ptr(), codes.codes.shape[-1], codes.scales.data_ptr(), Cn // 32)))
   _launch(_lib.load().sf_hip_add_rms_norm_fwd, x2, "sf_hip_add_rms_norm_fwd", C.byref(a))
