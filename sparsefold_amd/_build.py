@@ -1,4 +1,5 @@
-"""Builds ``libsparsefold_hip.so`` from ``csrc/*.hip`` for gfx950 with hipcc.
+"""Builds ``libsparsefold_hip.so`` from ``csrc/*.hip`` for gfx950 with hipcc, and from ``csrc/front.cpp`` the host module
+through which the serving-step calls reach it from Python.
 
 Objects are compiled in parallel into ``sparsefold_amd/_build/`` and linked in-tree, so the
 library travels with the source tree.  Every HIP translation unit is compiled with the
@@ -10,7 +11,10 @@ import concurrent.futures
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
+
+from sparsefold_amd._lib import front_path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
@@ -45,12 +49,31 @@ def _compile(src: Path) -> Path:
   return obj
 
 
+def _build_front() -> Path:
+  """The host module, for the torch that is installed (its name holds the version)."""
+  import torch
+  path, cc = front_path(), hipcc()
+  at = Path(torch.__file__).resolve().parent
+  includes = [at / "include", at / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], Path(cc).resolve().parents[1] / "include"]
+  tmp = path.with_suffix(".so.tmp")
+  cmd = [cc, "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *(f"-isystem{i}" for i in includes),
+         str(CSRC / "front.cpp"), "-o", str(tmp), f"-L{at / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+  res = subprocess.run(cmd, capture_output=True, text=True)
+  if res.returncode != 0:
+    raise RuntimeError(f"hipcc failed for front.cpp:\n{res.stderr}")
+  os.replace(tmp, path)
+  return path
+
+
 def build(verbose: bool = False) -> Path:
-  """Compiles every ``csrc/*.hip`` and links ``libsparsefold_hip.so``; returns its path."""
+  """Compiles every ``csrc/*.hip`` and links ``libsparsefold_hip.so``, and builds the host module; returns the library's path."""
   BUILD.mkdir(exist_ok=True)
   srcs = sorted(CSRC.glob("*.hip"))
-  with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+  with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+    front = ex.submit(_build_front)
     objs = list(ex.map(_compile, srcs))
+    front.result()
   tmp = LIB.with_suffix(".so.tmp")
   cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
   res = subprocess.run(cmd, capture_output=True, text=True)

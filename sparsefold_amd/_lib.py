@@ -7,6 +7,8 @@ loudly: there is no fallback implementation behind this module.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 from struct import Struct
 
@@ -331,6 +333,32 @@ def load() -> C.CDLL:
     raise RuntimeError(f"libsparsefold_hip ABI version {ver} != expected {ABI_VERSION}")
   _lib = lib
   return lib
+
+
+def front_path() -> Path:
+  """The host module for the installed torch, whose version it is bound to."""
+  import torch
+  return LIB_PATH.with_name(f"_front-{torch.__version__}.so")
+
+
+# The entries that the host module calls, in its order.
+_FRONT = ("sf_hip_last_error", "sf_hip_add_rms_norm_fwd", "sf_hip_mx_encode_fwd", "sf_hip_mx_decode_fwd", "sf_hip_mx_linear_workspace_bytes", "sf_hip_mx_linear_fwd",
+          "sf_hip_paged_write_fwd", "sf_hip_paged_attention_workspace_bytes", "sf_hip_paged_attention_fwd")
+
+
+def front(lib: C.CDLL, microscaled: type):
+  """The host module (csrc/front.cpp) bound to the library, or None where none is built for this torch: its calls then go
+  through ctypes, with the same results."""
+  path = front_path()
+  if not path.exists():
+    return None
+  loader = importlib.machinery.ExtensionFileLoader("sparsefold_amd._front", str(path))
+  module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+  loader.exec_module(module)
+  if module.abi_version != ABI_VERSION:
+    raise RuntimeError(f"{path.name} is built for ABI version {module.abi_version}, not {ABI_VERSION}")
+  module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in _FRONT), microscaled)
+  return module
 
 
 def last_error() -> str:

@@ -136,3 +136,139 @@ def test_captured_step(formats):
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
     assert torch.equal(layer.k, eager.k) and torch.equal(layer.v, eager.v)
     assert torch.isfinite(out[0]).all()
+
+
+# ---- the calls' common form in the host module against ctypes ------------------------------------------
+
+def forms(name):
+  """Arguments that the host module takes."""
+  g = torch.Generator().manual_seed(5)
+  r = lambda *s, dtype=BF: torch.randn(*s, generator=g).to(dtype).to(DEV)
+  if name == "norm":
+    for shape, dtype in (((8, 512), BF), ((3, 5, 96), torch.float16), ((64,), torch.float32), ((2, 77), BF)):
+      x = r(*shape, dtype=dtype)
+      for residual in (r(*shape, dtype=dtype), None):
+        for weight in (r(shape[-1], dtype=torch.float32), None):
+          for output in (None,) if shape[-1] % 32 else (None, "mxfp8", "mxfp4"):
+            yield (x, residual, weight, 1e-5, output), lambda: ops.add_rms_norm(x, residual, weight, eps=1e-5, output=output)
+  elif name == "quantize":
+    for shape, dtype in (((7, 64), BF), ((2, 3, 128), torch.float32), ((32,), torch.float16)):
+      x = r(*shape, dtype=dtype)
+      for f in ("mxfp8", "mxfp4"):
+        yield (x, f), lambda: ops.mx_quantize(x, f)
+  elif name == "dequantize":
+    for shape in ((7, 64), (2, 3, 128), (32,)):
+      for f in ("mxfp8", "mxfp4"):
+        x = ops.mx_quantize(r(*shape), f)
+        for dtype in (BF, torch.float16, torch.float32):
+          yield (*x, dtype), lambda: ops.mx_dequantize(x, dtype)
+  elif name == "linear":
+    for lead, N, K in (((8,), 100, 256), ((2, 100), 256, 4096), ((), 64, 64), ((300,), 64, 1024)):
+      for fx, fw in mx.FORMATS:
+        x, w = ops.mx_quantize(r(*lead, K), fx), ops.mx_quantize(r(N, K), fw)
+        for bias in (r(N, dtype=torch.float32), None):
+          for dtype in (BF, torch.float16):
+            yield (*x, *w, bias, dtype), lambda: ops.mx_linear(x, w, bias, dtype=dtype)
+  else:
+    for T, lens, heads, layout in ((4, [1, 1, 1, 1], 4, "rows"), (90, [70, 1, 0, 19], 2, "both"), (1, [1, 0, 0, 0], 1, "heads")):
+      shape = {"rows": (40, 16, heads, 64), "both": (40, 2, 16, heads, 64), "heads": (40, heads, 16, 64)}[layout]
+      kp, vp = r(*shape), r(*shape)
+      kp, vp = (kp[:, 0], kp[:, 1]) if layout == "both" else (kp.transpose(1, 2), vp.transpose(1, 2)) if layout == "heads" else (kp, vp)
+      table = torch.randperm(40, generator=g)[:32].view(4, 8).to(torch.int32).to(DEV)
+      cu, len_k = attention.offsets(lens), ints([100, 30, 128, 19])
+      y = r(T, 6 * heads, 64)
+      q, k, v = y[:, :4 * heads], y[:, 4 * heads:5 * heads], y[:, 5 * heads:]
+      if name == "write":
+        for new in (None, ints([1, 1, 0, 3])):
+          def write():
+            a, b = kp.clone(), vp.clone()
+            ops.paged_cache_write(k, v, kp, vp, table, cu, len_k, len_new=new)
+            result = kp.clone(), vp.clone()
+            kp.copy_(a)
+            vp.copy_(b)
+            return result
+          yield (k, v, kp, vp, table, cu, len_k, new), write
+      else:
+        for len_q, causal, scale, most in ((None, True, None, None), (ints([1, 1, 0, 3]), False, 0.25, 128), (None, True, None, 0)):
+          def call():                                          # (rows outside every sequence hold what was there)
+            out = ops.paged_attention(q, kp, vp, table, cu, len_k, len_q=len_q, causal=causal, scale=scale, max_len=most)
+            rows = [i for b, n in enumerate(lens) for i in range(int(cu[b]), int(cu[b]) + (n if len_q is None else min(n, int(len_q[b]))))]
+            return out[rows]
+          yield (q, kp, vp, table, cu, len_k, len_q, causal, scale, most), call
+
+
+CALLS = {"norm": "add_rms_norm", "quantize": "mx_quantize", "dequantize": "mx_dequantize", "linear": "mx_linear", "write": "paged_cache_write", "attention": "paged_attention"}
+
+
+def flat(x):
+  return [t for y in x for t in flat(y)] if isinstance(x, tuple) else [] if x is None else [x]
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_host_module_gives_what_ctypes_gives(name, monkeypatch):
+  ops._library()
+  assert ops._front
+  for args, call in forms(name):
+    assert getattr(ops._front, CALLS[name])(*args) is not None
+    got = call()
+    with monkeypatch.context() as m:
+      m.setattr(ops, "_front", False)
+      want = call()
+    for a, b in zip(flat(got), flat(want), strict=True):
+      assert a.shape == b.shape and a.dtype is b.dtype and a.is_contiguous() and torch.equal(a.view(torch.uint8) if a.dim() else a, b.view(torch.uint8) if b.dim() else b)
+    assert type(got) is type(want)
+
+
+def test_host_module_leaves_other_forms():
+  """Copies, gradients, other devices' and wrong tensors are the wrapper's."""
+  ops._library()
+  x, w = torch.randn(4, 64, device=DEV, dtype=BF), torch.ones(64, device=DEV)
+  norm_of = ops._front.add_rms_norm
+  for args in ((x.t()[:4].contiguous().t(), None, None, 1e-6, None), (x[:, ::2], None, None, 1e-6, None), (x, x[:2], None, 1e-6, None), (x, x.half(), None, 1e-6, None),
+               (x, None, w[:32], 1e-6, None), (x, None, w.double(), 1e-6, None), (x, None, w, -1.0, None), (x, None, w, math.nan, None), (x, None, w, 1, None),
+               (x, None, w, 1e-6, "mxfp6"), (x, None, w, 1e-6, True), (x.cpu(), None, None, 1e-6, None), (x, x.cpu(), None, 1e-6, None), (x, None, None, 1e-6), ("x", None, w, 1e-6, None),
+               (x[:0], None, None, 1e-6, None), (x.clone().requires_grad_(), None, None, 1e-6, None), (x, None, w.clone().requires_grad_(), 1e-6, None),
+               (x[1:].view(-1)[4:36 + 96].view(2, 64), None, None, 1e-6, "mxfp8")):
+    assert norm_of(*args) is None
+  with pytest.raises(ValueError, match="no backward pass"):
+    ops.add_rms_norm(x.clone().requires_grad_(), None, None)
+  with torch.no_grad():
+    assert norm_of(x.clone().requires_grad_(), None, None, 1e-6, None) is not None
+  import torch.autograd.forward_ad as fwd
+  with fwd.dual_level():
+    assert norm_of(fwd.make_dual(torch.ones(2, 32, device=DEV), torch.ones(2, 32, device=DEV)), None, None, 1e-6, None) is None
+  with torch.inference_mode():
+    y, _ = ops.add_rms_norm(x, None, w)
+    assert y.is_inference()
+
+
+def test_writes_are_seen_by_autograd():
+  """Pages that a graph saved are not used behind a write, by either way."""
+  ops._library()
+  k = torch.randn(1, 2, 64, device=DEV, dtype=BF)
+  pages = [torch.zeros(2, 16, 2, 64, device=DEV, dtype=BF) for _ in range(2)]
+  before = [t._version for t in pages]
+  ops.paged_cache_write(k, k, *pages, ints([[0]]), ints([0, 1]), ints([1]))
+  assert all(t._version > n for t, n in zip(pages, before))
+  s = torch.ones((), device=DEV, requires_grad=True)
+  loss = (pages[0].float() * s).sum() + (pages[0] * s.to(BF)).sum()
+  ops.paged_cache_write(k, k, *pages, ints([[0]]), ints([0, 1]), ints([1]))
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    loss.backward()
+
+
+def test_streams_of_the_host_module():
+  """A call runs on the stream that is current where it is made."""
+  ops._library()
+  side = torch.cuda.Stream()
+  x = torch.randn(4096, 4096, device=DEV).to(BF)
+  want = ops.mx_quantize(x.clone().mul_(2), "mxfp8")
+  torch.cuda.synchronize()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    for _ in range(20):
+      x.mul_(1.0)
+    x.mul_(2)
+    got = ops.mx_quantize(x, "mxfp8")
+  side.synchronize()
+  assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(got.scales.view(torch.uint8), want.scales.view(torch.uint8))

@@ -487,3 +487,27 @@ def test_lds_slots_are_a_permutation(pieces):
     for p in range(2):
       assert len({half(r, p) % 256 for r in range(r0, r0 + 16)}) == 16
   assert len({half(r, p) for r in range(256) for p in range(2)}) == 512
+
+
+def test_host_module_does_nothing_of_other_forms(lib):
+  """The host module answers None to host tensors, other objects and other numbers of arguments."""
+  front = _lib.front(lib, ops.Microscaled)
+  assert front is not None and front.abi_version == _lib.ABI_VERSION
+  x = torch.zeros(2, 64, dtype=BF)
+  pages = torch.zeros(5, 16, 2, 32, dtype=BF)
+  for name, args in (("add_rms_norm", (x, x, None, 1e-6, None)), ("mx_quantize", (x, "mxfp8")), ("mx_linear", (*mx(2, 64), *mx(3, 64), None, BF)), ("mx_dequantize", (*mx(2, 64), BF)),
+                     ("paged_cache_write", (torch.zeros(6, 2, 32, dtype=BF),) * 2 + (pages, pages.clone(), torch.zeros(2, 3, dtype=I32), ints(0, 2, 6), ints(20, 40), None)),
+                     ("paged_attention", (torch.zeros(6, 4, 32, dtype=BF), pages, pages, torch.zeros(2, 3, dtype=I32), ints(0, 2, 6), ints(20, 40), None, True, None, None))):
+    call = getattr(front, name)
+    assert call(*args) is None and call(*args[:-1]) is None and call(*args, None) is None and call() is None
+    for i in range(len(args)):
+      for other in (None, 3, "x", x, object()):
+        assert call(*args[:i], other, *args[i + 1:]) is None
+  for args in ((), (1,) * 9, (0,) * 9 + (object,), ("a",) * 9 + (object,)):
+    with pytest.raises((TypeError, ValueError)):
+      front.bind(*args)
+
+
+def test_without_the_host_module(monkeypatch, lib):
+  monkeypatch.setattr(_lib, "front_path", lambda: _lib.LIB_PATH.with_name("absent.so"))
+  assert _lib.front(lib, ops.Microscaled) is None
