@@ -62,19 +62,42 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
 
-// Four scale bytes of a row from byte `at` on, of which `left` are in the row; one load where `wide` (rows of whole
-// aligned words).
-__device__ __forceinline__ uint32_t scales4(__amdgpu_buffer_rsrc_t r, uint32_t row, int at, int left, bool wide) {
-  if (wide) return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(left > 0 ? row + at : kOutside), 0, 0);
-  uint32_t v = 0;
+// Scales of rows from `base` on, of any alignment: a buffer of whole words, which may end up to three bytes past the last row's (in
+// one word with it) and begin as many before the first's; skip: where that row begins.
+struct Scales {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t skip;
+  __device__ __forceinline__ void init(const void* base, int64_t bytes) {
+    skip = (uint32_t)(uintptr_t)base & 3;
+    r = rsrc((const uint8_t*)base - skip, (skip + bytes + 3) & ~(int64_t)3);
+  }
+  // 16 scales from byte `row` + `at` on, zeros from the row's n-th on (at, n uniform): five words, shifted into place
+  __device__ __forceinline__ u32x4 load(uint32_t row, int at, int n) const {
+    const uint32_t off = skip + row + at, word = off & ~3u;
+    const int left = n - at;
+    uint32_t w[5];
+    if (left >= 20) {                                        // (uniform)
+      const u32x4 q = load16(r, word);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    v |= (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)(e < left ? row + at + e : kOutside), 0, 0) << (8 * e);
-  return v;
-}
+      for (int e = 0; e < 4; ++e) w[e] = q[e];
+      w[4] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(word + 16), 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 5; ++e)
+        w[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(4 * e < left + 3 ? word + 4 * e : kOutside), 0, 0);
+    }
+    u32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int valid = min(max(left - 4 * e, 0), 4);
+      v[e] = __builtin_amdgcn_alignbyte(w[e + 1], w[e], off) & (valid == 4 ? ~0u : (1u << (8 * valid)) - 1);
+    }
+    return v;
+  }
+};
 
 struct Extra {
-  bool wide;           // scales load as words
+  bool wide;           // whole steps of 128 k, scales of 16 blocks load as aligned words
   bool vector;         // rows of y take 16-byte stores
   int slices, steps;   // mx_tile_kernel: parts of k, steps of each
   float* part;         // [slices][M][N]
@@ -109,8 +132,7 @@ struct StepOperand {
   u32x4 c[SI][O::kParts];
   uint32_t scale[SI];                                        // of instruction s: byte 0
   // row: byte offset of the lane's row of codes, srow of scales; blocks: of the row
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rc, __amdgpu_buffer_rsrc_t rs, uint32_t row, uint32_t srow, int b0, int blocks,
-                                       bool wide) {
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rc, const Scales& rs, uint32_t row, uint32_t srow, int b0, int blocks, bool wide) {
     const int g = (threadIdx.x >> 4) & 3;
 #pragma unroll
     for (int s = 0; s < SI; ++s)
@@ -120,12 +142,17 @@ struct StepOperand {
         c[s][p] = load16(rc, b0 + at / O::kBlock < blocks ? row + b0 * O::kBlock + at : kOutside);
       }
     if (SI == 4 && wide && b0 + 16 <= blocks) {              // (uniform)
-      const u32x4 w = load16(rs, srow + b0);
+      const u32x4 w = load16(rs.r, srow + b0);
 #pragma unroll
       for (int s = 0; s < SI; ++s) scale[s] = w[s];
-    } else {
+    } else if (SI < 4 && wide) {
 #pragma unroll
-      for (int s = 0; s < SI; ++s) scale[s] = scales4(rs, srow, b0 + 4 * s, blocks - b0 - 4 * s, wide);
+      for (int s = 0; s < SI; ++s)
+        scale[s] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rs.r, (int)(b0 + 4 * s < blocks ? srow + b0 + 4 * s : kOutside), 0, 0);
+    } else {
+      const u32x4 w = rs.load(srow, b0, blocks);
+#pragma unroll
+      for (int s = 0; s < SI; ++s) scale[s] = w[s];
     }
 #pragma unroll
     for (int s = 0; s < SI; ++s) scale[s] >>= 8 * g;
@@ -142,9 +169,10 @@ __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_a
   const int n0 = blockIdx.x * (16 * NT);
   const int blocks = a.K / 32, wrows = min(16 * NT, a.N - n0), mrows = (int)a.M;
   const __amdgpu_buffer_rsrc_t wc = rsrc((const uint8_t*)a.w + n0 * a.w_rs, (wrows - 1) * a.w_rs + (int64_t)blocks * Op<FW>::kBlock),
-                               ws = rsrc((const uint8_t*)a.w_scales + n0 * a.ws_rs, (wrows - 1) * a.ws_rs + blocks),
-                               xc = rsrc(a.x, (mrows - 1) * a.x_rs + (int64_t)blocks * Op<FX>::kBlock),
-                               xs = rsrc(a.x_scales, (mrows - 1) * a.xs_rs + blocks);
+                               xc = rsrc(a.x, (mrows - 1) * a.x_rs + (int64_t)blocks * Op<FX>::kBlock);
+  Scales ws, xs;
+  ws.init((const uint8_t*)a.w_scales + n0 * a.ws_rs, (wrows - 1) * a.ws_rs + blocks);
+  xs.init(a.x_scales, (mrows - 1) * a.xs_rs + blocks);
   // (rows past the end repeat the last: their results are not stored)
   f32x4v acc[NT][MT];
 #pragma unroll
@@ -196,54 +224,39 @@ __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_a
 // ---------------------------------------------------------------------------------------
 // Tiles of 128 x 128, waves of 64 x 64, steps of 128 k through two LDS buffers.
 // ---------------------------------------------------------------------------------------
-// WIDE: scales load 16 at a time, 512 k, a row a thread, and go through LDS too (a word of 32 rows a load and step touched as many
-// lines as the codes); and two steps are in flight.  Else byte by byte and one step ahead (registers).
+// Scales load 16 at a time, 512 k, a row a thread, and go through LDS too (a word of 32 rows a load and step touched as many lines as
+// the codes); two steps are in flight.  WIDE: whole steps, so a step lies in the row or it does not, and its offset is scalar (777 rows x
+// 4096 x 4096 26.7 -> 25.1 us); else a lane's piece of the last one may lie outside, and scales are shifted into place (byte
+// by byte, 777 rows x 4096 x 4064 took 67.6 us in place of 30.8).
 template <class F, bool WIDE>
 struct TileOperand {
   using O = Op<F>;
   static constexpr int kRow = 4 * O::kBlock, kPieces = kRow / 16, kBytes = 128 * kRow, kN = kBytes / 16 / 256;
   // the 16 rows that are read together fall on 16 different 16-byte slots of the banks' 256 bytes
   static __device__ __forceinline__ int slot(int row, int piece) { return O::k8 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
-  static constexpr int kAhead = WIDE ? 2 : 1;                // steps in flight
-  u32x4 data[kAhead][kN];
-  uint32_t sdata[2];                                         // (not WIDE)
-  __amdgpu_buffer_rsrc_t rs;
+  u32x4 data[2][kN];                                         // of two steps
   const uint8_t* base;
   int bytes;
-  uint32_t off[kN], srow[2];
-  __device__ __forceinline__ void init(const void* codes, int64_t c_rs, const void* scales, int64_t s_rs, int64_t row0, int64_t rows, int blocks,
-                                       int wave_row) {
+  uint32_t off[kN];
+  __device__ __forceinline__ void init(const void* codes, int64_t c_rs, int64_t row0, int64_t rows, int blocks) {
     const int64_t n = rows - row0 < 128 ? rows - row0 : 128;
     base = (const uint8_t*)codes + row0 * c_rs;
     bytes = (int)((n - 1) * c_rs + (int64_t)blocks * O::kBlock);
-    rs = rsrc((const uint8_t*)scales + row0 * s_rs, (n - 1) * s_rs + blocks);
 #pragma unroll
     for (int u = 0; u < kN; ++u) {
       const int idx = u * 256 + (threadIdx.x & 255), row = idx / kPieces;
       off[u] = row < n ? (uint32_t)(row * c_rs) + idx % kPieces * 16 : kOutside;
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) srow[t] = (uint32_t)(min((int64_t)(wave_row + 32 * t + (threadIdx.x & 31)), n - 1) * s_rs);
   }
   // step `step` into slot D, zeros past the last
   template <int D>
   __device__ __forceinline__ void load(int step, int blocks) {
-    // (WIDE: whole steps, so a step lies in the row or it does not, and its offset is scalar: 777 rows x 4096 x 4096 26.7 -> 25.1 us)
-    const __amdgpu_buffer_rsrc_t r = rsrc(base, !WIDE || 4 * step < blocks ? bytes : 0);
+    const bool some = 4 * step < blocks;                     // (uniform)
+    const bool in = 4 * step + (int)(threadIdx.x % kPieces) * 16 / O::kBlock < blocks;
+    const __amdgpu_buffer_rsrc_t r = rsrc(base, some ? bytes : 0);
 #pragma unroll
-    for (int u = 0; u < kN; ++u) {
-      if constexpr (WIDE) {
-        data[D][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[u], 4 * step < blocks ? step * kRow : 0, 0));
-      } else {
-        const int piece = (u * 256 + (threadIdx.x & 255)) % kPieces;
-        const bool in = 4 * step + piece * 16 / O::kBlock < blocks;
-        data[D][u] = load16(r, in ? off[u] + step * kRow : kOutside);
-      }
-    }
-    if constexpr (!WIDE) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) sdata[t] = scales4(rs, srow[t], 4 * step, blocks - 4 * step, false);
-    }
+    for (int u = 0; u < kN; ++u)
+      data[D][u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(WIDE || in ? off[u] : kOutside), some ? step * kRow : 0, 0));
   }
   template <int D>
   __device__ __forceinline__ void store(uint8_t* lds) const {
@@ -269,8 +282,7 @@ template <class E, class FX, class FW, bool WIDE, int KG>
 __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear_args a, const Extra ex) {
   using X = TileOperand<FX, WIDE>;
   using W = TileOperand<FW, WIDE>;
-  constexpr int kAhead = X::kAhead;
-  constexpr int kScales = WIDE ? 256 * 16 : 0;               // of the 128 rows of x, then of w
+  constexpr int kScales = 256 * 16;                          // of the 128 rows of x, then of w
   constexpr int kGroup = 2 * (X::kBytes + W::kBytes) + 2 * kScales;
   __shared__ __attribute__((aligned(1024))) uint8_t shared[KG * kGroup];
   const int tid = threadIdx.x & 255, lane = tid & 63, half = lane >> 5, li = lane & 31;
@@ -284,8 +296,8 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
   const int s0 = first + kg * per, s1 = s0 + count, last = min(blocks, 4 * min(s0 + per, end));
   X x;
   W w;
-  x.init(a.x, a.x_rs, a.x_scales, a.xs_rs, m0, a.M, blocks, 64 * wm);
-  w.init(a.w, a.w_rs, a.w_scales, a.ws_rs, n0, a.N, blocks, 64 * wn);
+  x.init(a.x, a.x_rs, m0, a.M, blocks);
+  w.init(a.w, a.w_rs, n0, a.N, blocks);
   f32x16v acc[2][2];                                         // [columns][rows]
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -293,22 +305,26 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // scales 16 g .. + 15 of the thread's row, zeros past the row's end
+  // scales 16 g .. + 15 of the thread's row of x or w, zeros past the row's end
   u32x4 group = {0, 0, 0, 0};
+  const bool of_x = wave < 2;
+  const int srows = (int)(of_x ? min(a.M - m0, (int64_t)128) : (int64_t)min(a.N - n0, 128));
+  const int64_t s_rs = of_x ? a.xs_rs : a.ws_rs;
+  const uint32_t srow = (uint32_t)(min(tid & 127, srows - 1) * s_rs);
+  Scales sr;
+  sr.init(of_x ? (const uint8_t*)a.x_scales + m0 * a.xs_rs : (const uint8_t*)a.w_scales + n0 * a.ws_rs, (srows - 1) * s_rs + blocks);
   const auto load_group = [&](int g) __attribute__((always_inline)) {
-    const bool of_x = wave < 2;
-    const int row = tid & 127;
-    const __amdgpu_buffer_rsrc_t r = of_x ? x.rs : w.rs;
-    const uint32_t at = (uint32_t)((of_x ? min((int64_t)row, a.M - m0 - 1) * a.xs_rs : (int64_t)min(row, a.N - n0 - 1) * a.ws_rs)) + 16 * g;
-    if (16 * g + 16 <= blocks) {
-      group = load16(r, at);
+    if constexpr (!WIDE) {
+      group = sr.load(srow, 16 * g, blocks);
+    } else if (16 * g + 16 <= blocks) {
+      group = load16(sr.r, srow + 16 * g);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        group[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)(16 * g + 4 * e < blocks ? at + 4 * e : kOutside), 0, 0);
+        group[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr.r, (int)(16 * g + 4 * e < blocks ? srow + 16 * g + 4 * e : kOutside), 0, 0);
     }
   };
-  // Step s is stored to one of two LDS buffers while the next kAhead steps are in flight to registers: one barrier a step (the
+  // Step s is stored to one of two LDS buffers while the next two steps are in flight to registers: one barrier a step (the
   // buffer's readers, two steps before, passed the last one).
   const auto step = [&](auto constant, int s) __attribute__((always_inline)) {
     constexpr int D = decltype(constant)::value;
@@ -318,29 +334,19 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
     w.template store<D>(wt);
     uint32_t cx[2], cw[2];
     uint8_t* const sc = smem + 2 * (X::kBytes + W::kBytes) + ((s >> 2) & 1) * kScales;
-    if constexpr (WIDE) {
-      if (D == 0 && (s & 3) == 0) {                          // (uniform; the buffer's readers are four steps behind)
-        st16(sc + tid * 16, group);
-        load_group((s >> 2) + 1);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        cx[t] = x.sdata[t] >> (8 * half);                    // chunk 0: byte 0, chunk 1: byte 2
-        cw[t] = w.sdata[t] >> (8 * half);
-      }
+    if (D == 0 && (s & 3) == 0) {                            // (uniform; the buffer's readers are four steps behind)
+      st16(sc + tid * 16, group);
+      load_group((s >> 2) + 1);
     }
     lds_only_barrier();
-    x.template load<D>(s + kAhead, last);                    // (zeros past the slice's end)
-    w.template load<D>(s + kAhead, last);
+    x.template load<D>(s + 2, last);                         // (zeros past the slice's end)
+    w.template load<D>(s + 2, last);
     __builtin_amdgcn_sched_barrier(0);                       // (moved behind the products, the loads were waited for at once)
-    if constexpr (WIDE) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t* const at = sc + 4 * (s & 3) + (32 * t + li) * 16;
-        cx[t] = *reinterpret_cast<const uint32_t*>(at + 64 * wm * 16) >> (8 * half);
-        cw[t] = *reinterpret_cast<const uint32_t*>(at + (128 + 64 * wn) * 16) >> (8 * half);
-      }
+    for (int t = 0; t < 2; ++t) {                            // (chunk 0: byte 0, chunk 1: byte 2)
+      const uint8_t* const at = sc + 4 * (s & 3) + (32 * t + li) * 16;
+      cx[t] = *reinterpret_cast<const uint32_t*>(at + 64 * wm * 16) >> (8 * half);
+      cw[t] = *reinterpret_cast<const uint32_t*>(at + (128 + 64 * wn) * 16) >> (8 * half);
     }
     i32x8 wo[2][2], xo[2][2];
 #pragma unroll
@@ -360,18 +366,14 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
       for (int j = 0; j < 2; ++j) acc[i][j] = mfma32s<FW, FX, 2, 2>(wo[1][i], xo[1][j], acc[i][j], cw[i], cx[j]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  if constexpr (WIDE) load_group(s0 >> 2);
+  load_group(s0 >> 2);                                       // (s0 is a multiple of 4)
   x.template load<0>(s0, last);
   w.template load<0>(s0, last);
-  if constexpr (WIDE) {
-    x.template load<1>(s0 + 1, last);
-    w.template load<1>(s0 + 1, last);
-    for (int s = s0; s < s1; s += 2) {                       // (a step too many adds zeros)
-      step(std::integral_constant<int, 0>{}, s);
-      step(std::integral_constant<int, 1>{}, s + 1);
-    }
-  } else {
-    for (int s = s0; s < s1; ++s) step(std::integral_constant<int, 0>{}, s);
+  x.template load<1>(s0 + 1, last);
+  w.template load<1>(s0 + 1, last);
+  for (int s = s0; s < s1; s += 2) {                         // (a step too many adds zeros)
+    step(std::integral_constant<int, 0>{}, s);
+    step(std::integral_constant<int, 1>{}, s + 1);
   }
   // (the products' lanes all take part: no part of them is moved into the branches below)
 #pragma unroll
@@ -573,7 +575,7 @@ void route(const sf_mx_linear_args* a, Route& r) {
   r.stream = a->M <= 32 || (a->M <= 64 && stream_cost(a) <= tile_cost(a, steps, slices));
   if (r.stream || r.large) slices = 1;
   // two groups of waves where a workgroup has a CU to itself (777 rows above: 29.2 us with one)
-  r.groups = r.ex.wide && tiles * slices <= 256 && steps / slices >= 8 ? 2 : 1;
+  r.groups = tiles * slices <= 256 && steps / slices >= 8 ? 2 : 1;
   const int whole = 4 * r.groups;                            // (whole groups of scales for each group of waves)
   r.ex.steps = ((steps + slices - 1) / slices + whole - 1) / whole * whole;
   r.ex.slices = (steps + r.ex.steps - 1) / r.ex.steps;
@@ -611,9 +613,9 @@ int launch(const sf_mx_linear_args* a, const Route& r, hipStream_t st) {
     return launch<E, FX, FW>(&b, rest, st);
   }
   const dim3 grid((unsigned)((a->N + 127) / 128), (unsigned)gm, (unsigned)r.ex.slices);
-  if (!r.ex.wide) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, false, 1>), grid, dim3(256), 0, st, *a, r.ex);
-  else if (r.groups == 1) hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true, 1>), grid, dim3(256), 0, st, *a, r.ex);
-  else hipLaunchKernelGGL((mx_tile_kernel<E, FX, FW, true, 2>), grid, dim3(512), 0, st, *a, r.ex);
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256 * r.groups), 0, st, *a, r.ex); };
+  if (r.ex.wide) r.groups == 1 ? go(mx_tile_kernel<E, FX, FW, true, 1>) : go(mx_tile_kernel<E, FX, FW, true, 2>);
+  else r.groups == 1 ? go(mx_tile_kernel<E, FX, FW, false, 1>) : go(mx_tile_kernel<E, FX, FW, false, 2>);
   const int rc = sf_check_launch("mx_tile_kernel");
   if (rc || r.ex.slices == 1) return rc;
   const int64_t all = a->M * a->N;

@@ -301,3 +301,22 @@ def test_capture_replay_and_streams(M, N, K):
       got.append(step())
   torch.cuda.synchronize()
   assert all(torch.equal(t, want) for t in got)
+
+
+@pytest.mark.parametrize("formats", FORMATS, ids="-".join)
+@pytest.mark.parametrize("K", [96, 512, 640, 1056, 2080, 4064, 4096])
+@pytest.mark.parametrize("M", [5, 30, 50, 200, 700])
+def test_scales_of_any_alignment(M, K, formats):
+  """Scales that begin at any byte, rows of any length, beside bytes that stand for NaN, which are no part of any row."""
+  x, w = operands(M, 150, K, formats, M + K)
+  want = ops.mx_linear(x, w)
+  for at, pad in ((1, 3), (2, 4), (3, 1)):
+    def moved(q):
+      rows = torch.full((q.scales.shape[0], K // 32 + pad), 255, dtype=torch.uint8, device=DEV)
+      room = torch.full((rows.numel() + 8,), 255, dtype=torch.uint8, device=DEV)[at:at + rows.numel()].view(rows.shape)
+      room[:, :K // 32] = q.scales.view(torch.uint8)
+      return ops.Microscaled(q.codes, room[:, :K // 32])
+    y = ops.mx_linear(moved(x), moved(w))
+    check(y, x, w)
+    if K % 128:
+      assert torch.equal(y, want)
