@@ -124,7 +124,8 @@ __device__ __forceinline__ void put(const sf_mx_linear_args& a, bool vector, int
 
 // ---------------------------------------------------------------------------------------
 // Few rows of x.  A wave's step is 512 k, four instructions.  An instruction's loads take 64 consecutive bytes of each of 16 rows
-// (lanes that each read on along their own 64 bytes would touch four times the lines).
+// (lanes that each read on along their own 64 bytes would touch four times the lines).  Bound by the codes of w and by
+// latency: 8 rows x 12288 x 4096 of 8 and 4 bits 9.7 us, 26 MB that a large copy's rate moves in 5.7.
 // ---------------------------------------------------------------------------------------
 template <class F, int SI>
 struct StepOperand {
@@ -222,7 +223,8 @@ __global__ __launch_bounds__(64 * KW) void mx_stream_kernel(const sf_mx_linear_a
 }
 
 // ---------------------------------------------------------------------------------------
-// Tiles of 128 x 128, waves of 64 x 64, steps of 128 k through two LDS buffers.
+// Tiles of 128 x 128, waves of 64 x 64, steps of 128 k through two LDS buffers.  777 rows x 4096 x 4096 of 8 bits 25 us, 0.58 us
+// a step and 8 of start and end; with half the loads, LDS reads or products the loop takes 4 to 10% less each.
 // ---------------------------------------------------------------------------------------
 // Scales load 16 at a time, 512 k, a row a thread, and go through LDS too (a word of 32 rows a load and step touched as many lines as
 // the codes); two steps are in flight.  WIDE: whole steps, so a step lies in the row or it does not, and its offset is scalar (777 rows x
