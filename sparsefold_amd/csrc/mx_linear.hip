@@ -100,6 +100,7 @@ struct Extra {
   bool wide;           // whole steps of 128 k, scales of 16 blocks load as aligned words
   bool vector;         // rows of y take 16-byte stores
   int slices, steps;   // mx_tile_kernel: parts of k, steps of each
+  bool banded;         // its tiles in bands
   float* part;         // [slices][M][N]
 };
 
@@ -291,8 +292,20 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
   const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   uint8_t* const smem = shared + kg * kGroup;
-  const int n0 = blockIdx.x * 128;
-  const int64_t m0 = (int64_t)blockIdx.y * 128;
+  int bx = blockIdx.y, by = blockIdx.x;                      // tile row and column
+  if (ex.banded) {
+    // Workgroup b is assumed to run on XCD b % 8: each takes a contiguous range of tiles, in bands of kBand tile rows, so that those
+    // it runs together form a block of both operands (8000 x 8000 x 8096 of 8 and 8, 4 and 4 bits 1003, 642 -> 779, 496 us; up
+    // to 1024 tiles the divisions cost more: 300 x 2048 x 1536 of 8 and 4 bits 11.2 -> 11.6).
+    constexpr int kBand = 8;
+    const int gx = gridDim.y, gy = gridDim.x, total = gx * gy, id = bx * gy + by;
+    const int t = (id & 7) * (total >> 3) + min(id & 7, total & 7) + (id >> 3);
+    const int band = t / (kBand * gy), q = t - band * kBand * gy, bh = min(kBand, gx - band * kBand);
+    by = q / bh;
+    bx = band * kBand + q - by * bh;
+  }
+  const int n0 = by * 128;
+  const int64_t m0 = (int64_t)bx * 128;
   const int blocks = a.K / 32, per = ex.steps / KG, first = blockIdx.z * ex.steps, end = min(first + ex.steps, (blocks + 3) / 4);
   const int count = min(per, end - first);                   // steps of every group (the last one's may add zeros)
   const int s0 = first + kg * per, s1 = s0 + count, last = min(blocks, 4 * min(s0 + per, end));
@@ -615,7 +628,9 @@ int launch(const sf_mx_linear_args* a, const Route& r, hipStream_t st) {
     return launch<E, FX, FW>(&b, rest, st);
   }
   const dim3 grid((unsigned)((a->N + 127) / 128), (unsigned)gm, (unsigned)r.ex.slices);
-  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256 * r.groups), 0, st, *a, r.ex); };
+  Extra ex = r.ex;
+  ex.banded = gm * grid.x > 1024 && gm * grid.x < 1 << 30;
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256 * r.groups), 0, st, *a, ex); };
   if (r.ex.wide) r.groups == 1 ? go(mx_tile_kernel<E, FX, FW, true, 1>) : go(mx_tile_kernel<E, FX, FW, true, 2>);
   else r.groups == 1 ? go(mx_tile_kernel<E, FX, FW, false, 1>) : go(mx_tile_kernel<E, FX, FW, false, 2>);
   const int rc = sf_check_launch("mx_tile_kernel");

@@ -320,3 +320,32 @@ def test_scales_of_any_alignment(M, K, formats):
     check(y, x, w)
     if K % 128:
       assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("M,N,K", [(4230, 4200, 160), (131200, 130, 96), (140, 131100, 96)])
+def test_many_tiles(M, N, K):
+  """More tiles than the grid's order is kept for; sampled rows and columns."""
+  x, w = operands(M, N, K, FORMATS[1], M)
+  y = ops.mx_linear(x, w)
+  assert torch.isfinite(y).all()
+  rows = torch.tensor(sorted({0, 1, 127, 128, M // 2, M - 129, M - 1}), device=DEV)
+  cols = torch.tensor(sorted({0, 63, 127, 128, N // 2, N - 129, N - 1}), device=DEV)
+  take = lambda q, i: ops.Microscaled(q.codes.view(torch.uint8)[i].view(q.codes.dtype), q.scales.view(torch.uint8)[i])
+  check(y[rows][:, cols], take(x, rows), take(w, cols))
+  for part, xs, ws in ((y[:, cols], x, take(w, cols)), (y[rows], take(x, rows), w)):
+    a, b = ops.mx_dequantize(xs, torch.float32).cpu(), ops.mx_dequantize(ws, torch.float32).cpu()
+    want, size = a.double() @ b.double().T, a.abs().double() @ b.abs().double().T
+    tol = size * ((K + 8) * 2.0 ** -23 + 14 * 2.0 ** -13) * (1 + 2.0 ** -8) + (2.0 ** -8 + 2.0 ** -24) * want.abs()
+    assert ((part.cpu().double() - want).abs() <= tol).all()
+
+
+def test_more_rows_than_a_launch_holds():
+  """Rows past 65535 tiles of 128 are a launch of their own; rows at the seam."""
+  M, N, K = 65535 * 128 + 133, 8, 32
+  g = torch.Generator(device=DEV).manual_seed(0)
+  x = ops.mx_quantize(torch.randn(M, K, generator=g, device=DEV), "mxfp4")
+  w = ops.mx_quantize(torch.randn(N, K, generator=g, device=DEV), "mxfp4")
+  y = ops.mx_linear(x, w)
+  for rows in (slice(0, 3), slice(M - 140, M - 130), slice(M - 3, M)):
+    check(y[rows], ops.Microscaled(x.codes[rows], x.scales.view(torch.uint8)[rows]), w)
+  assert torch.isfinite(y).all()

@@ -511,3 +511,18 @@ def test_host_module_does_nothing_of_other_forms(lib):
 def test_without_the_host_module(monkeypatch, lib):
   monkeypatch.setattr(_lib, "front_path", lambda: _lib.LIB_PATH.with_name("absent.so"))
   assert _lib.front(lib, ops.Microscaled) is None
+
+
+@pytest.mark.parametrize("gx,gy", [(1, 1025), (1030, 1), (9, 131), (40, 32), (63, 64), (129, 8), (33, 33), (7, 300)])
+def test_bands_reach_every_tile_once(gx, gy):
+  """mx_tile_kernel's order of tiles beyond 1024 of them."""
+  total, band_rows, seen = gx * gy, 8, set()
+  for i in range(total):
+    t = (i & 7) * (total >> 3) + min(i & 7, total & 7) + (i >> 3)
+    band = t // (band_rows * gy)
+    q, bh = t - band * band_rows * gy, min(band_rows, gx - band * band_rows)
+    by = q // bh
+    bx = band * band_rows + q - by * bh
+    assert 0 <= bx < gx and 0 <= by < gy
+    seen.add((bx, by))
+  assert len(seen) == total
