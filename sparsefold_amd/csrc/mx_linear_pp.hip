@@ -14,7 +14,7 @@
 // Results are rounded in registers, brought together to whole lines by exchanges between lanes, and stored by buffer stores
 // that drop what lies outside, so that their number, which the waits count, does not depend on the tile.
 //
-// 8192^3: 287 us of 4 bits, 3.8 PFLOP/s, and 493 of 8 bits, 2.2 (products of 8192^3 in bf16: 1.3; matrix instructions alone, on random codes in
+// 8192^3: 287 to 312 us of 4 bits, 3.5 to 3.8 PFLOP/s, by the card, and 489 of 8 bits, 2.25 (products of 8192^3 in bf16: 1.3; matrix instructions alone, on random codes in
 // registers: 6.8 and 3.8, clocks held by power).  With all codes zero 236 us of 4 bits and 425 of 8; of 4 bits without the copies 240.  4 waves of 128 x 128, one a
 // SIMD, with the next step's reads between the products took as long (283 us, 285 with copies of whole 128-byte lines), so the two
 // groups' alternation is not what bounds it; L2 hits 90% of the lines asked for.
