@@ -67,7 +67,7 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int t) {
 __global__ __launch_bounds__(256) void paged_write_kernel(const sf_paged_write_args a, const int log_rows) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = a.D / 8, pieces = a.Hkv * per;              // 16-byte pieces of a row
-  const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) << log_rows;
+  const int64_t t0 = ((int64_t)workgroup() * 4 + wave) << log_rows;
   const int lanes = 64 >> log_rows, mine = lane / lanes;
   char* kd = nullptr;
   char* vd = nullptr;
@@ -133,8 +133,8 @@ extern "C" int sf_hip_paged_write_fwd(const sf_paged_write_args* a, void* stream
   const int pieces = a->Hkv * (a->D / 8);
   int log_rows = 0;
   while (log_rows < 4 && pieces << (log_rows + 1) <= 64) ++log_rows;
-  const int64_t rows = 4ll << log_rows;
-  hipLaunchKernelGGL(paged_write_kernel, dim3((unsigned)((a->T + rows - 1) / rows)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), *a,
-                     log_rows);
+  const int64_t rows = 4ll << log_rows, wgs = (a->T + rows - 1) / rows;          // (up to 2^28)
+  const dim3 grid = wgs <= kGridX ? dim3((unsigned)wgs) : dim3(kGridX, (unsigned)((wgs + kGridX - 1) / kGridX));
+  hipLaunchKernelGGL(paged_write_kernel, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), *a, log_rows);
   return sf_check_launch("paged_write_kernel");
 }

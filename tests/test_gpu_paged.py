@@ -348,3 +348,21 @@ def test_agrees_with_the_packed_attention():
     _, tol = definition(q[at:at + n], k[ak:ak + m], v[ak:ak + m], True, 1 / math.sqrt(96))
     assert ((a[at:at + n] - b[at:at + n]).cpu().double().abs() <= 2 * tol).all()
     at, ak = at + n, ak + m
+
+
+def test_write_of_more_tokens_than_a_launch_dimension_holds():
+  """2^26 tokens, a wave each: 2^24 workgroups of 256 threads and some.  The pages of the first tokens, of those on both sides of each grid
+  row's border and of the last are in the cache; the others are dropped."""
+  T, Hk, D, R = (1 << 26) + 5, 5, 128, 64
+  rows = torch.empty((T + 1) * 8 + Hk * D, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(4))
+  k, v = (rows.as_strided((T, Hk, D), (8, D, 1), at) for at in (0, 8))                # (rows that overlap)
+  used = sorted({0} | {p for b in range(1, 5) for p in ((b << 24) // R - 1, (b << 24) // R)} | {T // R})
+  table = torch.full((1, T // R + 1), -1, dtype=torch.int32, device=DEV)
+  table[0, used] = torch.arange(len(used), dtype=torch.int32, device=DEV)
+  kc, vc = (torch.full((len(used) + 1, R, Hk, D), 3.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+  ops.paged_cache_write(k, v, kc, vc, table, ints([0, T]), ints([T]))
+  for i, p in enumerate(used):
+    n = min(R, T - p * R)
+    for cache, new in ((kc, k), (vc, v)):
+      assert torch.equal(cache[i, :n], new[p * R:p * R + n]) and (cache[i, n:] == 3).all()
+  assert (kc[-1] == 3).all() and (vc[-1] == 3).all()
