@@ -88,6 +88,15 @@ PyObject* failed(const char* what, int rc) {
   return PyErr_Format(PyExc_RuntimeError, "%s failed (status %d): %s", what, rc, text);
 }
 
+// Without the interpreter's lock, as ctypes calls the library: allocations and launches may wait for the device (a full queue, whose
+// host functions may want the lock).
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // Codes and scales for rows like x's.
 struct Coded {
   at::Tensor codes, scales;
@@ -137,25 +146,32 @@ PyObject* add_rms_norm(PyObject* const* arg) {
   a.weight = weight ? weight->data_ptr<float>() : nullptr;
   a.x_rs = a.r_rs = a.h_rs = a.y_rs = C;
   const bool coded = arg[4] != Py_None;
-  at::Tensor y, h;
-  std::optional<Coded> q;
   if (coded) {
     a.format = format_of(arg[4]);
     need(C % 32 == 0 && al16(a.x) && al16(a.residual));
-    q.emplace(x, a.format);
-    a.codes = q->codes.data_ptr();
-    a.c_rs = q->codes.size(-1);
-    a.scales = q->scales.data_ptr();
-    a.s_rs = C / 32;
-  } else {
-    y = empty(x.sizes(), x, x.scalar_type());
-    a.y = y.data_ptr();
   }
-  if (res) {
-    h = empty(x.sizes(), x, x.scalar_type());
-    a.sum = h.data_ptr();
+  at::Tensor y, h;
+  std::optional<Coded> q;
+  int rc;
+  {
+    const Unlocked unlocked;
+    if (coded) {
+      q.emplace(x, a.format);
+      a.codes = q->codes.data_ptr();
+      a.c_rs = q->codes.size(-1);
+      a.scales = q->scales.data_ptr();
+      a.s_rs = C / 32;
+    } else {
+      y = empty(x.sizes(), x, x.scalar_type());
+      a.y = y.data_ptr();
+    }
+    if (res) {
+      h = empty(x.sizes(), x, x.scalar_type());
+      a.sum = h.data_ptr();
+    }
+    rc = entry.add_rms_norm(&a, call.stream());
   }
-  if (const int rc = entry.add_rms_norm(&a, call.stream())) return failed("sf_hip_add_rms_norm_fwd", rc);
+  if (rc) return failed("sf_hip_add_rms_norm_fwd", rc);
   PyObject* const first = coded ? q->wrap() : THPVariable_Wrap(y);
   PyObject* const second = res ? THPVariable_Wrap(h) : Py_NewRef(Py_None);
   PyObject* const both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
@@ -176,13 +192,19 @@ PyObject* mx_quantize(PyObject* const* arg) {
   a.R = x.numel() / a.K;
   a.x = x.data_ptr();
   a.x_rs = a.K;
-  const Coded q(x, a.format);
-  a.codes = q.codes.data_ptr();
-  a.c_rs = q.codes.size(-1);
-  a.scales = q.scales.data_ptr();
-  a.s_rs = a.K / 32;
-  if (const int rc = entry.mx_encode(&a, call.stream())) return failed("sf_hip_mx_encode_fwd", rc);
-  return q.wrap();
+  std::optional<Coded> q;
+  int rc;
+  {
+    const Unlocked unlocked;
+    q.emplace(x, a.format);
+    a.codes = q->codes.data_ptr();
+    a.c_rs = q->codes.size(-1);
+    a.scales = q->scales.data_ptr();
+    a.s_rs = a.K / 32;
+    rc = entry.mx_encode(&a, call.stream());
+  }
+  if (rc) return failed("sf_hip_mx_encode_fwd", rc);
+  return q->wrap();
 }
 
 // Checks codes and scales; returns K, and the format and rows.
@@ -215,14 +237,20 @@ PyObject* mx_dequantize(PyObject* const* arg) {
   need(a.R >= 1);
   c10::SmallVector<int64_t, 6> s(codes.sizes().begin(), codes.sizes().end());
   s.back() = a.K;
-  const at::Tensor x = empty(s, codes, type);
-  a.x = x.data_ptr();
   a.x_rs = a.K;
   a.codes = codes.data_ptr();
   a.c_rs = codes.size(-1);
   a.scales = scales.data_ptr();
   a.s_rs = a.K / 32;
-  if (const int rc = entry.mx_decode(&a, call.stream())) return failed("sf_hip_mx_decode_fwd", rc);
+  at::Tensor x;
+  int rc;
+  {
+    const Unlocked unlocked;
+    x = empty(s, codes, type);
+    a.x = x.data_ptr();
+    rc = entry.mx_decode(&a, call.stream());
+  }
+  if (rc) return failed("sf_hip_mx_decode_fwd", rc);
   return THPVariable_Wrap(x);
 }
 
@@ -253,13 +281,18 @@ PyObject* mx_linear(PyObject* const* arg) {
   a.bias = bias ? bias->data_ptr<float>() : nullptr;
   c10::SmallVector<int64_t, 6> s(xc.sizes().begin(), xc.sizes().end());
   s.back() = N;
-  const at::Tensor y = empty(s, xc, type);
-  a.y = y.data_ptr();
   a.y_rs = N;
-  const size_t bytes = entry.mx_linear_bytes(&a);
-  at::Tensor work;
-  if (bytes > 0) work = empty({(int64_t)bytes}, xc, at::kByte);
-  if (const int rc = entry.mx_linear(&a, bytes > 0 ? work.data_ptr() : nullptr, bytes, call.stream())) return failed("sf_hip_mx_linear_fwd", rc);
+  at::Tensor y, work;
+  int rc;
+  {
+    const Unlocked unlocked;
+    y = empty(s, xc, type);
+    a.y = y.data_ptr();
+    const size_t bytes = entry.mx_linear_bytes(&a);
+    if (bytes > 0) work = empty({(int64_t)bytes}, xc, at::kByte);
+    rc = entry.mx_linear(&a, bytes > 0 ? work.data_ptr() : nullptr, bytes, call.stream());
+  }
+  if (rc) return failed("sf_hip_mx_linear_fwd", rc);
   return THPVariable_Wrap(y);
 }
 
@@ -354,7 +387,12 @@ PyObject* paged_cache_write(PyObject* const* arg) {
     return (end <= k0 || k1 <= p) && (end <= v0 || v1 <= p);
   };
   need(read(a.k, a.k_s) && read(a.v, a.v_s));
-  if (const int rc = entry.paged_write(&a, call.stream())) return failed("sf_hip_paged_write_fwd", rc);
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = entry.paged_write(&a, call.stream());
+  }
+  if (rc) return failed("sf_hip_paged_write_fwd", rc);
   for (const at::Tensor* t : {&kp, &vp})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return Py_NewRef(Py_True);
@@ -393,15 +431,19 @@ PyObject* paged_attention(PyObject* const* arg) {
   a.q = token_rows(q, a.q_s);
   a.k = kp.data_ptr();
   a.v = vp.data_ptr();
-  const at::Tensor out = empty(q.sizes(), q, q.scalar_type());
-  a.out = out.data_ptr();
   a.o_s[0] = H * a.D;
   a.o_s[1] = a.D;
-  const size_t bytes = entry.paged_attention_bytes(&a);
-  at::Tensor work;
-  if (bytes > 0) work = empty({(int64_t)bytes}, q, at::kByte);
-  if (const int rc = entry.paged_attention(&a, bytes > 0 ? work.data_ptr() : nullptr, bytes, call.stream()))
-    return failed("sf_hip_paged_attention_fwd", rc);
+  at::Tensor out, work;
+  int rc;
+  {
+    const Unlocked unlocked;
+    out = empty(q.sizes(), q, q.scalar_type());
+    a.out = out.data_ptr();
+    const size_t bytes = entry.paged_attention_bytes(&a);
+    if (bytes > 0) work = empty({(int64_t)bytes}, q, at::kByte);
+    rc = entry.paged_attention(&a, bytes > 0 ? work.data_ptr() : nullptr, bytes, call.stream());
+  }
+  if (rc) return failed("sf_hip_paged_attention_fwd", rc);
   return THPVariable_Wrap(out);
 }
 
