@@ -49,16 +49,30 @@ def _compile(src: Path) -> Path:
   return obj
 
 
-def _build_front() -> Path:
-  """The host module, for the torch that is installed (its name holds the version)."""
+def _front_includes() -> list[Path] | None:
+  """Where the host module's headers are (torch's for HIP, Python's, HIP's), or None where one kind is not installed."""
+  try:
+    import torch
+  except ImportError:
+    return None
+  at = Path(torch.__file__).resolve().parent / "include"
+  python = Path(sysconfig.get_paths()["include"])
+  if not (at / "c10/hip/HIPStream.h").exists() or not (python / "Python.h").exists():
+    return None
+  return [at, at / "torch/csrc/api/include", python, Path(hipcc()).resolve().parents[1] / "include"]
+
+
+def _build_front() -> Path | None:
+  """The host module, for the torch that is installed (its name holds the version); None where its headers are not."""
+  includes = _front_includes()
+  if includes is None:
+    return None
   import torch
-  path, cc = front_path(), hipcc()
-  at = Path(torch.__file__).resolve().parent
-  includes = [at / "include", at / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], Path(cc).resolve().parents[1] / "include"]
+  path = front_path()
   tmp = path.with_suffix(".so.tmp")
-  cmd = [cc, "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+  cmd = [hipcc(), "-x", "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", *(f"-isystem{i}" for i in includes),
-         str(CSRC / "front.cpp"), "-o", str(tmp), f"-L{at / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+         str(CSRC / "front.cpp"), "-o", str(tmp), f"-L{includes[0].parent / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
   res = subprocess.run(cmd, capture_output=True, text=True)
   if res.returncode != 0:
     raise RuntimeError(f"hipcc failed for front.cpp:\n{res.stderr}")
@@ -67,13 +81,15 @@ def _build_front() -> Path:
 
 
 def build(verbose: bool = False) -> Path:
-  """Compiles every ``csrc/*.hip`` and links ``libsparsefold_hip.so``, and builds the host module; returns the library's path."""
+  """Compiles every ``csrc/*.hip`` and links ``libsparsefold_hip.so``, and builds the host module; returns the library's path.
+
+  The library needs neither torch nor Python: it is linked whatever becomes of the host module.  Without the headers of both there is no
+  host module (its calls then go through ctypes); one that does not compile is an error."""
   BUILD.mkdir(exist_ok=True)
   srcs = sorted(CSRC.glob("*.hip"))
   with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
     front = ex.submit(_build_front)
     objs = list(ex.map(_compile, srcs))
-    front.result()
   tmp = LIB.with_suffix(".so.tmp")
   cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
   res = subprocess.run(cmd, capture_output=True, text=True)
@@ -82,6 +98,11 @@ def build(verbose: bool = False) -> Path:
   os.replace(tmp, LIB)
   if verbose:
     print(f"built {LIB}")
+  if front.result() is None:
+    for stale in LIB.parent.glob("_front-*.so"):               # (of an earlier build, perhaps for another library)
+      stale.unlink()
+    if verbose:
+      print("no host module: torch's or Python's C++ headers are not installed")
   return LIB
 
 
