@@ -63,7 +63,7 @@ def _front_includes() -> list[Path] | None:
 
 
 def _build_front() -> Path | None:
-  """The host module, for the torch that is installed (its name holds the version); None where its headers are not."""
+  """The host module, for this Python and the torch that is installed (its name holds their versions); None where its headers are not."""
   includes = _front_includes()
   if includes is None:
     return None

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import sysconfig
 from pathlib import Path
 from struct import Struct
 
@@ -336,9 +337,9 @@ def load() -> C.CDLL:
 
 
 def front_path() -> Path:
-  """The host module for the installed torch, whose version it is bound to."""
+  """The host module for this Python and the installed torch: it is bound to the versions of both."""
   import torch
-  return LIB_PATH.with_name(f"_front-{torch.__version__}.so")
+  return LIB_PATH.with_name(f"_front-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
 
 
 # The entries that the host module calls, in its order.
@@ -347,7 +348,7 @@ _FRONT = ("sf_hip_last_error", "sf_hip_add_rms_norm_fwd", "sf_hip_mx_encode_fwd"
 
 
 def front(lib: C.CDLL, microscaled: type):
-  """The host module (csrc/front.cpp) bound to the library, or None where none is built for this torch: its calls then go
+  """The host module (csrc/front.cpp) bound to the library, or None where none is built for this Python and torch: its calls then go
   through ctypes, with the same results."""
   path = front_path()
   if not path.exists():

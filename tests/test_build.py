@@ -53,3 +53,12 @@ def test_host_module_that_does_not_compile(tree):
   with pytest.raises(RuntimeError, match="front.cpp"):
     _build.build()
   assert tree.lib.exists() and not tree.front.exists()
+
+
+def test_host_modules_of_two_pythons_stand_side_by_side(monkeypatch):
+  """One torch version, two interpreters, one tree: each looks for a module of its own."""
+  from sparsefold_amd import _lib
+  here = _lib.front_path()
+  assert any(str(here).endswith(s) and s != ".so" for s in _lib.importlib.machinery.EXTENSION_SUFFIXES)
+  monkeypatch.setattr(_lib.sysconfig, "get_config_var", lambda name: ".cpython-399-x86_64-linux-gnu.so")
+  assert _lib.front_path() != here and _lib.front_path().parent == here.parent
