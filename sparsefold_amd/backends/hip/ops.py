@@ -1235,8 +1235,8 @@ def mx_quantize(x: torch.Tensor, format: str = "mxfp4") -> Microscaled:
     raise ValueError(f"{what}: format {format!r} is not 'mxfp8' or 'mxfp4'")
   if x.dtype not in _ELEMENT_TYPES:
     raise ValueError(f"{what}: x must be bfloat16, float16 or float32, got {x.dtype}")
-  if x.ndim < 1 or x.shape[-1] < 32 or x.shape[-1] % 32 != 0:
-    raise ValueError(f"{what}: the last dim must be a multiple of 32, got {tuple(x.shape)}")
+  if x.ndim < 1 or not 32 <= x.shape[-1] < 1 << 31 or x.shape[-1] % 32 != 0:
+    raise ValueError(f"{what}: the last dim must be a multiple of 32 below 2^31, got {tuple(x.shape)}")
   K = x.shape[-1]
   result = _empty_microscaled(x.shape[:-1], K, format, dev)
   if x.numel() == 0:
@@ -1260,6 +1260,8 @@ def mx_dequantize(x: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.
   if dtype not in _ELEMENT_TYPES:
     raise ValueError(f"{what}: dtype must be bfloat16, float16 or float32, got {dtype}")
   format, R, K, codes, c_rs, scales, s_rs = _microscaled(x, "x", what)
+  if K >= 1 << 31:
+    raise ValueError(f"{what}: rows of {K}, not below 2^31")
   out = _empty_rows(x.codes.shape[:-1], K, dtype, codes.device)
   if R == 0:
     return out
