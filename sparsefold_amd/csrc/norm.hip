@@ -247,9 +247,13 @@ int launch_rows(const sf_add_rms_norm_args* a, hipStream_t st) {
   if (pieces <= 1024) return launch<E, F, 256, 4>(a, st);
   if (pieces <= 2048) return launch<E, F, 1024, 2>(a, st);
   const unsigned grid = (unsigned)(a->R < 4096 ? a->R : 4096);
-  if constexpr (std::is_same<F, Same>::value) hipLaunchKernelGGL(add_rms_norm_any_kernel<E>, dim3(grid), dim3(256), 0, st, *a);
-  else hipLaunchKernelGGL((add_rms_norm_long_kernel<E, F>), dim3(grid), dim3(256), 0, st, *a);
-  return sf_check_launch("add_rms_norm_any_kernel");
+  if constexpr (std::is_same<F, Same>::value) {
+    hipLaunchKernelGGL(add_rms_norm_any_kernel<E>, dim3(grid), dim3(256), 0, st, *a);
+    return sf_check_launch("add_rms_norm_any_kernel");
+  } else {
+    hipLaunchKernelGGL((add_rms_norm_long_kernel<E, F>), dim3(grid), dim3(256), 0, st, *a);
+    return sf_check_launch("add_rms_norm_long_kernel");
+  }
 }
 
 template <class E>
