@@ -104,23 +104,21 @@ struct Extra {
   float* part;         // [slices][M][N]
 };
 
-// 4 or 8 consecutive results of row m from column n on.
+// 4 consecutive results of row m from column n on, or one.
 template <class E, int C>
 __device__ __forceinline__ void put(const sf_mx_linear_args& a, bool vector, int64_t m, int n, const float (&v)[C]) {
   typename E::T* const y = (typename E::T*)a.y + m * a.y_rs + n;
-  if (vector && n + C <= a.N) {
-    if constexpr (C == 8) {
-      st16(y, E::pack(v));
-    } else if constexpr (C == 4) {
+  if constexpr (C == 4) {
+    if (vector && n + C <= a.N) {
       const float w[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
       const u32x4 p = E::pack(w);
       *reinterpret_cast<u32x2*>(y) = u32x2{p[0], p[1]};
+      return;
     }
-  } else {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (n + c < a.N) E::store(y + c, v[c]);
   }
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (n + c < a.N) E::store(y + c, v[c]);
 }
 
 // ---------------------------------------------------------------------------------------
