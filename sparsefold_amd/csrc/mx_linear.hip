@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "index.h"
 #include "mx.h"
 #include "mx_linear.h"
 
@@ -233,8 +234,7 @@ template <class F, bool WIDE>
 struct TileOperand {
   using O = Op<F>;
   static constexpr int kRow = 4 * O::kBlock, kPieces = kRow / 16, kBytes = 128 * kRow, kN = kBytes / 16 / 256;
-  // the 16 rows that are read together fall on 16 different 16-byte slots of the banks' 256 bytes
-  static __device__ __forceinline__ int slot(int row, int piece) { return O::k8 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
+  static __device__ __forceinline__ int slot(int row, int piece) { return tile_slot<O::k8>(row, piece); }
   u32x4 data[2][kN];                                         // of two steps
   const uint8_t* base;
   int bytes;
@@ -292,15 +292,11 @@ __global__ __launch_bounds__(256 * KG, 2) void mx_tile_kernel(const sf_mx_linear
   uint8_t* const smem = shared + kg * kGroup;
   int bx = blockIdx.y, by = blockIdx.x;                      // tile row and column
   if (ex.banded) {
-    // Workgroup b is assumed to run on XCD b % 8: each takes a contiguous range of tiles, in bands of kBand tile rows, so that those
-    // it runs together form a block of both operands (8000 x 8000 x 8096 of 8 and 8, 4 and 4 bits 1003, 642 -> 779, 496 us; up
-    // to 1024 tiles the divisions cost more: 300 x 2048 x 1536 of 8 and 4 bits 11.2 -> 11.6).
-    constexpr int kBand = 8;
-    const int gx = gridDim.y, gy = gridDim.x, total = gx * gy, id = bx * gy + by;
-    const int t = (id & 7) * (total >> 3) + min(id & 7, total & 7) + (id >> 3);
-    const int band = t / (kBand * gy), q = t - band * kBand * gy, bh = min(kBand, gx - band * kBand);
-    by = q / bh;
-    bx = band * kBand + q - by * bh;
+    // Each XCD takes a contiguous range of tiles, in bands of 8 tile rows, so that those it runs together form a block of both
+    // operands (8000 x 8000 x 8096 of 8 and 8, 4 and 4 bits 1003, 642 -> 779, 496 us; up to 1024 tiles the divisions cost more:
+    // 300 x 2048 x 1536 of 8 and 4 bits 11.2 -> 11.6).
+    const int gx = gridDim.y, gy = gridDim.x;
+    banded_tile<8>(tile_on_xcd(bx * gy + by, gx * gy), gx, gy, bx, by);
   }
   const int n0 = by * 128;
   const int64_t m0 = (int64_t)bx * 128;

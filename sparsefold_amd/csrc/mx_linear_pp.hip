@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "index.h"
 #include "mx.h"
 #include "mx_linear.h"
 
@@ -124,19 +125,14 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
   const bool late = wave >= 4;                                // the second wave of each SIMD
-  // Workgroup b is assumed to run on XCD b % 8; each XCD takes a contiguous range of tiles, in bands of kBand tile rows, so
-  // that the tiles it runs together form a block of both operands.
-  constexpr int kBand = 5;
-  const int per = (total + 7) >> 3, xcd = blockIdx.x & 7, G8 = gridDim.x >> 3;
-  const int tend = min(total, (xcd + 1) * per);
-  int tile = xcd * per + (int)(blockIdx.x >> 3);
+  // Each XCD takes a contiguous range of tiles, in bands of 5 tile rows, so that the tiles it runs together form a block of both
+  // operands.
+  const int G8 = gridDim.x >> 3;
+  const TileWalk walk = tiles_on_xcd(blockIdx.x, total);
+  const int tend = walk.end;
+  int tile = walk.first;
   if (tile >= tend) return;                                   // uniform over the workgroup
-  const auto place = [&](int t, int& bx, int& by) __attribute__((always_inline)) {
-    const int band = t / (kBand * gy), q = t - band * kBand * gy;
-    const int bh = min(kBand, gx - band * kBand);
-    by = q / bh;
-    bx = band * kBand + q - by * bh;
-  };
+  const auto place = [&](int t, int& bx, int& by) __attribute__((always_inline)) { banded_tile<5>(t, gx, gy, bx, by); };
   // Rows past the end read the last row (their results are not stored).
   const auto sources = [&](int t, Copies& c) __attribute__((always_inline)) {
     int bx, by;
@@ -180,8 +176,7 @@ __global__ __launch_bounds__(512) void mx_linear_pp_kernel(const sf_mx_linear_ar
 
   const int n = a.K / (32 * SB);                              // >= A (host rule)
   const int blocks = a.K / 32, groups = (n + GS - 1) / GS;
-  // first block of a group's 16: the last group ends with the row
-  const auto group_at = [&](int g) __attribute__((always_inline)) { return min(16 * g, blocks - 16); };
+  const auto group_at = [&](int g) __attribute__((always_inline)) { return scales_of_group(g, blocks); };
   Copies c;
   sources(tile, c);
   __builtin_amdgcn_global_load_lds(c.s + c.so, (lds_u32*)(smem + S * STAGE + wave * 1024), 16, 0, 0);

@@ -25,6 +25,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "index.h"
 #include "sf_common.h"
 
 namespace {
@@ -111,18 +112,8 @@ __device__ __forceinline__ void rescale(const float (&m)[N], float mnew, float c
 }
 
 // Where a cache's rows are.  A page holds a multiple of 16 rows; units of 16 consecutive keys have one page each.
-struct PageDiv {                                             // i / n = (i m) >> s of units i < 2^27, n units a page
-  uint32_t m;
-  int s;
-};
-__host__ __device__ inline PageDiv page_div(uint32_t n) {
-  int up = 0;
-  while ((1u << up) < n) ++up;                               // s = 31 + ceil(log2 n), m = floor(2^s / n) + 1: exact while i < 2^31
-  return PageDiv{(uint32_t)((1ull << (31 + up)) / n + 1), 31 + up};
-}
-__device__ __forceinline__ int page_of(const PageDiv& p, uint32_t unit) { return (int)(((uint64_t)unit * p.m) >> p.s); }
 struct PagedArgs : sf_paged_attention_args {
-  PageDiv div;                                               // of a page's units
+  PageDiv div;                                               // of a page's units (units < 2^27)
 };
 
 // A launch dimension holds less than 2^32 threads: workgroups past kGridX (of up to 512) continue in the next row of the grid.
