@@ -525,8 +525,11 @@ __global__ __launch_bounds__(256) void mx_join_kernel(const sf_mx_linear_args a,
 // ---------------------------------------------------------------------------------------
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// From more rows of w on a workgroup takes 32 of them.
-constexpr int kWideRows = 6144;
+// With more rows of w than 16 a CU, a workgroup takes 32 of them: the second round of workgroups costs more than the wider ones (us with
+// 16 / 32 rows a workgroup, 4096 rows of w: 8 rows of x, K = 4096, 8 and 8 bits 6.6 / 8.1, 4 and 4 4.1 / 5.4; 32 rows 9.5 / 11.0, 5.8 / 7.2; K = 1024
+// 3.9 / 4.5; 5120 rows of w: 9.9 / 8.2, 6.1 / 5.5; 16.1 / 11.2, 9.4 / 7.4; K = 1024 5.7 / 4.6; 4112 rows and K = 8192 16.4 / 14.5, 32 rows 27.8 / 20.2, K = 512
+// as long; 12288 rows 13.8 / 15.3, 8.6 / 9.0; 24.6 / 21.7, 12.9 / 12.2; 16384 17.2 / 17.1, 10.3 / 9.1; 31.4 / 23.5, 16.2 / 12.3).  With 33 to 64 rows of x both take as long.
+constexpr int kWideRows = 4096;
 
 struct Route {
   bool stream, large;

@@ -25,8 +25,8 @@ def operand(rows, K, format, scaled, g):
   return ops.Microscaled(codes.to(DEV), s.to(DEV)), values
 
 
-# streamed, up to 32 and 64 rows; tiles of 128, whole steps and not, k in parts and not; tiles of 256, one a workgroup and more
-SHAPES = [(1, 16, 512), (8, 6200, 1184), (30, 300, 96), (60, 257, 2048), (65, 128, 128), (200, 1000, 1600), (100, 520, 4096), (777, 264, 2080), (1000, 700, 640),
+# streamed, up to 16, 32 and 64 rows, 16 and 32 rows of w a workgroup; tiles of 128, whole steps and not, k in parts and not; tiles of 256, one a workgroup and more
+SHAPES = [(1, 16, 512), (8, 6200, 1184), (30, 300, 96), (60, 257, 2048), (5, 4097, 544), (16, 4096, 1056), (17, 4113, 672), (30, 5000, 1184), (33, 4099, 512), (64, 7000, 96), (65, 128, 128), (200, 1000, 1600), (100, 520, 4096), (777, 264, 2080), (1000, 700, 640),
           (4230, 4200, 160), (2305, 4104, 1152), (4099, 4104, 640), (4099, 4104, 512), (2570, 4352, 768), (9000, 1032, 512)]
 
 
