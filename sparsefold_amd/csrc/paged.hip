@@ -62,8 +62,8 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int t) {
   return b;
 }
 
-// A wave takes as many rows as its lanes hold at 16 bytes each, or one row in turns.  Bound by latency (64 tokens of 8 heads of
-// 128 2.7 us) and, from some MB on, by memory (6959 tokens 10.8 us, 5.3 TB/s).
+// A wave takes one row, in turns where it has more than 64 pieces, or as many narrow ones as sf_hip_paged_write_fwd says.  Bound by
+// latency (64 tokens of 8 heads of 128 2.7 us) and, from some MB on, by memory (6959 tokens 10.8 us, 5.3 TB/s).
 __global__ __launch_bounds__(256) void paged_write_kernel(const sf_paged_write_args a, const int log_rows) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = a.D / 8, pieces = a.Hkv * per;              // 16-byte pieces of a row
@@ -130,9 +130,13 @@ extern "C" int sf_hip_paged_write_fwd(const sf_paged_write_args* a, void* stream
   }
   for (int i = 0; i < 2; ++i)
     if (a->k_s[i] % 8 || a->v_s[i] % 8) { sf_set_error("paged write: strides must be multiples of 8 elements"); return 1; }
-  const int pieces = a->Hkv * (a->D / 8);
+  // A row a wave up to 8192, which the chip runs at once: a wave's rows are found one after another.  Beyond, up to four that its lanes
+  // hold at 16 bytes each (us with 1 / 2 / 4 / up to 16 rows a wave: 64 tokens of 1 head of 32 3.0 / 3.4 / 4.5 / 11.2, 8192 5.3 / 5.0 / 5.4 / 11.6,
+  // 16384 8.0 / 7.4 / 7.5 / 11.8, 65536 25.4 / 22.1 / 21.0 / 22.9, 262144 93 / 77 / 70 / 69; of 128 64 tokens 2.8 / 3.3 / 4.5, 8192 5.5 / 5.3 / 5.8, 65536
+  // 26.5 / 22.9 / 21.5).
+  const int pieces = a->Hkv * (a->D / 8), most = a->T <= 8192 ? 0 : 2;
   int log_rows = 0;
-  while (log_rows < 4 && pieces << (log_rows + 1) <= 64) ++log_rows;
+  while (log_rows < most && pieces << (log_rows + 1) <= 64) ++log_rows;
   const int64_t rows = 4ll << log_rows, wgs = (a->T + rows - 1) / rows;          // (up to 2^28)
   const dim3 grid = wgs <= kGridX ? dim3((unsigned)wgs) : dim3(kGridX, (unsigned)((wgs + kGridX - 1) / kGridX));
   hipLaunchKernelGGL(paged_write_kernel, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream), *a, log_rows);

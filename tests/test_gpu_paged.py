@@ -366,3 +366,34 @@ def test_write_of_more_tokens_than_a_launch_dimension_holds():
     for cache, new in ((kc, k), (vc, v)):
       assert torch.equal(cache[i, :n], new[p * R:p * R + n]) and (cache[i, n:] == 3).all()
   assert (kc[-1] == 3).all() and (vc[-1] == 3).all()
+
+
+@pytest.mark.parametrize("heads,D,rows", [(1, 8, 16), (1, 32, 48), (3, 40, 16), (2, 64, 32), (5, 48, 16), (8, 64, 16)])
+@pytest.mark.parametrize("T", [8192, 8193, 30000])
+def test_write_of_narrow_rows(T, heads, D, rows):
+  """Numbers of tokens on both sides of where a wave takes several rows; sequences of no and of one new token among others, and
+  tokens without a place."""
+  g = torch.Generator().manual_seed(T + D)
+  cut = torch.sort(torch.randint(0, T + 1, (99,), generator=g)).values.tolist()
+  lens = [b - a for a, b in zip([0, *cut, cut[-1] + 1], [*cut, cut[-1] + 1, T])] if cut[-1] < T else [b - a for a, b in zip([0, *cut], [*cut, T])]
+  lens_k = [n + int(x) for n, x in zip(lens, torch.randint(0, 50, (len(lens),), generator=g))]
+  need = [-(-n // rows) for n in lens_k]
+  P, order = sum(need), torch.randperm(sum(need), generator=g).to(torch.int32)
+  table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+  at = 0
+  for b, n in enumerate(need):
+    table[b, :n] = order[at:at + n]
+    at += n
+  table[7, 0] = P                                              # (a page outside the cache)
+  k, v = (torch.randn(T, heads, D, generator=g).bfloat16() for _ in range(2))
+  kc, vc = (torch.zeros(P, rows, heads, D, dtype=torch.bfloat16) for _ in range(2))
+  b = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+  place = torch.tensor(lens_k)[b] - torch.tensor(lens)[b] + torch.arange(T) - torch.tensor([0, *lens]).cumsum(0)[b]
+  page = table[b, place // rows].long()
+  there = (page >= 0) & (page < P)
+  want = kc.clone(), vc.clone()
+  for w, new in zip(want, (k, v)):
+    w[page[there], (place % rows)[there]] = new[there]
+  kc, vc = kc.to(DEV), vc.to(DEV)
+  ops.paged_cache_write(k.to(DEV), v.to(DEV), kc, vc, table.to(DEV), offsets(lens), ints(lens_k))
+  assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1])
