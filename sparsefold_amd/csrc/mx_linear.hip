@@ -528,7 +528,8 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // With more rows of w than 16 a CU, a workgroup takes 32 of them: the second round of workgroups costs more than the wider ones (us with
 // 16 / 32 rows a workgroup, 4096 rows of w: 8 rows of x, K = 4096, 8 and 8 bits 6.6 / 8.1, 4 and 4 4.1 / 5.4; 32 rows 9.5 / 11.0, 5.8 / 7.2; K = 1024
 // 3.9 / 4.5; 5120 rows of w: 9.9 / 8.2, 6.1 / 5.5; 16.1 / 11.2, 9.4 / 7.4; K = 1024 5.7 / 4.6; 4112 rows and K = 8192 16.4 / 14.5, 32 rows 27.8 / 20.2, K = 512
-// as long; 12288 rows 13.8 / 15.3, 8.6 / 9.0; 24.6 / 21.7, 12.9 / 12.2; 16384 17.2 / 17.1, 10.3 / 9.1; 31.4 / 23.5, 16.2 / 12.3).  With 33 to 64 rows of x both take as long.
+// as long; 12288 rows 13.8 / 15.3, 8.6 / 9.0; 24.6 / 21.7, 12.9 / 12.2; 16384 17.2 / 17.1, 10.3 / 9.1; 31.4 / 23.5, 16.2 / 12.3; 64 rows, 5120
+// rows of w, K = 1024 9.7 / 6.9, 6.9 / 5.4).
 constexpr int kWideRows = 4096;
 
 struct Route {
@@ -567,10 +568,12 @@ double tile_cost(const sf_mx_linear_args* a, int steps, int slices) {
   return 4.0 + step * ((steps + slices - 1) / slices) + join;
 }
 
-// us of mx_stream_kernel with more than 32 rows: bound by the workgroups' loads of x (64 rows, 4096 x 4096 weights, 8 and 4 bits of x: 16.9
-// and 11.9; 12288 x 4096 38 and 25).
+// us of mx_stream_kernel with more than 32 rows: bound by the workgroups' loads of x, so by their rounds on the chip, wide ones a quarter
+// longer (64 rows, 8 and 4 bits of x, K = 4096: 4096 rows of w 16.9 and 11.9, 8192 20.6 and 14.3, 12288 38 and 25; K = 1024: 4096 6.3 and 5.2, 8192 7.3 and
+// 6.0, where tiles take 9.3 and 7.1).
 double stream_cost(const sf_mx_linear_args* a) {
-  return 3.0 + (a->x_format == SF_FORMAT_MXFP4 ? 9.0 : 13.5) * (a->K / 4096.0) * std::max(1.0, a->N / 4096.0);
+  const double rounds = a->N <= kWideRows ? 1.0 : 1.25 * ((a->N + 2 * kWideRows - 1) / (2 * kWideRows));
+  return 3.0 + (a->x_format == SF_FORMAT_MXFP4 ? 9.0 : 13.5) * (a->K / 4096.0) * rounds;
 }
 
 void route(const sf_mx_linear_args* a, Route& r) {
