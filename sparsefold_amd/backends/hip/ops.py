@@ -1096,7 +1096,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
   ``max_len``: the most keys that a sequence has (None: what the table holds).  The launch is chosen by it; a wrong one costs
   time, no result.  Offsets, lengths and table are read on the device only: the call can be captured.  What pages hold behind
-  a sequence's end has no influence; a page outside the cache counts as zeros."""
+  a sequence's end has no influence; a page outside the cache counts as zeros.
+
+  Logits, sums and results are fp32 up to their rounding; the weights are rounded to the type of ``q`` for the product with the values, and
+  the sum takes the rounded ones, as in ``packed_attention`` (errors up to 1.4 times those of 32-bit weights)."""
   if _front and out is None:
     result = _front.paged_attention(q, k_pages, v_pages, page_table, cu_q, len_k, len_q, causal, scale, max_len)
     if result is not None:

@@ -14,8 +14,10 @@
 // Results are rounded in registers, brought together to whole lines by exchanges between lanes, and stored by buffer stores
 // that drop what lies outside, so that their number, which the waits count, does not depend on the tile.
 //
-// 8192^3: 287 to 312 us of 4 bits, 3.5 to 3.8 PFLOP/s, by the card, and 489 of 8 bits, 2.25 (products of 8192^3 in bf16: 1.3; matrix instructions alone, on random codes in
-// registers: 6.8 and 3.8, clocks held by power).  With all codes zero 236 us of 4 bits and 425 of 8; of 4 bits without the copies 240.  4 waves of 128 x 128, one a
+// 8192^3: 287 to 315 us of 4 bits, 3.5 to 3.8 PFLOP/s, by the card, and 489 to 515 of 8 bits, 2.25 to 2.13 (products of 8192^3 in bf16: 1.3; matrix
+// instructions alone, on random codes in registers: 6.8 and 3.8, clocks held by power).  Over K from 512 to 8192 at 8192 x 8192 a tile takes 6 us
+// (9.6 of 8 and 8 bits) and 1.08 us a step of 128 k of 4 bits, 0.92 a step of 64 k of 8 and 8, 0.90 of 8 and 4: the step, not the tile's start
+// and end, is 90% of the time.  With all codes zero 236 us of 4 bits and 425 of 8; of 4 bits without the copies 240.  4 waves of 128 x 128, one a
 // SIMD, with the next step's reads between the products took as long (283 us, 285 with copies of whole 128-byte lines), so the two
 // groups' alternation is not what bounds it; L2 hits 90% of the lines asked for.
 #include <algorithm>
@@ -358,7 +360,8 @@ int launch_formats(const sf_mx_linear_args* a, hipStream_t st) {
 }  // namespace
 
 // What the kernel assumes: whole steps, at least four of them, 16 scales a row and words of them aligned, aligned rows, offsets inside a tile that fit 32 bits; and sizes
-// for which its tiles pay.
+// for which its tiles pay.  The rest takes tiles of 128 (8000 x 8000 x 8064, 8 and 8, 8 and 4, 4 and 4 bits: 505, 480, 302 us here; of
+// 8096 k 788, 652, 495; 8001 columns 660, 595, 456).
 bool sf_mx_linear_pp_ok(const sf_mx_linear_args* a) {
   if (a->K % 128 != 0 || a->K < 512 || a->N % 8 != 0 || a->M < kTile || a->N < kTile) return false;
   if (!al16(a->y) || a->y_rs % 8 != 0 || a->y_rs >= 1 << 22 || (a->bias && !al16(a->bias))) return false;

@@ -149,7 +149,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void add_rms_norm_kernel(con
   }
 }
 
-// Rows of any length and alignment, an element at a time.
+// Rows of any length and alignment, an element at a time, twice over the row.  Bound by the latency of its dependent steps (us beside the
+// kernel above: bf16 with residual, 8 rows of 4095 / 4096 11.6 / 4.0, 16384 291 / 104, 100000 of 99 / 96 98 / 46, 2048 of 16392 / 16384 126 / 51).
 template <class E>
 __global__ __launch_bounds__(256) void add_rms_norm_any_kernel(const sf_add_rms_norm_args a) {
   typedef typename E::T T;
