@@ -1198,6 +1198,11 @@ def _microscaled(x, name: str, what: str):
   return format, R, K, c2, (c2.stride(0) if R > 1 else cs[-1]), s2, (s2.stride(0) if R > 1 else ss[-1])
 
 
+def _resolved(t: torch.Tensor | None) -> torch.Tensor | None:
+  """t as its memory holds it: a view that is negated when read (the imaginary part of a lazily conjugated tensor) is copied."""
+  return t if t is None or not t.is_neg() else t.resolve_neg()
+
+
 def _empty_rows(lead, n: int, dtype: torch.dtype, dev) -> torch.Tensor:
   """``torch.empty((*lead, n))``, for a matrix in 3/5 of its host time."""
   if len(lead) == 1:
@@ -1240,7 +1245,7 @@ def mx_quantize(x: torch.Tensor, format: str = "mxfp4") -> Microscaled:
     raise ValueError(f"{what}: x must be bfloat16, float16 or float32, got {x.dtype}")
   if x.ndim < 1 or not 32 <= x.shape[-1] < 1 << 31 or x.shape[-1] % 32 != 0:
     raise ValueError(f"{what}: the last dim must be a multiple of 32 below 2^31, got {tuple(x.shape)}")
-  K = x.shape[-1]
+  x, K = _resolved(x), x.shape[-1]
   result = _empty_microscaled(x.shape[:-1], K, format, dev)
   if x.numel() == 0:
     return result
@@ -1297,6 +1302,7 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
   if bias is not None:
     if bias.shape != (N,):
       raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias.shape)}")
+    bias = _resolved(bias)
     if bias.dtype is not torch.float32 or not bias.is_contiguous():
       bias = _f32(bias)
   shape = (*x.codes.shape[:-1], N)
@@ -1307,6 +1313,8 @@ def mx_linear(x: Microscaled, w: Microscaled, bias: torch.Tensor | None = None, 
     y_rs = N
   else:
     dtype = out.dtype
+    if out.is_neg():
+      raise ValueError(f"{what}: out is a view that is negated when read")
     if out.shape != shape or dtype not in (torch.bfloat16, torch.float16) or (N > 1 and out.stride(-1) != 1):
       raise ValueError(f"{what}: out must be bfloat16 or float16 {shape} with a unit last stride, got {dtype} {tuple(out.shape)}")
     result = out
@@ -1354,6 +1362,8 @@ def _norm_outputs(what, shape, dtype, R, inputs, weight, aligned, outs):
   for o, name in zip(outs, ("out", "out_sum")):
     if o is None:
       continue
+    if o.is_neg():
+      raise ValueError(f"{what}: {name} is a view that is negated when read")
     if o.shape != shape or o.dtype is not dtype or (Cn > 1 and o.stride(-1) != 1):
       raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)} with a unit last stride")
     try:
@@ -1412,9 +1422,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
   if weight is not None:
     if weight.shape != (Cn,):
       raise ValueError(f"{what}: weight must be [{Cn}], got {tuple(weight.shape)}")
+    weight = _resolved(weight)
     if weight.dtype is not torch.float32 or not weight.is_contiguous():
       weight = _f32(weight)
-  aligned = output is not None
+  x, residual, aligned = _resolved(x), _resolved(residual), output is not None
   x2, x_rs = _rows2(x, aligned)
   R, x_p = x2.shape[0], x2.data_ptr()
   r2, r_p, r_rs = None, 0, 0

@@ -49,7 +49,7 @@ struct Call {
     const at::Tensor& t = THPVariable_Unpack(o);
     need(t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.has_storage());
     need(!t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
-                                                   c10::DispatchKey::FuncTorchGradWrapper})));
+                                                   c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Negative})));
     need(!(grad && t.requires_grad()) && !t._fw_grad(0).defined());
     if (device < 0) {
       device = t.get_device();
